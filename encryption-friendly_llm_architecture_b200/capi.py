@@ -142,6 +142,29 @@ class Lib:
         self._chk(self._fn("encode_ext")(self.ctx, _f64(re), _f64(im), C.c_size_t(re.size), C.c_int(level), C.byref(out)))
         return Handle(self, out, "pt")
 
+    def qweight(self, codes, scales, rows, group):
+        """A weight matrix in 4 bits: W[r][c] = (code - 8) * scales[r // group][c], two rows a byte (the even one in the low half).
+        codes: uint8 [ceil(rows / 2)][cols], scales: float32 [ceil(rows / group)][cols]."""
+        codes, scales = np.ascontiguousarray(codes), np.ascontiguousarray(scales)
+        if codes.dtype != np.uint8 or scales.dtype != np.float32 or codes.ndim != 2 or scales.ndim != 2:
+            raise ValueError("codes are a matrix of uint8, scales one of float32")
+        if rows < 1 or group < 1 or codes.shape[0] != (rows + 1) // 2 or scales.shape != ((rows + group - 1) // group, codes.shape[1]):
+            raise ValueError(f"{rows} rows in groups of {group}: codes {codes.shape}, scales {scales.shape}")
+        out = C.c_void_p()
+        self._chk(self._fn("qweight_create")(self.ctx, codes.ctypes.data_as(C.POINTER(C.c_uint8)), scales.ctypes.data_as(C.POINTER(C.c_float)), C.c_int(rows),
+                                             C.c_int(codes.shape[1]), C.c_int(group), C.byref(out)))
+        return Handle(self, out, "qweight")
+
+    def encode_q4(self, w, tile, first, count, level, diagonal=True):
+        """Plaintext operands of the blocks first .. first + count - 1 of a 4-bit weight matrix (K-groups of four row tiles innermost)."""
+        out = (C.c_void_p * max(0, count))()
+        self._chk(self._fn("encode_q4")(self.ctx, w.ptr, C.c_int(tile), C.c_int(1 if diagonal else 0), C.c_int(first), C.c_int(count), C.c_int(level), out))
+        return [Handle(self, C.c_void_p(p), "pt") for p in out]
+
+    def matvec_q4(self, x, w, tile):
+        """Encrypted vectors (their K-groups innermost in the batch) times a 4-bit weight matrix, un-rescaled."""
+        return self._op("matvec_q4", x.ptr, w.ptr, C.c_int(tile))
+
     def decode(self, pt):
         re = np.zeros(self.slots); im = np.zeros(self.slots)
         self._chk(self._fn("decode")(self.ctx, pt.ptr, _f64(re), _f64(im)))
@@ -360,6 +383,32 @@ class Lib:
     def mul(self, a, b): return self._op("mul", a.ptr, b.ptr)
     def rotate(self, a, s): return self._op("rotate", a.ptr, C.c_int64(s))
     def conjugate(self, a): return self._op("conjugate", a.ptr)
+
+    def tensor_acc_cross(self, a, b, groups, heads=1, acc=None):
+        """out[j][h][i] = sum_g tensor(a[g][h][i], b[g][h][j]); with `acc` the sum goes there, and `acc` comes back."""
+        out = C.c_void_p(acc.ptr.value if acc is not None else None)
+        self._chk(self._fn("tensor_acc_cross")(self.ctx, a.ptr, b.ptr, C.c_int(groups), C.c_int(heads), C.byref(out)))
+        return acc if acc is not None else Handle(self, out, "ct")
+
+    def matmul_acc_grouped(self, pre, inputs, sizes, pts, row_step, order=None):
+        """Products grouped by expert: pts[e][t][b], the first sizes[0] positions at expert 0 and so on, position p with input order[p]
+        (None: p); member p * tiles + t of the result.  pts[e] may be None where sizes[e] is 0."""
+        sizes = [int(n) for n in sizes]
+        there = [rows for rows, n in zip(pts, sizes) if n]
+        if len(pts) != len(sizes) or not there:
+            raise ValueError("one list of weights per expert, and an expert with inputs")
+        tiles, bcount = len(there[0]), len(there[0][0])
+        if any(len(rows) != tiles or any(len(row) != bcount for row in rows) for rows in there):
+            raise ValueError("experts with other numbers of tiles or K-groups")
+        if order is not None and len(order) != sum(sizes):
+            raise ValueError(f"{sum(sizes)} positions, an order of {len(order)}")
+        arr = (C.c_void_p * (len(sizes) * tiles * bcount))()
+        for e, (rows, n) in enumerate(zip(pts, sizes)):
+            if n:
+                arr[e * tiles * bcount:(e + 1) * tiles * bcount] = [p.ptr.value for row in rows for p in row]
+        which = None if order is None else (C.c_int32 * len(order))(*[int(i) for i in order])
+        return self._op("matmul_acc_grouped", pre.ptr, C.c_int(inputs), which, (C.c_int32 * len(sizes))(*sizes), C.c_int(len(sizes)), arr, C.c_int(bcount), C.c_int(tiles),
+                        C.c_int64(row_step))
 
     def rotate_sum(self, xs, steps):
         """sum_t rot(xs[t], steps[t]) with one ModDown for the whole sum."""

@@ -5,11 +5,14 @@
 #include "../../include/hemmer_b200.h"
 #include "host_ctx.hpp"
 #include "kernels.cuh"
+#include "pairs.cuh"
+#include "experts.cuh"
 #include "ntt.cuh"
 #include "convcols.cuh"
 #include "convmma.cuh"
 #include "ksrows.cuh"
 #include "embed.cuh"
+#include "weights4.cuh"
 #include "host_threads.hpp"
 #include "launch_rules.hpp"
 #include "pool.hpp"
@@ -111,7 +114,7 @@ struct hb_ctx {
     int N = 0, logn = 0, L = 0, K = 0, nprimes = 0;
     unsigned long long launches = 0; // kernels launched by this context
     int *dev_err = nullptr;          // raised by a kernel whose bounded wait ran out; read by hb_sync
-    bool smem_opt_in_parts = false; // the opt-in to more than 48 KB of shared memory is per kernel and per device: once per context
+    bool smem_opt_in_experts[2][4] = {}, smem_opt_in_parts = false; // the opt-in to more than 48 KB of shared memory is per kernel and per device: once per context
     // Compulsory HBM traffic of the primitives called so far, in limbs of N words: every input of a primitive read once,
     // every output written once, a switching key or plaintext once per batch (temporaries and transforms inside a
     // primitive do not count).  Divided by the HBM peak this is the time the call sequence cannot go below.
@@ -133,6 +136,8 @@ struct hb_pt { hb_ctx *ctx; int level, spow; u64 *d; int ext = 0; }; // ext: K f
 struct hb_digits { hb_ctx *ctx; int level, batch; u64 *d; };
 // a switching key multiplied by a plaintext mask, restricted to one level: key [nd][2][ne][N], pm = P * mask on the Q limbs [n][N]
 struct hb_mkey { hb_ctx *ctx; int level; u32 g; u64 *key, *pm; };
+// a weight matrix in 4 bits, as it came from the caller: codes, and behind them (at a multiple of four) the scales
+struct hb_qweight { hb_ctx *ctx; Weights4 w; unsigned char *d; };
 
 namespace {
 
@@ -981,6 +986,114 @@ void launch_matmul_tiles(hb_ctx *c, const hb_ct *pre, int btotal, int b0, const 
     acc_opt_in(c);
     LAUNCH(c), k_matmul_acc<T><<<dim3((unsigned)(c->N / 256), (unsigned)n), 256, acc_smem(T), c->st>>>(tp, pre->d, kc, btotal, b0, bcount, dg, n, c->qmap(pre->level), c->pc, c->logn, c->N);
 }
+// ---- products grouped by expert ----
+template <int M, int T> void launch_experts(hb_ctx *c, const ExpertList &el, const hb_ct *pre, u64 *out, int copies, int inputs, const u32 *gal) {
+    const int n = pre->level + 1;
+    constexpr size_t smem = expert_smem<M, T>();
+    if (!c->smem_opt_in_experts[M - 1][T - 1]) {
+        CK(cudaFuncSetAttribute(k_matmul_experts<M, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        c->smem_opt_in_experts[M - 1][T - 1] = true;
+    }
+    LAUNCH(c), k_matmul_experts<M, T><<<dim3((unsigned)(c->N / 256) * (unsigned)el.first_block[el.experts], (unsigned)n), 256, smem, c->st>>>(out, el, pre->d, copies, inputs, gal, n, c->qmap(pre->level),
+                                                                                                                                            c->pc, c->logn, c->N);
+    CK(cudaGetLastError());
+}
+hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts, const hb_pt *const *pts, int bcount, int tiles, i64 row_step) {
+    if (!pre || !sizes || !pts) fail(HB_E_ARG, "matmul_acc_grouped: null argument");
+    own(c, pre);
+    if (pre->np != 2 || pre->spow != 1) fail(HB_E_SHAPE, "matmul_acc_grouped: operands");
+    if (inputs < 1 || experts < 1 || tiles < 1 || bcount < 1 || bcount > 16) fail(HB_E_SHAPE, "matmul_acc_grouped: inputs, experts, tiles from 1, K-groups 1 to 16");
+    if (pre->batch % ((i64)inputs * bcount)) fail(HB_E_SHAPE, "matmul_acc_grouped: the copies do not split into that many inputs");
+    if (c->N % 256) fail(HB_E_LIMIT, "matmul_acc_grouped: ring degree below 256");
+    i64 positions = 0, used = 0;
+    for (int e = 0; e < experts; ++e) {
+        if (sizes[e] < 0) fail(HB_E_SHAPE, "matmul_acc_grouped: a group of negative size");
+        positions += sizes[e]; used += sizes[e] > 0;
+        for (i64 k = 0; sizes[e] && k < (i64)tiles * bcount; ++k) {
+            const hb_pt *p = pts[(i64)e * tiles * bcount + k];
+            if (!p) fail(HB_E_ARG, "matmul_acc_grouped: null plaintext of an expert that has inputs");
+            own(c, p);
+            if (p->level != pre->level) fail(HB_E_LEVEL, "matmul_acc_grouped: plaintext level differs from the ciphertexts'");
+            if (p->spow != 1) fail(HB_E_SHAPE, "matmul_acc_grouped: operands");
+        }
+    }
+    if (!positions) fail(HB_E_SHAPE, "matmul_acc_grouped: no expert has an input");
+    if (!order && positions > inputs) fail(HB_E_SHAPE, "matmul_acc_grouped: more positions than inputs, and no order");
+    if (positions * tiles > INT32_MAX / 64) fail(HB_E_LIMIT, "matmul_acc_grouped: too many results");
+    for (i64 p = 0; order && p < positions; ++p) if (order[p] < 0 || order[p] >= inputs) fail(HB_E_ARG, "matmul_acc_grouped: an input that is not there");
+    const int n = pre->level + 1, copies = pre->batch / (inputs * bcount);
+    const u32 *gal = galois_table(c, copies, row_step);
+    hb_ct *r = new_ct(c, pre->level, 2, (int)(positions * tiles), 2);
+    try {
+        ALG(c, pre->limbs() + (size_t)used * tiles * bcount * n + (size_t)positions * tiles * 2 * n);
+        const int at_once = std::min(tiles, kExpertPts / bcount); // tiles of a launch
+        for (int tile0 = 0; tile0 < tiles; tile0 += at_once) {
+            const int tn = std::min(at_once, tiles - tile0), T = (tn + (tn + 3) / 4 - 1) / ((tn + 3) / 4); // even blocks of at most four
+            ExpertList el;
+            i64 next = 0; // the first position that no launch has yet
+            int largest = 0;
+            auto begin = [&] { el.experts = 0; el.tiles = tn; el.bcount = bcount; el.out_tiles = tiles; el.tile0 = tile0; el.first_pos[0] = 0; el.pos0 = (int)next; largest = 0; };
+            auto flush = [&] {
+                if (!el.experts) return;
+                const int M = largest > 1 ? 2 : 1;
+                el.first_block[0] = 0;
+                for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + M - 1) / M * ((tn + T - 1) / T);
+                auto go = [&](auto m) {
+                    constexpr int MM = decltype(m)::value;
+                    switch (T) {
+                    case 1: launch_experts<MM, 1>(c, el, pre, r->d, copies, inputs, gal); break;
+                    case 2: launch_experts<MM, 2>(c, el, pre, r->d, copies, inputs, gal); break;
+                    case 3: launch_experts<MM, 3>(c, el, pre, r->d, copies, inputs, gal); break;
+                    default: launch_experts<MM, 4>(c, el, pre, r->d, copies, inputs, gal);
+                    }
+                };
+                if (M == 2) go(std::integral_constant<int, 2>{}); else go(std::integral_constant<int, 1>{});
+            };
+            begin();
+            for (int e = 0; e < experts; ++e)
+                for (int left = sizes[e]; left > 0;) {
+                    if (el.experts == kExpertGroups || (el.experts + 1) * tn * bcount > kExpertPts || el.first_pos[el.experts] == kExpertPositions) { flush(); begin(); }
+                    const int at = el.first_pos[el.experts], take = std::min(left, kExpertPositions - at);
+                    for (int t = 0; t < tn * bcount; ++t) el.w[el.experts * tn * bcount + t] = pts[((i64)e * tiles + tile0) * bcount + t]->d;
+                    for (int k = 0; k < take; ++k) el.input[at + k] = order ? order[next + k] : (int)(next + k);
+                    el.first_pos[++el.experts] = at + take;
+                    largest = std::max(largest, take);
+                    next += take; left -= take;
+                }
+            flush();
+        }
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
+// ---- tensor products of all pairs of tiles ----
+template <int QI, int KJ> void launch_pairs(hb_ctx *c, const hb_ct *a, const hb_ct *b, hb_ct *r, const PairShape &s, bool accumulate) {
+    const int n = a->level + 1, blocks = ((s.nq + QI - 1) / QI) * ((s.nk + KJ - 1) / KJ);
+    launch(c, k_tensor_pairs<QI, KJ>, dim3((unsigned)(c->N / 256) * (unsigned)blocks, (unsigned)(s.heads * n)), 256, 0, r->d, (const u64 *)a->d, (const u64 *)b->d, s, n, c->qmap(a->level), c->pc, c->N,
+           accumulate ? 1 : 0);
+}
+// acc[j][h][i] (+)= sum_g tensor(a[g][h][i], b[g][h][j])
+hb_ct *do_tensor_pairs(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, int heads, hb_ct *acc) {
+    if (!a || !b) fail(HB_E_ARG, "tensor_acc_cross: null argument");
+    own(c, a, b, acc);
+    if (a->level != b->level) fail(HB_E_LEVEL, "tensor_acc_cross: level mismatch");
+    if (a->np != 2 || a->spow != 1 || b->np != 2 || b->spow != 1) fail(HB_E_SHAPE, "tensor_acc_cross: operands must be rescaled 2-poly ciphertexts");
+    if (groups < 1 || heads < 1 || a->batch % ((i64)groups * heads) || b->batch % ((i64)groups * heads)) fail(HB_E_SHAPE, "tensor_acc_cross: a batch does not split into that many groups and heads");
+    const PairShape s{groups, heads, a->batch / (groups * heads), b->batch / (groups * heads)};
+    const int n = a->level + 1;
+    const i64 members = (i64)s.nq * s.nk * heads;
+    if (members > INT32_MAX / 64 || (i64)heads * n > 65535) fail(HB_E_LIMIT, "tensor_acc_cross: too many heads or pairs");
+    hb_ct *r = acc;
+    if (r) { if (r->level != a->level || r->np != 3 || r->batch != members || r->spow != 2) fail(HB_E_SHAPE, "tensor_acc_cross: accumulator mismatch"); }
+    else r = new_ct(c, a->level, 3, (int)members, 2);
+    ALG(c, a->limbs() + b->limbs() + (size_t)(acc ? 2 : 1) * r->limbs());
+    try {
+        if (s.nq == 1 && s.nk == 1) launch_pairs<1, 1>(c, a, b, r, s, acc != nullptr);
+        else if (s.nq == 1) launch_pairs<1, 2>(c, a, b, r, s, acc != nullptr);
+        else if (s.nk == 1) launch_pairs<2, 1>(c, a, b, r, s, acc != nullptr);
+        else launch_pairs<2, 2>(c, a, b, r, s, acc != nullptr);
+    } catch (...) { if (!acc) hb_ct_free(r); throw; }
+    return r;
+}
 hb_ct *do_level_down(hb_ctx *c, const hb_ct *a, int target) {
     own(c, a);
     if (target > a->level || target < 0) fail(HB_E_LEVEL, "level_down: bad target");
@@ -1134,6 +1247,24 @@ void embed_inverse(hb_ctx *c, i64 *coef, const double *re, const double *im, int
         CK(cudaPeekAtLastError());
     }
 }
+// ---- plaintext operands from 4-bit weights ----
+struct Tiles4 { int kb, nb; }; // K-groups of four row tiles, column tiles
+Tiles4 tiles4(const hb_ctx *c, const hb_qweight *w, int d) {
+    if (d < 1 || (i64)2 * d * d > c->h->slots) fail(HB_E_SHAPE, "4-bit weights: two tiles of that side do not fit the slots");
+    return {(int)((w->w.rows + (i64)4 * d - 1) / ((i64)4 * d)), (int)((w->w.cols + (i64)d - 1) / d)};
+}
+// residues out [count][level + 1][N] of the blocks first .. first + count - 1, transform order
+void encode_blocks4(hb_ctx *c, const hb_qweight *w, int d, int kb, bool diagonal, int first, int count, int level, u64 *out) {
+    const int slots = c->h->slots;
+    TmpBytes v(c, (size_t)count * slots * 16), coef(c, (size_t)count * c->N * 8);
+    double *re = (double *)v.p, *im = re + (size_t)count * slots;
+    launch(c, k_weight_slots, dim3((unsigned)((slots + 255) / 256), (unsigned)count), 256, 0, re, im, w->w, Blocks4{first, kb, d, diagonal ? 1 : 0}, slots);
+    embed_inverse(c, (i64 *)coef.p, re, im, slots, count, c->h->scale[level]);
+    const LimbMap qm = c->qmap(level);
+    message_residues(c, out, (const i64 *)coef.p, count, qm);
+    ntt_inplace(c, out, count * (level + 1), qm, false);
+}
+constexpr int kBlocks4 = 32; // blocks encoded at a time
 // slot values of the residues t [count][2][N]: member b, slot s at re[(b * slots + s) * stride], im likewise
 void embed_forward(hb_ctx *c, double *re, double *im, int stride, const u64 *t, const DecItem *items, int count) {
     if (c->logn == 16) {
@@ -1534,6 +1665,77 @@ int hb_encode_ext(hb_ctx *c, const double *re, const double *im, size_t n, int l
         *out = p;
     });
 }
+int hb_qweight_create(hb_ctx *c, const uint8_t *codes, const float *scales, int rows, int cols, int group, hb_qweight **out) {
+    return guard(c, [&] {
+        no_capture(c, "qweight_create");
+        if (!codes || !scales || !out) fail(HB_E_ARG, "qweight: null argument");
+        if (rows < 1 || cols < 1 || group < 1) fail(HB_E_SHAPE, "qweight: rows, columns and group from 1");
+        const size_t bytes = ((size_t)rows + 1) / 2 * cols, at = (bytes + 3) & ~(size_t)3, words = (((size_t)rows - 1) / group + 1) * cols;
+        for (size_t k = 0; k < words; ++k) if (!std::isfinite(scales[k])) fail(HB_E_ARG, "qweight: a scale is not finite");
+        std::unique_ptr<hb_qweight> w(new hb_qweight{c, {}, nullptr});
+        w->d = (unsigned char *)c->pool.get(at + words * 4);
+        w->w = Weights4{w->d, (const float *)(w->d + at), rows, cols, group};
+        try {
+            CK(cudaMemcpyAsync(w->d, codes, bytes, cudaMemcpyHostToDevice, c->st));
+            CK(cudaMemcpyAsync(w->d + at, scales, words * 4, cudaMemcpyHostToDevice, c->st));
+            CK(cudaStreamSynchronize(c->st)); // codes and scales are the caller's memory
+        } catch (...) { c->pool.put(w->d); throw; }
+        *out = w.release();
+    });
+}
+void hb_qweight_free(hb_qweight *w) { if (w) { w->ctx->pool.put(w->d); delete w; } }
+int hb_qweight_meta(const hb_qweight *w, int *rows, int *cols, int *group) {
+    if (!w) return HB_E_ARG;
+    if (rows) *rows = w->w.rows;
+    if (cols) *cols = w->w.cols;
+    if (group) *group = w->w.group;
+    return HB_OK;
+}
+int hb_encode_q4(hb_ctx *c, const hb_qweight *w, int tile, int diagonal, int first, int count, int level, hb_pt **out) {
+    return guard(c, [&] {
+        if (!w || !out) fail(HB_E_ARG, "encode_q4: null argument");
+        own(c, w);
+        if (level < 0 || level > c->L) fail(HB_E_LEVEL, "encode_q4: bad level");
+        const Tiles4 t = tiles4(c, w, tile);
+        if (first < 0 || count < 1 || (i64)first + count > (i64)t.kb * t.nb) fail(HB_E_ARG, "encode_q4: blocks that are not there");
+        std::vector<hb_pt *> r((size_t)count, nullptr);
+        const size_t words = (size_t)(level + 1) * c->N;
+        try {
+            for (hb_pt *&p : r) p = new_pt(c, level, 1);
+            ALG(c, (size_t)count * (level + 1));
+            for (int k = 0; k < count; k += kBlocks4) {
+                const int m = std::min(kBlocks4, count - k);
+                Tmp t4(c, (size_t)m * (level + 1));
+                encode_blocks4(c, w, tile, t.kb, diagonal != 0, first + k, m, level, t4.p);
+                for (int i = 0; i < m; ++i) CK(cudaMemcpyAsync(r[(size_t)(k + i)]->d, t4.p + i * words, words * 8, cudaMemcpyDeviceToDevice, c->st));
+            }
+        } catch (...) { for (hb_pt *p : r) hb_pt_free(p); throw; }
+        std::copy(r.begin(), r.end(), out);
+    });
+}
+int hb_matvec_q4(hb_ctx *c, const hb_ct *x, const hb_qweight *w, int tile, hb_ct **out) {
+    return guard(c, [&] {
+        if (!x || !w || !out) fail(HB_E_ARG, "matvec_q4: null argument");
+        own(c, x); own(c, w);
+        if (x->np != 2 || x->spow != 1) fail(HB_E_SHAPE, "matvec_q4: operands must be rescaled 2-poly ciphertexts");
+        const Tiles4 t = tiles4(c, w, tile);
+        if (x->batch % t.kb) fail(HB_E_SHAPE, "matvec_q4: the batch is no whole number of vectors");
+        const int vectors = x->batch / t.kb, n = x->level + 1;
+        if ((i64)vectors * t.nb > INT32_MAX / 64 || (i64)vectors * std::min(t.nb, kBlocks4) > 65535) fail(HB_E_LIMIT, "matvec_q4: too many results");
+        hb_ct *r = new_ct(c, x->level, 2, vectors * t.nb, 2);
+        try {
+            ALG(c, x->limbs() + r->limbs());
+            const int columns = std::max(1, kBlocks4 / t.kb);
+            for (int j = 0; j < t.nb; j += columns) {
+                const int m = std::min(columns, t.nb - j);
+                Tmp p(c, (size_t)m * t.kb * n);
+                encode_blocks4(c, w, tile, t.kb, false, j * t.kb, m * t.kb, x->level, p.p);
+                launch(c, k_matvec, dim3((unsigned)(c->N / 256), (unsigned)n, (unsigned)(vectors * m)), 256, 0, r->d, (const u64 *)x->d, (const u64 *)p.p, t.kb, m, t.nb, j, n, c->qmap(x->level), c->pc, c->N);
+            }
+        } catch (...) { hb_ct_free(r); throw; }
+        *out = r;
+    });
+}
 int hb_decode(hb_ctx *c, const hb_pt *p, double *re, double *im) {
     return guard(c, [&] {
         no_capture(c, "decode");
@@ -1635,6 +1837,7 @@ int hb_pt_export(hb_ctx *c, const hb_pt *x, uint64_t *host) {
     return guard(c, [&] { no_capture(c, "pt_export"); own(c, x); CK(cudaMemcpyAsync(host, x->d, (size_t)(x->level + 1) * c->N * 8, cudaMemcpyDeviceToHost, c->st)); CK(cudaStreamSynchronize(c->st)); });
 }
 void *hb_ct_device_ptr(const hb_ct *x) { return x ? x->d : nullptr; }
+void *hb_pt_device_ptr(const hb_pt *x) { return x ? x->d : nullptr; }
 int hb_batch_set(hb_ctx *c, hb_ct *dst, int idx, const hb_ct *src) {
     return guard(c, [&] {
         own(c, dst, src);
@@ -1909,6 +2112,12 @@ int hb_assemble_masked_into(hb_ctx *c, const hb_ct *a, const hb_digits *dg, cons
     });
 }
 int hb_tensor_acc_groups(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, hb_ct **acc) { return guard(c, [&] { *acc = do_tensor(c, a, b, *acc, groups); }); }
+int hb_tensor_acc_cross(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, int heads, hb_ct **acc) {
+    return guard(c, [&] {
+        if (!acc) fail(HB_E_ARG, "tensor_acc_cross: null argument");
+        *acc = do_tensor_pairs(c, a, b, groups, heads, *acc);
+    });
+}
 // sum_t rot(xs[t], steps[t]): every term is decomposed, the inner products of all terms are added up in Q_level u P by
 // one kernel, and one ModDown serves the sum; unrotated terms (step 0) are added as they are.
 // sum_t rot(x_t, steps[t]) with one ModDown; x_t = `batch` members starting at base[t] (all of one shape)
@@ -2098,6 +2307,12 @@ int hb_matmul_acc_tiles(hb_ctx *c, const hb_ct *pre, int btotal, int b0, const h
             CK(cudaGetLastError());
         } catch (...) { for (hb_ct *r : rs) if (r) hb_ct_free(r); throw; }
         for (int t = 0; t < tiles; ++t) out[t] = rs[(size_t)t];
+    });
+}
+int hb_matmul_acc_grouped(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts, const hb_pt *const *pts, int bcount, int tiles, int64_t row_step, hb_ct **out) {
+    return guard(c, [&] {
+        if (!out) fail(HB_E_ARG, "matmul_acc_grouped: null argument");
+        *out = do_matmul_experts(c, pre, inputs, order, sizes, experts, pts, bcount, tiles, row_step);
     });
 }
 int hb_matmul_acc(hb_ctx *c, const hb_ct *pre, const hb_pt *pt, int64_t row_step, hb_ct **out) { return hb_matmul_acc_multi(c, pre, 1, 0, &pt, 1, row_step, out); }

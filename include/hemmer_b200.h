@@ -29,6 +29,7 @@ typedef struct hb_ct hb_ct;
 typedef struct hb_pt hb_pt;
 typedef struct hb_digits hb_digits;
 typedef struct hb_mkey hb_mkey;
+typedef struct hb_qweight hb_qweight;
 
 enum {
     HB_OK = 0,
@@ -98,6 +99,23 @@ int hb_decode(hb_ctx *ctx, const hb_pt *pt, double *re, double *im);
 /* hb_encode with K further limbs modulo the special primes after the level + 1 usual ones: the plaintext operand of
  * hb_assemble_rot.  Usable wherever a plaintext of that level is.  No counterpart in the reference. */
 int hb_encode_ext(hb_ctx *ctx, const double *re, const double *im, size_t n_slots, int level, hb_pt **out);
+/* Weights in 4 bits with a scale per group of rows, kept as they are on the device: W[r][c] = (code - 8) * scale[r / group][c].
+ * codes: [ceil(rows / 2)][cols] bytes, row 2k in the low half of byte row k, row 2k + 1 in the high half; scales:
+ * [ceil(rows / group)][cols] floats, all finite (HB_E_ARG otherwise); any group from 1, the last one may be shorter.  Half a byte a
+ * weight, where an encoded plaintext holds 16 (level + 1).  No counterpart in the reference. */
+int hb_qweight_create(hb_ctx *ctx, const uint8_t *codes, const float *scales, int rows, int cols, int group, hb_qweight **out);
+void hb_qweight_free(hb_qweight *w);
+int hb_qweight_meta(const hb_qweight *w, int *rows, int *cols, int *group);
+/* Plaintext operands of such a matrix, made on the device: out[0 .. count) receives the blocks first .. first + count - 1.  With tiles of
+ * side `tile` (two of them fit the slots) block (j, b), b < kb = ceil(rows / (4 tile)), is number j * kb + b and holds the rows 4 tile b ..
+ * of the columns tile j .., zeros outside: 1/2 (W1 - i W3) | 1/2 (W2 - i W4) of its four row tiles, row-major over 2 tile columns.
+ * diagonal: every column c of a tile rolled up by c (HEMMer::msgDiagonalToRow4, the operand of hb_matmul_acc*); without it the operand
+ * of hb_matvec_q4.  Bit for bit hb_encode of those slot values.  Nothing is copied from the host, so the call can be recorded. */
+int hb_encode_q4(hb_ctx *ctx, const hb_qweight *w, int tile, int diagonal, int first, int count, int level, hb_pt **out);
+/* Encrypted vectors times such a matrix, the operands made on the way: out[v * nb + j] = sum over b < kb of x[v * kb + b] (.) block (j, b)
+ * (not diagonal), un-rescaled; nb = ceil(cols / tile).  x: a whole number of vectors of kb members each.  Vectors spread over the
+ * columns give y by a sum over the rows (hb_hemmer_matvec_q4). */
+int hb_matvec_q4(hb_ctx *ctx, const hb_ct *x, const hb_qweight *w, int tile, hb_ct **out);
 /* Encryptor::encrypt(ptxt, sk, ctxt) -- Encryptor.hpp:84; `nonce` selects the random streams */
 int hb_encrypt(hb_ctx *ctx, const hb_pt *pt, uint64_t nonce, hb_ct **out);
 /* encode + encrypt `count` messages (message i at re + i * n_slots, im likewise or NULL) into ONE handle of batch
@@ -130,6 +148,7 @@ int hb_ct_import(hb_ctx *ctx, hb_ct *ct, const uint64_t *host);
 int hb_ct_export(hb_ctx *ctx, const hb_ct *ct, uint64_t *host);
 int hb_pt_export(hb_ctx *ctx, const hb_pt *pt, uint64_t *host);
 void *hb_ct_device_ptr(const hb_ct *ct);
+void *hb_pt_device_ptr(const hb_pt *pt);
 /* Files.  HEaaN's binary format is not published, so these calls write and read this library's own container:
  * a 96-byte header (magic, kind, ring degree, level, polynomial count, batch, scale power, a hash of the primes),
  * the plain residues in device layout, and a checksum.  A file is accepted only under the parameters it was
@@ -260,6 +279,10 @@ int hb_tensor_acc(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, hb_ct **acc);
 /* *acc (+)= sum over g < groups of tensor(a[g], b[g]); a and b hold groups * batch members (group-major), *acc holds
  * batch members (NULL: created).  Same residues as `groups` calls of hb_tensor_acc. */
 int hb_tensor_acc_groups(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, int groups, hb_ct **acc);
+/* All pairs of tiles of a head: *acc[j][h][i] (+)= sum over g < groups of tensor(a[g][h][i], b[g][h][j]).  a holds groups * heads * nq
+ * members in that order, b groups * heads * nk, of one level; *acc (NULL: created) nk * heads * nq, the key tile outermost, so that scores
+ * can be the left operand of a product with the values.  Pair by pair the residues of hb_tensor_acc_groups. */
+int hb_tensor_acc_cross(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, int groups, int heads, hb_ct **acc);
 /* acc += tensor(first half of the members of x, second half); *acc may be NULL on entry */
 int hb_tensor_acc_halves(hb_ctx *ctx, const hb_ct *x, hb_ct **acc);
 /* out = sum_k pre[k] (.) rot_rows(pt, k * row_step), un-rescaled -- HomEvaluator::matmul :595-601 */
@@ -272,6 +295,13 @@ int hb_matmul_acc_multi(hb_ctx *ctx, const hb_ct *pre, int btotal, int b0, const
  * out[t] = sum over b of matmul(copies of input b0 + b, pts[t * bcount + b]); the copies are read once per four tiles. */
 int hb_matmul_acc_tiles(hb_ctx *ctx, const hb_ct *pre, int btotal, int b0, const hb_pt *const *pts, int bcount, int tiles, int64_t row_step,
                         hb_ct **out);
+/* Products grouped by expert: position p belongs to the expert whose run of sizes[e] positions (0 allowed) it lies in and takes input
+ * order[p] (NULL: input p; an input may be at several positions), and
+ *     out[p * tiles + t] = sum over b < bcount of matmul(copies of K-group b of input order[p], pts[(e * tiles + t) * bcount + b]).
+ * pre: copy k of K-group b of input i at batch position (k * inputs + i) * bcount + b; at most 16 K-groups.  The plaintexts of an expert
+ * without positions are not looked at (NULL allowed).  Position by position the residues of hb_matmul_acc_multi. */
+int hb_matmul_acc_grouped(hb_ctx *ctx, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts, const hb_pt *const *pts, int bcount,
+                          int tiles, int64_t row_step, hb_ct **out);
 /* rotation of a plaintext (pure slot permutation, no key) -- leftRotate(ptxt) used at MatrixUtils.cpp:1503 */
 int hb_pt_rotate(hb_ctx *ctx, const hb_pt *p, int64_t left_steps, hb_pt **out);
 /* mult(ptxt, ptxt) with rescale and add(ptxt, ptxt), as multMatMat<Plaintext> uses them -- MatrixUtils.cpp:1556-1558 */
