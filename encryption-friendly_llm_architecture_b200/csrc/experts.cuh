@@ -1,15 +1,17 @@
 // Ciphertext x plaintext products grouped by expert (sm_100a).
 //
 //     out[p][t] = sum_b sum_k pre[k][order[p]][b] (.) perm_{g_k}(w[e][t][b]),   e = the expert whose group position p lies in
-// with groups of any size: k_matmul_acc for several inputs that share weights.  A thread works on one coefficient of both polynomials of M positions and T
-// output tiles: a weight word is read (and converted) once for M positions, a copy word once for T tiles.  The blocks of one coefficient range, over
-// all experts, run side by side, so that copies and weights come from L2 for all but the first of them.
+// with groups of any size: what k_matmul_acc does, for several inputs that share weights.  A lane has one residue of both polynomials of M positions and of T
+// output tiles: 2 M + T words a product step for 2 M T products.  The words come through a ring of stages in shared memory that belongs to the warp alone, by
+// 16-byte asynchronous copies a few steps ahead: lines of 32 residues, of rotated weights the line that holds the residues wanted (a rotation permutes aligned
+// runs of 32 as units, and within them), from which every lane reads its own.  The blocks of one range of residues, over all experts, run side by side, so that
+// copies and weights come from L2 for all but the first of them.
 #pragma once
-#include "kernels.cuh"
+#include "pieces.cuh"
 
 namespace hb {
 
-// What one launch works on: experts with their positions and weight words' addresses.  An argument, so that calls can be recorded and nothing is uploaded.
+// What one launch works on: experts with their positions and their weights' addresses.  An argument, so that calls can be recorded and nothing is uploaded.
 constexpr int kExpertPts = 384, kExpertGroups = 64, kExpertPositions = 256;
 struct ExpertList {
     int experts, tiles, bcount;               // tiles: of this launch; w[(e * tiles + t) * bcount + b]
@@ -20,129 +22,136 @@ struct ExpertList {
     int pos0;                                 // member positions before this launch's first
     int input[kExpertPositions];              // which input a position has
 };
-template <int T> constexpr int kExpertRing = T >= 3 ? 6 : 8;
-template <int M, int T> constexpr size_t expert_smem() { return (size_t)kExpertRing<T> * (2 * M + T) * 256 * 8; }
-// pre [copies][inputs][bcount][2][n][N].  grid = (N / 256 * blocks, n)
+// CTAs of four warps that an SM holds: their registers have the sums
+template <int M, int T> constexpr int kExpertCtas = M * T > 8 ? 2 : M * T > 3 ? 3 : 4;
+constexpr int kExpertRing = 4;
+template <int M, int T> constexpr size_t expert_smem() { return (size_t)4 * kExpertRing * (2 * M + T) * 256; }
+// pre [copies][inputs][bcount][2][n][N].  Four warps side by side, 32 residues each.  grid = (N / 128 * blocks, n)
 template <int M, int T>
-__global__ void __launch_bounds__(256, 2) k_matmul_experts(u64 *out, const __grid_constant__ ExpertList el, const u64 *__restrict__ pre, int copies, int inputs, const u32 *__restrict__ gal, int n,
-                                                           const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, int logn, int N) {
+__global__ void __launch_bounds__(128, kExpertCtas<M, T>) k_matmul_experts(u64 *out, const __grid_constant__ ExpertList el, const u64 *__restrict__ pre, int copies, int inputs, const u32 *__restrict__ gal,
+                                                                           int n, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, int logn, int N) {
     extern __shared__ __align__(16) u64 words[];
-    constexpr int kRing = kExpertRing<T>;
-    const int blocks = el.first_block[el.experts], blk = blockIdx.x % blocks, l = blockIdx.y;
+    __shared__ const u64 *weights[T * 16];
+    constexpr int S = kExpertRing;
+    const int blocks = el.first_block[el.experts], blk = blockIdx.x % blocks, l = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int e = 0;
     while (blk >= el.first_block[e + 1]) ++e;
     const int tile_blocks = (el.tiles + T - 1) / T, in_e = blk - el.first_block[e];
     const int t0 = in_e % tile_blocks * T, p0 = el.first_pos[e] + in_e / tile_blocks * M, pn = min(M, el.first_pos[e + 1] - p0), tn = min(T, el.tiles - t0);
     const PrimeConst m = pc[map.prime[l]];
     const size_t poly = (size_t)n * N, limb = (size_t)l * N;
-    const u32 x0 = blockIdx.x / blocks * 256 + threadIdx.x;
-    const u64 *ring = words + threadIdx.x;
-    const u32 ring_at = smem_u32(ring);
+    const u32 x0 = blockIdx.x / blocks * 128 + warp * 32, x = x0 + lane;
+    u64 *const ring = words + warp * (S * (2 * M + T) * 32);
     const int bcount = el.bcount, total = copies * bcount;
-    const u64 *const *w = el.w + (size_t)(e * el.tiles) * bcount;
-    u64 *const o = out + ((size_t)(el.pos0 + p0) * el.out_tiles + el.tile0 + t0) * 2 * poly + limb + x0;
+    u64 *const o = out + ((size_t)(el.pos0 + p0) * el.out_tiles + el.tile0 + t0) * 2 * poly + limb + x;
+    const int half = lane >> 4, part = (lane & 15) * 2; // a lane copies two residues of one of two lines
+    if (threadIdx.x < T * bcount) weights[threadIdx.x] = el.w[(e * el.tiles + min(t0 + (int)threadIdx.x / bcount, el.tiles - 1)) * bcount + threadIdx.x % bcount] + limb; // [tile][K-group]
+    __syncthreads();
 
-    // positions p .. p + MM - 1 of the block; past the end: the last one again, not stored
-    auto body = [&](auto mm, int p, auto acc) {
-        constexpr int MM = decltype(mm)::value, kStage = (2 * MM + T) * 256;
-        using Acc = decltype(acc);
-        const u64 *fa[MM];
+    // Positions p .. p + MM - 1 and tiles q .. q + TT - 1 of the block; tiles past the end: the last one again, not stored.  The products of a sum: all copies of one
+    // K-group, then the next.
+    auto body = [&](auto mm, auto tt, int p, int q, auto kind) {
+        constexpr int MM = decltype(mm)::value, TT = decltype(tt)::value, kStage = (2 * MM + TT) * 32, kLoads = (TT + 1) / 2;
+        using Sums = decltype(kind);
+        const u64 *from[MM], *w[kLoads]; // both polynomials of a position and two tiles: one copy each
+        auto weights_of = [&](int b) {
 #pragma unroll
-        for (int i = 0; i < MM; ++i) fa[i] = pre + (size_t)el.input[p0 + min(p + i, pn - 1)] * bcount * 2 * poly + limb + x0;
-        const size_t to_next_copy = (size_t)(inputs * bcount - bcount + 1) * 2 * poly;
-        int fk = 0, fb = 0;
-        u32 to = 0, g = __ldg(gal), src = g == 1 ? x0 : ntt_perm(x0, g, logn);
-        auto fetch = [&] {
-            const u32 r = ring_at + to;
+            for (int t = 0; t < kLoads; ++t) w[t] = weights[min(q + 2 * t + half, T - 1) * bcount + b] + part;
+        };
 #pragma unroll
-            for (int i = 0; i < MM; ++i) { cp_async8(r + i * 4096, fa[i]); cp_async8(r + i * 4096 + 2048, fa[i] + poly); }
+        for (int i = 0; i < MM; ++i) from[i] = pre + ((size_t)el.input[p0 + p + i] * bcount * 2 + half) * poly + limb + x0 + part;
+        weights_of(0);
+        const i64 to_next = (i64)inputs * bcount * 2 * poly, to_group = (i64)2 * poly - (copies - 1) * to_next;
+        const u32 ring_at = smem_u32(ring) + lane * 16, ex0 = 2 * (__brev(x0) >> (32 - logn)) + 1, ex = 2 * (__brev(x) >> (32 - logn)) + 1, mask = (2u << logn) - 1;
+        auto turned = [&](u32 exponent, u32 g) { return __brev((g * exponent & mask) >> 1) >> (32 - logn); }; // ntt_perm of the residue with that exponent
+        int fk = 0, fb = 0, rk = 0;
+        u32 f_g = __ldg(gal), r_g = f_g; // of the copy that is fetched next, and of the one whose products come next
+        auto fetch = [&](int stage) {
+            const u32 to = ring_at + stage * (kStage * 8), line = turned(ex0, f_g) & ~31u;
+            const bool last = ++fk == copies;
+            if (last) fk = 0;
+            f_g = __ldg(gal + fk);
 #pragma unroll
-            for (int t = 0; t < T; ++t) cp_async8(r + (2 * MM + t) * 2048, w[min(t0 + t, el.tiles - 1) * bcount + fb] + limb + src);
+            for (int i = 0; i < MM; ++i) { cp_async16(to + i * 512, from[i]); from[i] += last ? to_group : to_next; }
+#pragma unroll
+            for (int t = 0; t < kLoads; ++t)
+                if (2 * t + 1 < TT || !half) cp_async16(to + MM * 512 + t * 512, w[t] + line);
+            if (last && ++fb < bcount) weights_of(fb);
+        };
+        __syncwarp(); // the ring may still be read from a body before
+#pragma unroll
+        for (int k = 0; k < S - 1; ++k) {
+            if (k < total) fetch(k);
             cp_async_commit();
-            if (++fb < bcount) {
-#pragma unroll
-                for (int i = 0; i < MM; ++i) fa[i] += 2 * poly;
-            } else if (fk + 1 < copies) {
-                fb = 0; ++fk;
-#pragma unroll
-                for (int i = 0; i < MM; ++i) fa[i] += to_next_copy;
-                g = __ldg(gal + fk);
-                src = g == 1 ? x0 : ntt_perm(x0, g, logn);
-            }
-            to += kStage * 8;
-            if (to == kRing * kStage * 8) to = 0;
-        };
-#pragma unroll 1
-        for (int k = 0; k < kRing - 1; ++k) {
-            if (k < total) fetch();
-            else cp_async_commit();
         }
-        Acc s[MM][T][2];
+        Sums s[MM][TT][2];
+        auto each = [&](auto &&f) { // every sum, with its position, tile and polynomial
 #pragma unroll
-        for (int i = 0; i < MM; ++i)
+            for (int i = 0; i < MM; ++i)
 #pragma unroll
-            for (int t = 0; t < T; ++t) { s[i][t][0].zero(); s[i][t][1].zero(); }
-        constexpr bool FP = std::is_same<Acc, FpAcc>::value;
-        const double qd = (double)m.q;
-        const int room = !FP ? 8 : m.q < (1ull << 42) ? 128 : 8;
-        int held = 0, from = 0;
-        auto term = [&](auto &&then) {
-            cp_async_wait<kRing - 2>();
-            const u64 *q = ring + from;
-            u64 v[MM][2], wv[T];
+                for (int t = 0; t < TT; ++t)
 #pragma unroll
-            for (int i = 0; i < MM; ++i) { v[i][0] = q[i * 512]; v[i][1] = q[i * 512 + 256]; }
+                    for (int k = 0; k < 2; ++k) f(s[i][t][k], i, t, k);
+        };
+        each([](Sums &sum, int, int, int) { sum.zero(); });
+        int left = total - (S - 1); // steps that are still to be fetched
+        auto step = [&](int stage) { // always a constant
+            cp_async_wait<S - 2>();
+            __syncwarp();
+            const u64 *at = ring + stage * kStage;
+            const u32 place = turned(ex, r_g) & 31u; // of this lane's residue in a line of weights
+            u64 v[MM][2], wv[TT];
 #pragma unroll
-            for (int t = 0; t < T; ++t) wv[t] = q[(2 * MM + t) * 256];
-            from += kStage;
-            if (from == kRing * kStage) from = 0;
-            then();
-            if (++held > room) {
-                held = 1;
+            for (int t = 0; t < TT; ++t) wv[t] = at[MM * 64 + t * 32 + place];
 #pragma unroll
-                for (int i = 0; i < MM; ++i)
+            for (int i = 0; i < MM; ++i) { v[i][0] = at[i * 64 + lane]; v[i][1] = at[i * 64 + 32 + lane]; }
+            if (left-- > 0) fetch((stage + S - 1) % S); // into the stage of a step ago
+            cp_async_commit();
+            if (++rk == copies) rk = 0;
+            r_g = __ldg(gal + rk);
+            typename Sums::Factor f[MM][2];
 #pragma unroll
-                    for (int t = 0; t < T; ++t)
+            for (int i = 0; i < MM; ++i) { f[i][0] = Sums::factor(v[i][0]); f[i][1] = Sums::factor(v[i][1]); }
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) s[i][t][k].relax(m);
-            }
-            if constexpr (FP) {
-                double vd[MM][2];
+            for (int t = 0; t < TT; ++t) {
+                const typename Sums::Factor fw = Sums::factor(wv[t]);
 #pragma unroll
-                for (int i = 0; i < MM; ++i) { vd[i][0] = u52_to_double(v[i][0]); vd[i][1] = u52_to_double(v[i][1]); }
-#pragma unroll
-                for (int t = 0; t < T; ++t) {
-                    const double wd = u52_to_double(wv[t]);
-#pragma unroll
-                    for (int i = 0; i < MM; ++i) { s[i][t][0].mac(vd[i][0], wd); s[i][t][1].mac(vd[i][1], wd); }
-                }
-            } else {
-#pragma unroll
-                for (int t = 0; t < T; ++t)
-#pragma unroll
-                    for (int i = 0; i < MM; ++i) { s[i][t][0].mac(v[i][0], wv[t]); s[i][t][1].mac(v[i][1], wv[t]); }
+                for (int i = 0; i < MM; ++i) { s[i][t][0].mac(f[i][0], fw); s[i][t][1].mac(f[i][1], fw); }
             }
         };
-        const int fetching = max(0, total - (kRing - 1));
-#pragma unroll 2
-        for (int k = 0; k < fetching; ++k) term(fetch);
+        const int room = Sums::room(m);
+        auto relax = [&](int done) { if (done && done % room == 0) each([&](Sums &sum, int, int, int) { sum.relax(m); }); };
+        int done = 0;
 #pragma unroll 1
-        for (int k = fetching; k < total; ++k) term([] { cp_async_commit(); });
+        for (; done + S <= total; done += S) { // as many steps as stages: the stages are constants, and FP64 sums may change registers
+            relax(done);
 #pragma unroll
-        for (int i = 0; i < MM; ++i)
+            for (int k = 0; k < S; ++k) step(k);
+        }
+        if (done < total) relax(done);
 #pragma unroll
-            for (int t = 0; t < T; ++t)
-                if (p + i < pn && t < tn) {
-                    u64 *z = o + ((size_t)(p + i) * el.out_tiles + t) * 2 * poly;
-                    if constexpr (FP) { z[0] = s[i][t][0].finish(m.q_inv_f, qd); z[poly] = s[i][t][1].finish(m.q_inv_f, qd); }
-                    else { z[0] = s[i][t][0].finish(m); z[poly] = s[i][t][1].finish(m); }
-                }
+        for (int k = 0; k < S - 1; ++k) if (done + k < total) step(k);
+        each([&](Sums &sum, int i, int t, int k) {
+            if (q + t < tn) o[((size_t)(p + i) * el.out_tiles + q + t) * 2 * poly + k * poly] = sum.finish(m);
+        });
     };
-    if (m.fp) body(std::integral_constant<int, M>{}, 0, FpAcc{});
-    else
-        for (int p = 0; p < pn; ++p) { // the accumulators of one position fill the registers
-            body(std::integral_constant<int, 1>{}, p, PieceAcc{});
+    // as many positions as there are; modulo long primes as many sums at once as find room in the registers
+    constexpr std::integral_constant<int, 1> one{};
+    constexpr std::integral_constant<int, (M > 1 ? 2 : 1)> two{};
+    if (m.fp) {
+        constexpr std::integral_constant<int, T> all{};
+        if (pn == M) body(std::integral_constant<int, M>{}, all, 0, 0, WholeSums{});
+        else if (M > 2 && pn == 2) body(two, all, 0, 0, WholeSums{});
+        else body(one, all, 0, 0, WholeSums{});
+    } else {
+        constexpr int TT = T > 4 ? T / 2 : T;
+        constexpr std::integral_constant<int, TT> some{};
+        for (int q = 0; q < T; q += TT) {
+            int p = 0;
+            if constexpr (kExpertCtas<M, T> == 2) for (; p + 1 < pn; p += 2) body(two, some, p, q, PieceSums{});
+            for (; p < pn; ++p) body(one, some, p, q, PieceSums{});
         }
+    }
 }
 
 } // namespace hb

@@ -114,7 +114,7 @@ struct hb_ctx {
     int N = 0, logn = 0, L = 0, K = 0, nprimes = 0;
     unsigned long long launches = 0; // kernels launched by this context
     int *dev_err = nullptr;          // raised by a kernel whose bounded wait ran out; read by hb_sync
-    bool smem_opt_in_experts[2][4] = {}, smem_opt_in_parts = false; // the opt-in to more than 48 KB of shared memory is per kernel and per device: once per context
+    bool smem_opt_in_experts[3][8] = {}, smem_opt_in_pairs[6] = {}, smem_opt_in_parts = false; // the opt-in to more than 48 KB of shared memory is per kernel and per device: once per context
     // Compulsory HBM traffic of the primitives called so far, in limbs of N words: every input of a primitive read once,
     // every output written once, a switching key or plaintext once per batch (temporaries and transforms inside a
     // primitive do not count).  Divided by the HBM peak this is the time the call sequence cannot go below.
@@ -994,7 +994,7 @@ template <int M, int T> void launch_experts(hb_ctx *c, const ExpertList &el, con
         CK(cudaFuncSetAttribute(k_matmul_experts<M, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
         c->smem_opt_in_experts[M - 1][T - 1] = true;
     }
-    LAUNCH(c), k_matmul_experts<M, T><<<dim3((unsigned)(c->N / 256) * (unsigned)el.first_block[el.experts], (unsigned)n), 256, smem, c->st>>>(out, el, pre->d, copies, inputs, gal, n, c->qmap(pre->level),
+    LAUNCH(c), k_matmul_experts<M, T><<<dim3((unsigned)(c->N / 128) * (unsigned)el.first_block[el.experts], (unsigned)n), 128, smem, c->st>>>(out, el, pre->d, copies, inputs, gal, n, c->qmap(pre->level),
                                                                                                                                             c->pc, c->logn, c->N);
     CK(cudaGetLastError());
 }
@@ -1028,26 +1028,28 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
         ALG(c, pre->limbs() + (size_t)used * tiles * bcount * n + (size_t)positions * tiles * 2 * n);
         const int at_once = std::min(tiles, kExpertPts / bcount); // tiles of a launch
         for (int tile0 = 0; tile0 < tiles; tile0 += at_once) {
-            const int tn = std::min(at_once, tiles - tile0), T = (tn + (tn + 3) / 4 - 1) / ((tn + 3) / 4); // even blocks of at most four
+            const int tn = std::min(at_once, tiles - tile0);
             ExpertList el;
             i64 next = 0; // the first position that no launch has yet
-            int largest = 0;
-            auto begin = [&] { el.experts = 0; el.tiles = tn; el.bcount = bcount; el.out_tiles = tiles; el.tile0 = tile0; el.first_pos[0] = 0; el.pos0 = (int)next; largest = 0; };
+            auto begin = [&] { el.experts = 0; el.tiles = tn; el.bcount = bcount; el.out_tiles = tiles; el.tile0 = tile0; el.first_pos[0] = 0; el.pos0 = (int)next; };
             auto flush = [&] {
                 if (!el.experts) return;
-                const int M = largest > 1 ? 2 : 1;
+                const int M = expert_positions(el.experts, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; }), T = expert_tiles(M, tn);
                 el.first_block[0] = 0;
                 for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + M - 1) / M * ((tn + T - 1) / T);
-                auto go = [&](auto m) {
+                auto go = [&](auto m, auto t) { launch_experts<decltype(m)::value, decltype(t)::value>(c, el, pre, r->d, copies, inputs, gal); };
+                auto by_tiles = [&](auto m) {
                     constexpr int MM = decltype(m)::value;
                     switch (T) {
-                    case 1: launch_experts<MM, 1>(c, el, pre, r->d, copies, inputs, gal); break;
-                    case 2: launch_experts<MM, 2>(c, el, pre, r->d, copies, inputs, gal); break;
-                    case 3: launch_experts<MM, 3>(c, el, pre, r->d, copies, inputs, gal); break;
-                    default: launch_experts<MM, 4>(c, el, pre, r->d, copies, inputs, gal);
+                    case 1: go(m, std::integral_constant<int, 1>{}); break;
+                    case 2: go(m, std::integral_constant<int, 2>{}); break;
+                    case 3: go(m, std::integral_constant<int, 3>{}); break;
+                    case 4: go(m, std::integral_constant<int, 4>{}); break;
+                    case 6: if constexpr (MM < 3) go(m, std::integral_constant<int, 6>{}); break;
+                    default: if constexpr (MM < 2) go(m, std::integral_constant<int, 8>{});
                     }
                 };
-                if (M == 2) go(std::integral_constant<int, 2>{}); else go(std::integral_constant<int, 1>{});
+                if (M == 1) by_tiles(std::integral_constant<int, 1>{}); else if (M == 2) by_tiles(std::integral_constant<int, 2>{}); else by_tiles(std::integral_constant<int, 3>{});
             };
             begin();
             for (int e = 0; e < experts; ++e)
@@ -1057,7 +1059,6 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
                     for (int t = 0; t < tn * bcount; ++t) el.w[el.experts * tn * bcount + t] = pts[((i64)e * tiles + tile0) * bcount + t]->d;
                     for (int k = 0; k < take; ++k) el.input[at + k] = order ? order[next + k] : (int)(next + k);
                     el.first_pos[++el.experts] = at + take;
-                    largest = std::max(largest, take);
                     next += take; left -= take;
                 }
             flush();
@@ -1066,9 +1067,16 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
     return r;
 }
 // ---- tensor products of all pairs of tiles ----
-template <int QI, int KJ> void launch_pairs(hb_ctx *c, const hb_ct *a, const hb_ct *b, hb_ct *r, const PairShape &s, bool accumulate) {
-    const int n = a->level + 1, blocks = ((s.nq + QI - 1) / QI) * ((s.nk + KJ - 1) / KJ);
-    launch(c, k_tensor_pairs<QI, KJ>, dim3((unsigned)(c->N / 256) * (unsigned)blocks, (unsigned)(s.heads * n)), 256, 0, r->d, (const u64 *)a->d, (const u64 *)b->d, s, n, c->qmap(a->level), c->pc, c->N,
+template <int TR, int TC, int LR, int LC> void launch_pairs(hb_ctx *c, int variant, u64 *d, const PairSides &sides, const PairShape &s, int level, bool accumulate) {
+    using T = PairTile<TR, TC, LR, LC>;
+    if (!c->smem_opt_in_pairs[variant]) {
+        CK(cudaFuncSetAttribute(k_tensor_pairs<TR, TC, LR, LC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
+        c->smem_opt_in_pairs[variant] = true;
+    }
+    const int n = level + 1, blocks = ((sides.nr + T::kRows - 1) / T::kRows) * ((sides.nc + T::kCols - 1) / T::kCols);
+    int run = 1; // ranges of a CTA: more of them, and the ring runs dry less often; but every SM wants several CTAs
+    while (run < 16 && c->N / (16 * T::kX * run) >= 1 && (i64)c->N / (16 * T::kX * run) * blocks * s.heads * n >= 148 * 8) run *= 2;
+    launch(c, k_tensor_pairs<TR, TC, LR, LC>, dim3((unsigned)(c->N / (8 * T::kX * run)) * (unsigned)blocks, (unsigned)(s.heads * n)), 256, T::kSmem, d, sides, s, run, n, c->qmap(level), c->pc, c->N,
            accumulate ? 1 : 0);
 }
 // acc[j][h][i] (+)= sum_g tensor(a[g][h][i], b[g][h][j])
@@ -1087,10 +1095,18 @@ hb_ct *do_tensor_pairs(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, in
     else r = new_ct(c, a->level, 3, (int)members, 2);
     ALG(c, a->limbs() + b->limbs() + (size_t)(acc ? 2 : 1) * r->limbs());
     try {
-        if (s.nq == 1 && s.nk == 1) launch_pairs<1, 1>(c, a, b, r, s, acc != nullptr);
-        else if (s.nq == 1) launch_pairs<1, 2>(c, a, b, r, s, acc != nullptr);
-        else if (s.nk == 1) launch_pairs<2, 1>(c, a, b, r, s, acc != nullptr);
-        else launch_pairs<2, 2>(c, a, b, r, s, acc != nullptr);
+        const bool keys = s.nk > s.nq;
+        const PairSides sides{keys ? b->d : a->d, keys ? a->d : b->d, std::max(s.nq, s.nk), std::min(s.nq, s.nk), keys ? 1 : 0};
+        const int rows = sides.nr > 2 ? 4 : sides.nr, cols = sides.nc > 2 ? 4 : sides.nc;
+        auto go = [&](auto tr, auto tc, auto lr, auto lc, int variant) {
+            launch_pairs<decltype(tr)::value, decltype(tc)::value, decltype(lr)::value, decltype(lc)::value>(c, variant, r->d, sides, s, a->level, acc != nullptr);
+        };
+        constexpr std::integral_constant<int, 1> one{};
+        constexpr std::integral_constant<int, 2> two{};
+        constexpr std::integral_constant<int, 4> four{};
+        if (cols == 1) { if (rows == 1) go(one, one, one, one, 0); else if (rows == 2) go(two, one, one, one, 1); else go(four, one, one, one, 2); }
+        else if (cols == 2) { if (rows == 2) go(two, two, one, one, 3); else go(two, two, two, one, 4); }
+        else go(two, two, two, two, 5);
     } catch (...) { if (!acc) hb_ct_free(r); throw; }
     return r;
 }

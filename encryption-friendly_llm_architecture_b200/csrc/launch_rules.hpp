@@ -91,4 +91,21 @@ constexpr int streamed_polynomials(int terms, int parts) {
     return line > 10 ? line : 10;
 }
 
+// Products grouped by expert: positions (M) and output tiles (T) of a block.  A lane keeps 2 M T sums, and a block of fewer positions than M does their work alone,
+// but in the registers of M.
+constexpr int expert_tiles(int M, int tiles) { // even blocks of at most eight, six or four tiles; there are none of five and seven
+    const int most = M == 1 ? 8 : M == 2 ? 6 : 4, blocks = (tiles + most - 1) / most, t = (tiles + blocks - 1) / blocks;
+    return t == 5 || t == 7 ? t + 1 : t;
+}
+template <class SIZE> constexpr int expert_positions(int experts, SIZE &&size) {
+    long cost[4] = {};
+    for (int e = 0; e < experts; ++e)
+        for (int M = 1; M <= 3; ++M) {
+            const int n = size(e), rest = n % M;
+            const int whole[4] = {0, 100, 165, 228}, part[4][3] = {{}, {}, {0, 108, 0}, {0, 115, 190}};
+            cost[M] += (long)(n / M) * whole[M] + part[M][rest];
+        }
+    return cost[3] < cost[2] && cost[3] < cost[1] ? 3 : cost[2] < cost[1] ? 2 : 1;
+}
+
 } // namespace hb

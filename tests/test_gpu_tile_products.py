@@ -108,6 +108,33 @@ def test_cross_full_ring(gpu_full, level, groups, heads, nq, nk):
             assert np.array_equal(got[(j * heads + h) * nq + i], single[h])
 
 
+OTHER_PRIMES = [dict(log_n=10, max_level=4, dnum=3, q_bits=43), dict(log_n=10, max_level=4, dnum=3, q_bits=44), dict(log_n=10, max_level=4, dnum=3, q_bits=46, p_bits=58),
+                dict(log_n=11, max_level=4, dnum=3, q_bits=59), dict(log_n=16, max_level=3, dnum=3, q_bits=44), dict(log_n=16, max_level=3, dnum=3, q0_bits=58, q_bits=50, p_bits=58)]
+
+
+@pytest.mark.parametrize("prm", OTHER_PRIMES)
+def test_other_primes(pkg, prm):
+    """Primes of 43 and 44 bits, whose sums have less room, and longer ones; the largest residues and uniform ones."""
+    g = pkg.open_gpu(pkg.make_params(num_special=3, hamming_weight=32, **prm))
+    try:
+        rng = np.random.default_rng(1)
+        at = np.unique(np.concatenate([[0, g.N - 1], rng.integers(0, g.N, 10)]))
+        for edge in (False, True):
+            for groups, nq, nk in ((1, 1, 1), (3, 2, 1), (9, 4, 3), (17, 1, 4), (34, 2, 2)):
+                a, b = _rand(g, 3, groups * nq, 3, edge=edge), _rand(g, 3, groups * nk, 4, edge=edge)
+                _same(g.ct_export(g.tensor_acc_cross(_ct(g, a), _ct(g, b), groups)), _cross_expected(a, b, groups, 1, g.primes, at), at)
+            for copies, bcount, sizes, tiles in ((9, 1, [1], 8), (17, 1, [3, 1], 4), (9, 2, [2], 6)):
+                pre, pts = _rand(g, 3, copies * 3 * bcount, 5, edge=edge), _weights(g, 3, len(sizes), tiles, bcount, 6)
+                if edge:
+                    pts[:] = np.array([int(q) - 1 for q in g.primes[:4]], dtype=U64)[None, None, None, :, None]
+                order = list(range(sum(sizes)))
+                order = [i % 3 for i in order]
+                got = g.ct_export(g.matmul_acc_grouped(_ct(g, pre), 3, sizes, _handles(g, pts, sizes), 2, order=order))
+                _same(got, _grouped_expected(g, pre, pts, copies, 3, sizes, order, 2, at), at)
+    finally:
+        g.close()
+
+
 def test_cross_accumulates(gpu_small):
     """*acc += sum: in two halves the same as at once; the accumulator's handle stays the caller's."""
     g = gpu_small
@@ -194,6 +221,7 @@ GROUPED = [  # copies, inputs, bcount, sizes, order, tiles
     (16, 2, 3, [1, 2], [1, 0, 1], 6),
     (3, 2, 16, [1, 1], None, 2),                       # the most K-groups
     (2, 5, 1, [0, 0, 0, 0, 1], [4], 7),
+    (6, 2, 1, [1, 1], None, 8), (6, 2, 1, [1, 1], None, 5), (7, 3, 2, [3], None, 6), (5, 3, 1, [6, 1, 3], [0, 1, 2, 0, 1, 2, 2, 1, 1, 0], 9), (3, 4, 1, [4], None, 12),
 ]
 
 
