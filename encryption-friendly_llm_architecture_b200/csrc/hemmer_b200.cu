@@ -1264,23 +1264,43 @@ void embed_inverse(hb_ctx *c, i64 *coef, const double *re, const double *im, int
     }
 }
 // ---- plaintext operands from 4-bit weights ----
+constexpr size_t kMatvecBytes = (size_t)48 << 20;
 struct Tiles4 { int kb, nb; }; // K-groups of four row tiles, column tiles
 Tiles4 tiles4(const hb_ctx *c, const hb_qweight *w, int d) {
     if (d < 1 || (i64)2 * d * d > c->h->slots) fail(HB_E_SHAPE, "4-bit weights: two tiles of that side do not fit the slots");
     return {(int)((w->w.rows + (i64)4 * d - 1) / ((i64)4 * d)), (int)((w->w.cols + (i64)d - 1) / d)};
 }
-// residues out [count][level + 1][N] of the blocks first .. first + count - 1, transform order
-void encode_blocks4(hb_ctx *c, const hb_qweight *w, int d, int kb, bool diagonal, int first, int count, int level, u64 *out) {
-    const int slots = c->h->slots;
-    TmpBytes v(c, (size_t)count * slots * 16), coef(c, (size_t)count * c->N * 8);
-    double *re = (double *)v.p, *im = re + (size_t)count * slots;
-    launch(c, k_weight_slots, dim3((unsigned)((slots + 255) / 256), (unsigned)count), 256, 0, re, im, w->w, Blocks4{first, kb, d, diagonal ? 1 : 0}, slots);
-    embed_inverse(c, (i64 *)coef.p, re, im, slots, count, c->h->scale[level]);
-    const LimbMap qm = c->qmap(level);
-    message_residues(c, out, (const i64 *)coef.p, count, qm);
-    ntt_inplace(c, out, count * (level + 1), qm, false);
+Blocks4 blocks4(const hb_qweight *w, int d, int kb, bool diagonal, int first) {
+    const u64 two32 = (u64)1 << 32, per = 2 * (u64)d, group = (u64)w->w.group;
+    return Blocks4{first, kb, d, diagonal ? 1 : 0, (u32)((two32 + per - 1) / per), group < 2 * per ? (two32 + group - 1) / group : 0};
 }
-constexpr int kBlocks4 = 32; // blocks encoded at a time
+// coef [count][N] = rounded coefficients of the blocks first .. first + count - 1
+void coefficients4(hb_ctx *c, const hb_qweight *w, const Blocks4 &b, int count, int level, i64 *coef) {
+    const double sc = c->h->scale[level];
+    if (c->logn == 16) {
+        Tmp v(c, (size_t)count);
+        launch(c, k_weight_cols, dim3(16, (unsigned)count), kEmbThreads, 0, (double2 *)v.p, w->w, b, c->emb_tb);
+        launch(c, k_embed_inv_rows, dim3(16, (unsigned)count), kEmbThreads, 0, coef, (const double2 *)v.p, sc, c->emb_tb);
+    } else launch(c, k_weight_small, dim3((unsigned)count), 256, 0, coef, w->w, b, c->logn - 1, sc, c->emb_tb);
+}
+// residues of the limbs l0 .. l0 + limbs - 1, transform order, as those limbs of the members of `to`
+void transform4(hb_ctx *c, const PtList &to, const i64 *coef, int count, int l0, int limbs) {
+    LimbMap map{};
+    map.n = limbs;
+    for (int i = 0; i < limbs; ++i) map.prime[i] = (unsigned char)(l0 + i);
+    if (c->logn != 16) { launch(c, k_coef_small, dim3((unsigned)limbs, (unsigned)count), 256, sizeof(u64) << c->logn, to, l0, coef, map, c->pc, c->tb, c->logn); return; }
+    PtList rows = to;
+    for (int i = 0; i < count; ++i) rows.p[i] += (size_t)l0 * c->N;
+    auto passes = [&](auto *cols, auto *second) {
+        launch(c, cols, dim3(16, (unsigned)(count * limbs)), 256, 0, to, l0, coef, map, c->pc, c->tb.t16);
+        launch(c, second, dim3(16, (unsigned)(count * limbs)), 256, 0, (const u64 *)nullptr, rows, (u64 *)nullptr, rows, map, c->pc, c->tb.t16);
+    };
+    if (c->tb.t16.pm) passes(k_coef_cols<LongPm>, ntt16v2_fwd_rows<4, LongPm, PtList>);
+    else passes(k_coef_cols<LongShoup>, ntt16v2_fwd_rows<4, LongShoup, PtList>);
+}
+template <int V, int C> void launch_matvec(hb_ctx *c, u64 *out, const u64 *x, const u64 *p, const MatvecShape &s, int limbs) {
+    launch(c, k_matvec<V, C>, dim3((unsigned)(c->N / 256) * (unsigned)(((s.vectors + V - 1) / V) * ((s.columns + C - 1) / C)), (unsigned)limbs), 256, 0, out, x, p, s, c->pc, c->N);
+}
 // slot values of the residues t [count][2][N]: member b, slot s at re[(b * slots + s) * stride], im likewise
 void embed_forward(hb_ctx *c, double *re, double *im, int stride, const u64 *t, const DecItem *items, int count) {
     if (c->logn == 16) {
@@ -1715,15 +1735,16 @@ int hb_encode_q4(hb_ctx *c, const hb_qweight *w, int tile, int diagonal, int fir
         const Tiles4 t = tiles4(c, w, tile);
         if (first < 0 || count < 1 || (i64)first + count > (i64)t.kb * t.nb) fail(HB_E_ARG, "encode_q4: blocks that are not there");
         std::vector<hb_pt *> r((size_t)count, nullptr);
-        const size_t words = (size_t)(level + 1) * c->N;
         try {
             for (hb_pt *&p : r) p = new_pt(c, level, 1);
             ALG(c, (size_t)count * (level + 1));
             for (int k = 0; k < count; k += kBlocks4) {
                 const int m = std::min(kBlocks4, count - k);
-                Tmp t4(c, (size_t)m * (level + 1));
-                encode_blocks4(c, w, tile, t.kb, diagonal != 0, first + k, m, level, t4.p);
-                for (int i = 0; i < m; ++i) CK(cudaMemcpyAsync(r[(size_t)(k + i)]->d, t4.p + i * words, words * 8, cudaMemcpyDeviceToDevice, c->st));
+                TmpBytes coef(c, (size_t)m * c->N * sizeof(i64));
+                PtList to{};
+                for (int i = 0; i < m; ++i) to.p[i] = r[(size_t)(k + i)]->d;
+                coefficients4(c, w, blocks4(w, tile, t.kb, diagonal != 0, first + k), m, level, (i64 *)coef.p);
+                transform4(c, to, (const i64 *)coef.p, m, 0, level + 1);
             }
         } catch (...) { for (hb_pt *p : r) hb_pt_free(p); throw; }
         std::copy(r.begin(), r.end(), out);
@@ -1737,16 +1758,31 @@ int hb_matvec_q4(hb_ctx *c, const hb_ct *x, const hb_qweight *w, int tile, hb_ct
         const Tiles4 t = tiles4(c, w, tile);
         if (x->batch % t.kb) fail(HB_E_SHAPE, "matvec_q4: the batch is no whole number of vectors");
         const int vectors = x->batch / t.kb, n = x->level + 1;
-        if ((i64)vectors * t.nb > INT32_MAX / 64 || (i64)vectors * std::min(t.nb, kBlocks4) > 65535) fail(HB_E_LIMIT, "matvec_q4: too many results");
+        if ((i64)vectors * t.nb > INT32_MAX / 64 || (i64)t.kb * c->N > INT32_MAX) fail(HB_E_LIMIT, "matvec_q4: too many results or rows");
         hb_ct *r = new_ct(c, x->level, 2, vectors * t.nb, 2);
         try {
             ALG(c, x->limbs() + r->limbs());
-            const int columns = std::max(1, kBlocks4 / t.kb);
+            // columns whose operands make one launch (a column of many K-groups several), and as many limbs at once as stay in L2 with them: x is read once per set of columns
+            const int columns = std::max(1, kBlocks4 / t.kb), N = c->N;
             for (int j = 0; j < t.nb; j += columns) {
-                const int m = std::min(columns, t.nb - j);
-                Tmp p(c, (size_t)m * t.kb * n);
-                encode_blocks4(c, w, tile, t.kb, false, j * t.kb, m * t.kb, x->level, p.p);
-                launch(c, k_matvec, dim3((unsigned)(c->N / 256), (unsigned)n, (unsigned)(vectors * m)), 256, 0, r->d, (const u64 *)x->d, (const u64 *)p.p, t.kb, m, t.nb, j, n, c->qmap(x->level), c->pc, c->N);
+                const int m = std::min(columns, t.nb - j), blocks = m * t.kb, at_once = (int)std::clamp<size_t>(kMatvecBytes / ((size_t)blocks * N * 8), 1, (size_t)n);
+                TmpBytes coef(c, (size_t)blocks * N * sizeof(i64));
+                for (int k = 0; k < blocks; k += kBlocks4)
+                    coefficients4(c, w, blocks4(w, tile, t.kb, false, j * t.kb + k), std::min(kBlocks4, blocks - k), x->level, (i64 *)coef.p + (size_t)k * N);
+                for (int l0 = 0; l0 < n; l0 += at_once) {
+                    const int limbs = std::min(at_once, n - l0);
+                    Tmp p(c, (size_t)blocks * limbs);
+                    for (int k = 0; k < blocks; k += kBlocks4) {
+                        const int some = std::min(kBlocks4, blocks - k);
+                        PtList to{};
+                        for (int i = 0; i < some; ++i) to.p[i] = p.p + ((size_t)(k + i) * limbs - l0) * N;
+                        transform4(c, to, (const i64 *)coef.p + (size_t)k * N, some, l0, limbs);
+                    }
+                    const MatvecShape s{vectors, t.kb, m, t.nb, j, n, l0};
+                    if (vectors == 1) launch_matvec<1, 4>(c, r->d, x->d, p.p, s, limbs);
+                    else if (vectors == 2) launch_matvec<2, 4>(c, r->d, x->d, p.p, s, limbs);
+                    else launch_matvec<4, 2>(c, r->d, x->d, p.p, s, limbs);
+                }
             }
         } catch (...) { hb_ct_free(r); throw; }
         *out = r;

@@ -456,8 +456,8 @@ __global__ void __launch_bounds__(256, MINB) ntt16v2_fwd_cols(const u64 *src, Li
 }
 
 // ---- forward, row pass: stages 9..16; stores canonical residues ----
-template <int MINB, class LONG>
-__global__ void __launch_bounds__(256, MINB) ntt16v2_fwd_rows(const u64 *src, LimbAddr16 sa, u64 *dst, LimbAddr16 da,
+template <int MINB, class LONG, class ADDR = LimbAddr16>
+__global__ void __launch_bounds__(256, MINB) ntt16v2_fwd_rows(const u64 *src, const __grid_constant__ ADDR sa, u64 *dst, const __grid_constant__ ADDR da,
                                                         const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, Ntt16Tables tb) {
     __shared__ u64 sm[16 * kRowStride];
     const int li = blockIdx.y, pi = map.prime[li % map.n];

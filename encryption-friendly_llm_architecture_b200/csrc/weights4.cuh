@@ -4,54 +4,225 @@
 // four tiles of d rows of one column tile, 1/2 (W1 - i W3) | 1/2 (W2 - i W4); `diagonal`: column j rolled up by j, as the shifted copies meet it.
 #pragma once
 #include "embed.cuh"
+#include "ntt.cuh"
 
 namespace hb {
 
 // codes [ceil(rows / 2)][cols], the even row in the low half of a byte; scales [ceil(rows / group)][cols]
 struct Weights4 { const unsigned char *codes; const float *scales; int rows, cols, group; };
-// the weight at (r, c), halved; zero outside
-__device__ __forceinline__ double half_weight(const Weights4 &w, int r, int c) {
-    if (r >= w.rows || c >= w.cols) return 0.0;
-    const int byte = __ldg(w.codes + (size_t)(r >> 1) * w.cols + c), code = r & 1 ? byte >> 4 : byte & 15;
-    return (double)(code - 8) * (0.5 * (double)__ldg(w.scales + (size_t)(r / w.group) * w.cols + c));
-}
-struct Blocks4 { int first, kb, d, diagonal; }; // block number first + y is K-group (.) % kb of column tile (.) / kb
-// the value of slot i of a block
-__device__ __forceinline__ double2 slot_weight(const Weights4 &w, const Blocks4 &b, int block, int i) {
-    const int d = b.d, r = i / (2 * d);
-    if (r >= d) return make_double2(0.0, 0.0);
-    const int c2 = i - r * 2 * d, half = c2 >= d, c = half ? c2 - d : c2;
-    int from = r;
-    if (b.diagonal) { from += c; if (from >= d) from -= d; }
-    const int row = (block % b.kb * 4 + half) * d + from, col = block / b.kb * d + c;
-    const double im = half_weight(w, row + 2 * d, col);
-    return make_double2(half_weight(w, row, col), im == 0.0 ? 0.0 : -im);
-}
-// slots re, im [count][slots].  grid = (slots / 256, count)
-__global__ void __launch_bounds__(256) k_weight_slots(double *re, double *im, Weights4 w, Blocks4 b, int slots) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
+// block number first + y is K-group (.) % kb of column tile (.) / kb.  Quotients by 2 d and by the group come from products: by_row = ceil(2^32 / 2d) is exact for slots
+// below 2^15, by_group = ceil(2^32 / group) for rows of a block, counted from the start of a group; 0 where a group is at least as long as a block, so that a block meets two
+struct Blocks4 { int first, kb, d, diagonal; u32 by_row; u64 by_group; };
+// Rows and columns of one block.
+struct Block4 {
+    const Weights4 &w;
+    const Blocks4 &b;
+    int row0, col0, group0, rest; // its first row and column; the group that row lies in, and its place there
+    __device__ __forceinline__ Block4(const Weights4 &w_, const Blocks4 &b_, int block) : w(w_), b(b_) {
+        row0 = block % b.kb * 4 * b.d; col0 = block / b.kb * b.d;
+        group0 = row0 / w.group; rest = row0 - group0 * w.group;
+    }
+    // the weight at row r and column c of the block, halved; zero outside the matrix, of which the last row and column are read instead, so that no load waits for a branch
+    __device__ __forceinline__ double half(int r, int c) const {
+        const bool there = r < w.rows - row0 && c < w.cols - col0;
+        const int rr = min(r, w.rows - 1 - row0), cc = min(col0 + c, w.cols - 1), row = row0 + rr; // the block's first row and column are there
+        const int byte = __ldg(w.codes + (size_t)(row >> 1) * w.cols + cc), code = row & 1 ? byte >> 4 : byte & 15;
+        const u32 t = (u32)(rest + rr), group = (u32)group0 + (b.by_group ? (u32)(t * b.by_group >> 32) : t >= (u32)w.group);
+        const float scale = __ldg(w.scales + (size_t)group * w.cols + cc);
+        return there ? (double)(code - 8) * (0.5 * (double)scale) : 0.0;
+    }
+    __device__ __forceinline__ double2 slot(int i) const { // the value of slot i
+        const int d = b.d, r = (int)__umulhi((u32)i, b.by_row), c2 = i - r * 2 * d, right = c2 >= d, c = right ? c2 - d : c2;
+        int from = r;
+        if (b.diagonal) { from += c; if (from >= d) from -= d; }
+        if (r >= d) from = 4 * d; // past the tiles
+        else from += right * d;
+        const double re = half(from, c), im = half(from + 2 * d, c);
+        return r < d ? make_double2(re, 0.0 - im) : make_double2(0.0, 0.0);
+    }
+};
+// Where the members of a batch of plaintexts lie: one buffer each.
+constexpr int kBlocks4 = 64; // blocks of a launch
+struct PtList {
+    u64 *p[kBlocks4];
+    __device__ __forceinline__ u64 *at(int member, int limb, int N) const { return p[member] + (size_t)limb * N; }
+    __device__ __forceinline__ size_t off(int li, int period) const { return (size_t)(at(li / period, li % period, kN16) - (u64 *)nullptr); } // from a null base: the address of ntt16.cuh
+};
+// ---- slots -> coefficients: k_embed_inv_cols and k_embed_inv_small with the slots made on the way ----
+// half-transformed slots v [count][2^15].  grid = (16, count)
+__global__ void __launch_bounds__(kEmbThreads) k_weight_cols(double2 *v, const __grid_constant__ Weights4 w, const __grid_constant__ Blocks4 b, EmbedTables tb) {
+    __shared__ double2 sm[kEmbRows * 8];
+    const int lane = threadIdx.x & 7, sub = threadIdx.x >> 3, col = blockIdx.x * 8 + lane;
+    const Block4 block(w, b, b.first + (int)blockIdx.y);
+    double2 x[16];
     pdl_wait();
-    if (i >= slots) return;
-    const double2 v = slot_weight(w, b, b.first + (int)blockIdx.y, i);
-    re[(size_t)blockIdx.y * slots + i] = v.x; im[(size_t)blockIdx.y * slots + i] = v.y;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = block.slot((e * 16 + sub) * kEmbCols + col);
+    inv_round<8>(x, tb.inv, 16 * kEmbCols, sub * kEmbCols + col);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) sm[(e * 16 + sub) * 8 + lane] = x[e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] = sm[(sub * 16 + e) * 8 + lane];
+    inv_round<8>(x, tb.inv, kEmbCols, col);
+    double2 *o = v + (size_t)blockIdx.y * kSlots16 + col;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[(sub * 16 + e) * kEmbCols] = x[e];
 }
-// out[v][j] (+)= sum_b x[v][b] (.) p[j][b], one coefficient of both polynomials a thread: x [vectors][kb][2][n][N], p [columns][kb][n][N], out [vectors][nb][2][n][N] from column j0.
-// grid = (N / 256, n, vectors * columns)
-__global__ void __launch_bounds__(256) k_matvec(u64 *out, const u64 *x, const u64 *p, int kb, int columns, int nb, int j0, int n, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, int N) {
-    const int l = blockIdx.y, v = blockIdx.z / columns, j = blockIdx.z % columns;
-    const PrimeConst m = pc[map.prime[l]];
-    const size_t poly = (size_t)n * N, at = (size_t)l * N + blockIdx.x * 256 + threadIdx.x;
-    const u64 *xp = x + (size_t)v * kb * 2 * poly + at, *pp = p + (size_t)j * kb * poly + at;
-    u64 *o = out + ((size_t)v * nb + j0 + j) * 2 * poly + at;
+// rounded coefficients at scale sc, coef [count][2 slots].  grid = count
+__global__ void __launch_bounds__(256) k_weight_small(i64 *coef, const __grid_constant__ Weights4 w, const __grid_constant__ Blocks4 b, int log_slots, double sc, EmbedTables tb) {
+    __shared__ double2 sm[kEmbSmallMax];
+    const int slots = 1 << log_slots;
+    const Block4 block(w, b, b.first + (int)blockIdx.x);
     pdl_wait();
-    auto sum = [&](auto s0, int room) {
-        auto s1 = s0;
-        s0.zero(); s1.zero();
-        for (int b = 0; b < kb; ++b, xp += 2 * poly, pp += poly) {
-            if (b && b % room == 0) { s0.relax(m); s1.relax(m); }
-            s0.product(xp[0], pp[0]); s1.product(xp[poly], pp[0]);
+    for (int i = threadIdx.x; i < slots; i += 256) sm[i] = block.slot(i);
+    for (int h = slots >> 1; h >= 1; h >>= 1) {
+        __syncthreads();
+        for (int t = threadIdx.x; t < slots / 2; t += 256) {
+            const int j = t & (h - 1), a = (t - j) * 2 + j;
+            inv_bfly(sm[a], sm[a + h], __ldg(tb.inv + h + j));
         }
-        o[0] = s0.canonical(m); o[poly] = s1.canonical(m);
+    }
+    __syncthreads();
+    const double inv = 1.0 / (double)slots;
+    i64 *o = coef + (size_t)blockIdx.x * 2 * slots;
+    for (int i = threadIdx.x; i < slots; i += 256) {
+        const double2 x = sm[__brev((u32)i) >> (32 - log_slots)];
+        o[i] = to_i64(rint(__dmul_rn(__dmul_rn(x.x, inv), sc)));
+        o[i + slots] = to_i64(rint(__dmul_rn(__dmul_rn(x.y, inv), sc)));
+    }
+}
+// ---- coefficients -> residues in transform order ----
+// The column pass of ntt16v2_fwd_cols on coefficients coef [count][2^16], reduced on the way: a pass over the residues of every limb less.  Limbs l0 .. of the members of `to`; map
+// names their primes.  32 members at level 5, with the reduction apart: 97 us, 45 with it (the butterflies hide behind nothing: FP64 bound).  grid = (16, count * map.n)
+template <class LONG>
+__global__ void __launch_bounds__(256, 4) k_coef_cols(const __grid_constant__ PtList to, int l0, const i64 *coef, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, Ntt16Tables tb) {
+    __shared__ u64 sm[4096];
+    const int member = blockIdx.y / map.n, li = blockIdx.y % map.n, pi = map.prime[li];
+    const PrimeConst m = pc[pi];
+    const ulonglong2 *tab = tb.fwd + (size_t)pi * Ntt16Layout::kEntries;
+    const int tid = threadIdx.x, lane = tid & 15, sub = tid >> 4;
+    const i64 *p = coef + (size_t)member * kN16 + blockIdx.x * 16 + lane;
+    u64 *o = to.at(member, l0 + li, kN16) + blockIdx.x * 16 + lane;
+    i64 a[16];
+    u64 large = 0; // the magnitudes' bits: as a rule the coefficients are far below 2^44
+    pdl_wait();
+#pragma unroll
+    for (int e = 0; e < 16; ++e) a[e] = p[(e * 16 + sub) * 256];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) large |= (u64)(a[e] ^ (a[e] >> 63));
+    if (m.small) {
+        const DsConst c = ds_const(m);
+        double v[16];
+        if (large >> 50)
+            for (int e = 0; e < 16; ++e) v[e] = ds_load(reduce_i64(a[e], m));
+        else
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = ds_reduce(__longlong_as_double(a[e] + 0x4338000000000000ll) - kMagicS, c); // 2^52 + 2^51 + a
+        fwd16_ds(v, TwiddlesA(tab + Ntt16Layout::colsA(0)), c);
+        double *smd = reinterpret_cast<double *>(sm);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) smd[(e * 16 + sub) * 16 + lane] = v[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = smd[(sub * 16 + e) * 16 + lane];
+        fwd16_ds(v, TwiddlesA(tab + Ntt16Layout::colsB(sub, 0)), c);
+        double *od = reinterpret_cast<double *>(o);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) od[(sub * 16 + e) * 256] = v[e];
+    } else {
+        u64 v[16];
+        if (large >> 44)
+            for (int e = 0; e < 16; ++e) v[e] = reduce_i64(a[e], m);
+        else
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[e] = a[e] < 0 ? (u64)a[e] + m.q : (u64)a[e];
+        const typename LONG::Const c = LONG::make(m);
+        LONG::template fwd16<0>(v, TwiddlesA(tab + Ntt16Layout::colsA(0)), c);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sm[(e * 16 + sub) * 16 + lane] = v[e];
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e] = sm[(sub * 16 + e) * 16 + lane];
+        LONG::template fwd16<1>(v, TwiddlesA(tab + Ntt16Layout::colsB(sub, 0)), c);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[(sub * 16 + e) * 256] = v[e];
+    }
+}
+// the whole transform of a small ring's limb: ntt_small on coefficients.  grid = (map.n, count)
+__global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtList to, int l0, const i64 *coef, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, NttTables tb, int logn) {
+    extern __shared__ u64 sm_dyn[];
+    const int N = 1 << logn, pi = map.prime[blockIdx.x];
+    const PrimeConst m = pc[pi];
+    const u64 q = m.q, q2 = q << 1;
+    const i64 *p = coef + (size_t)blockIdx.y * N;
+    u64 *o = to.at(blockIdx.y, l0 + blockIdx.x, N);
+    const u64 *w = tb.psi + (size_t)pi * N, *ws = tb.psi_sh + (size_t)pi * N;
+    pdl_wait();
+    for (int i = threadIdx.x; i < N; i += 256) sm_dyn[i] = reduce_i64_any(p[i], m);
+    __syncthreads();
+    for (int h = 1, t = N >> 1; h < N; h <<= 1, t >>= 1) {
+        for (int k = threadIdx.x; k < N / 2; k += 256) {
+            const int i = k / t, i0 = 2 * i * t + (k - i * t);
+            ct_bfly(sm_dyn[i0], sm_dyn[i0 + t], w[h + i], ws[h + i], q, q2);
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < N; i += 256) {
+        u64 x = sm_dyn[i];
+        x = x >= q2 ? x - q2 : x;
+        o[i] = x >= q ? x - q : x;
+    }
+}
+// ---- products ----
+// out[v][j] = sum_b x[v][b] (.) p[j][b]: x [vectors][kb][2][n][N], operands p [columns][kb][limbs][N] of the limbs l0 .. and the columns j0 .., out [vectors][nb][2][n][N].  A thread has one
+// coefficient of both polynomials of V vectors and of C columns: 2 V + C words for 2 V C products, as many in flight.  Bound by the words of x and of the results.  The blocks of one
+// range of coefficients run side by side.  grid = (N / 256 * blocks, limbs)
+struct MatvecShape { int vectors, kb, columns, nb, j0, n, l0; };
+template <int V, int C>
+__global__ void __launch_bounds__(256, 2) k_matvec(u64 *out, const u64 *x, const u64 *p, MatvecShape s, const PrimeConst *__restrict__ pc, int N) {
+    const int bv = (s.vectors + V - 1) / V, blocks = bv * ((s.columns + C - 1) / C), blk = blockIdx.x % blocks, v0 = blk % bv * V, c0 = blk / bv * C, l = s.l0 + blockIdx.y, limbs = gridDim.y;
+    const PrimeConst m = pc[l];
+    const u32 at = blockIdx.x / blocks * 256 + threadIdx.x;
+    const size_t poly = (size_t)s.n * N, limb = (size_t)limbs * N;
+    const u64 *xp[V], *pp[C];
+#pragma unroll
+    for (int i = 0; i < V; ++i) xp[i] = x + (size_t)min(v0 + i, s.vectors - 1) * s.kb * 2 * poly + (size_t)l * N + at; // past the end: the last one again, not stored
+#pragma unroll
+    for (int j = 0; j < C; ++j) pp[j] = p + (size_t)min(c0 + j, s.columns - 1) * s.kb * limb + (size_t)blockIdx.y * N + at;
+    pdl_wait();
+    auto sum = [&](auto kind, int room) {
+        decltype(kind) a[V][C][2];
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j) { a[i][j][0].zero(); a[i][j][1].zero(); }
+#pragma unroll 1
+        for (int b = 0; b < s.kb; ++b) {
+            u64 xv[V][2], pv[C];
+#pragma unroll
+            for (int i = 0; i < V; ++i) { xv[i][0] = xp[i][0]; xv[i][1] = xp[i][poly]; xp[i] += 2 * poly; }
+#pragma unroll
+            for (int j = 0; j < C; ++j) { pv[j] = pp[j][0]; pp[j] += limb; }
+            if (b && b % room == 0) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+#pragma unroll
+                    for (int j = 0; j < C; ++j) { a[i][j][0].relax(m); a[i][j][1].relax(m); }
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+#pragma unroll
+                for (int j = 0; j < C; ++j) { a[i][j][0].product(xv[i][0], pv[j]); a[i][j][1].product(xv[i][1], pv[j]); }
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                if (v0 + i >= s.vectors || c0 + j >= s.columns) continue;
+                u64 *o = out + ((size_t)(v0 + i) * s.nb + s.j0 + c0 + j) * 2 * poly + (size_t)l * N + at;
+                o[0] = a[i][j][0].canonical(m); o[poly] = a[i][j][1].canonical(m);
+            }
     };
     if (m.fp) sum(FpAcc{}, m.q < (1ull << 42) ? 128 : 8);
     else sum(PieceAcc{}, 8);
