@@ -138,6 +138,15 @@ class HEMMer {
     // singleCCMatMul in two halves (transforms, then the product loop), for batching operands of different levels
     void ccMatMulPrepare(const CtxtTensor &a, const CtxtTensor &b, int target_level, Ciphertext &sigma_a, Ciphertext &tau_b);
     CtxtTensor ccMatMulCore(Ciphertext sigma_a, Ciphertext tau_b, i64 rows, i64 inner, i64 cols, i64 width, int target_level);
+    // Products of tiles with tiles of another number (the reference's sequences are one tile long): for every head h, query tile i and key tile j the
+    // product sum over r < inner of a[r][h][i] * b[r][h][j], members in that order; the result's are [j][h][i], so that scores can be the left operand
+    // of the product with the values (inner = key tiles).  crossScores transposes the key tiles first.
+    CtxtTensor crossMatMul(const CtxtTensor &a, const CtxtTensor &b, int heads = 1, int inner = 1, int target_level = 4);
+    CtxtTensor crossScores(const CtxtTensor &query, const CtxtTensor &key, int heads = 1, int target_level = 4);
+    // Encrypted vectors times a matrix in 4 bits (hb_qweight): x has ceil(rows / 4 tile) members a vector, entry 4 tile b + s of it in all columns of row
+    // s % tile (member b; s < tile: left half, real part; < 2 tile: right half, real part; < 3 tile: left half, imaginary part; then right half,
+    // imaginary part).  One member per vector and column tile: y / 2 is the sum of the real parts of the halves, the same in every row, one level lower.
+    CtxtTensor vecMatMul4(const CtxtTensor &x, const hb_qweight *w);
     CtxtTensor packedMatMul(const CtxtTensor &a, const CtxtTensor &b, int target_level = 4);
     CtxtTensor packedMatMulPre(const CtxtTensor &a, int target_level = 4);
     Ciphertext packedMatMulPreRot(const CtxtTensor &a, int target_level = 4);

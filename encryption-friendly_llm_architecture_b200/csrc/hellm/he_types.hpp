@@ -247,6 +247,13 @@ class Evaluator {
         acc = Ciphertext(c_, p);
         check(c_, rc);
     }
+    // acc[j][h][i] += sum_g tensor(a[g][h][i], b[g][h][j])
+    void tensorAccumulateCross(Ciphertext &acc, const Ciphertext &a, const Ciphertext &b, int groups, int heads) const {
+        hb_ct *p = acc.release();
+        int rc = hb_tensor_acc_cross(c_, a.raw(), b.raw(), groups, heads, &p);
+        acc = Ciphertext(c_, p);
+        check(c_, rc);
+    }
     Ciphertext concat(const std::vector<Ciphertext> &parts) const {
         std::vector<const hb_ct *> raw;
         for (const auto &x : parts) raw.push_back(x.raw());
@@ -297,6 +304,14 @@ class Evaluator {
     Ciphertext matmulGroups(const Ciphertext &pre, int btotal, int b0, const std::vector<const hb_pt *> &pts, i64 row_step) const {
         hb_ct *o = nullptr; check(c_, hb_matmul_acc_multi(c_, pre.raw(), btotal, b0, pts.data(), (int)pts.size(), row_step, &o)); return Ciphertext(c_, o);
     }
+    // products grouped by expert: pts[(e * tiles + t) * bcount + b], member p * tiles + t of the result; order empty: position p has input p
+    Ciphertext matmulGrouped(const Ciphertext &pre, int inputs, const std::vector<int32_t> &order, const std::vector<int32_t> &sizes, const std::vector<const hb_pt *> &pts, int bcount, int tiles, i64 row_step) const {
+        hb_ct *o = nullptr;
+        check(c_, hb_matmul_acc_grouped(c_, pre.raw(), inputs, order.empty() ? nullptr : order.data(), sizes.data(), (int)sizes.size(), pts.data(), bcount, tiles, row_step, &o));
+        return Ciphertext(c_, o);
+    }
+    // encrypted vectors times a matrix in 4 bits, un-rescaled
+    Ciphertext matvec4(const Ciphertext &x, const hb_qweight *w, int tile) const { hb_ct *o = nullptr; check(c_, hb_matvec_q4(c_, x.raw(), w, tile, &o)); return Ciphertext(c_, o); }
     Ciphertext stack(const std::vector<Ciphertext> &v) const {
         int level = 0, np = 0, sp = 0, b = 1; hb_ct_meta(v[0].raw(), &level, &np, &b, &sp);
         hb_ct *o = nullptr; check(c_, hb_ct_create(c_, level, np, (int)v.size() * b, sp, &o)); // copy k of input j at k*b + j

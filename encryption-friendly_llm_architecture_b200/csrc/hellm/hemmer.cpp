@@ -108,6 +108,17 @@ void HEMMer::ccMatMulPrepare(const CtxtTensor &a, const CtxtTensor &b, int t, Ci
 CtxtTensor HEMMer::ccMatMulCore(Ciphertext sa, Ciphertext tb, i64 rows, i64 inner, i64 cols, i64 width, int t) {
     HB_ENV; return sched::ccmmCore(env, std::move(sa), std::move(tb), rows, inner, cols, width, t);
 }
+CtxtTensor HEMMer::crossMatMul(const CtxtTensor &a, const CtxtTensor &b, int heads, int inner, int t) { HB_ENV; return sched::multCross(env, a, b, heads, inner, t); }
+CtxtTensor HEMMer::crossScores(const CtxtTensor &query, const CtxtTensor &key, int heads, int t) {
+    CtxtTensor turned(key.getShape(), eval_.view(key.get(), 0, key.get().getBatch()));
+    transposeInplace(turned, schedule_ == sched::kLazy ? t + 3 : 0); // in the fast schedule at the lowest level that leaves enough for the product
+    return crossMatMul(query, turned, heads, 1, t);
+}
+CtxtTensor HEMMer::vecMatMul4(const CtxtTensor &x, const hb_qweight *w) {
+    Ciphertext y = eval_.rescale(eval_.matvec4(x.get(), w, (int)tile_));
+    for (i64 rot = 1; rot < tile_; rot <<= 1) y = eval_.add(y, eval_.leftRotate(y, rot * 2 * tile_)); // the sum over the rows, in all of them
+    return CtxtTensor(TileTensorShape(tile_, tile_, 2 * tile_), std::move(y));
+}
 CtxtTensor HEMMer::packedMatMul(const CtxtTensor &a, const CtxtTensor &b, int t) { HB_ENV; return sched::multPackedMatMat(env, a, b, t); }
 CtxtTensor HEMMer::packedMatMulPre(const CtxtTensor &a, int t) { HB_ENV; return sched::multPackedMatMatPre(env, a, t); }
 Ciphertext HEMMer::packedMatMulPreRot(const CtxtTensor &a, int t) { HB_ENV; return sched::multPackedMatMatPreRot(env, a, t); }

@@ -207,6 +207,32 @@ int hb_hemmer_matmul_cc_core(hb_hemmer *h, const hb_ct *sa, const hb_ct *tb, int
         *out = h->h.ccMatMulCore(Ciphertext(ba.c), Ciphertext(bb.c), rows, inner, cols, width, target).get().release();
     });
 }
+int hb_hemmer_cross_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa, const hb_ct *b, int rb, int cb, int wb, int heads, int inner, int target, hb_ct **out) {
+    return guard([&] {
+        if (!a || !b || !out) throw std::invalid_argument("[crossMatMul] null argument");
+        Borrow ba(h->ctx, a), bb(h->ctx, b);
+        *out = h->h.crossMatMul(view(ba, ra, ca, wa), view(bb, rb, cb, wb), heads, inner, target).get().release();
+    });
+}
+int hb_hemmer_cross_scores(hb_hemmer *h, const hb_ct *query, const hb_ct *key, int rows, int cols, int width, int heads, int target, hb_ct **out) {
+    return guard([&] {
+        if (!query || !key || !out) throw std::invalid_argument("[crossScores] null argument");
+        Borrow bq(h->ctx, query), bk(h->ctx, key);
+        *out = h->h.crossScores(view(bq, rows, cols, width), view(bk, rows, cols, width), heads, target).get().release();
+    });
+}
+int hb_hemmer_matmul_reuse_grouped(hb_hemmer *h, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts, const hb_pt *const *pts, int bcount, int tiles, int width,
+                                   hb_ct **out) {
+    return guard([&] { hb_ct *o = nullptr; check(h->ctx, hb_matmul_acc_grouped(h->ctx, pre, inputs, order, sizes, experts, pts, bcount, tiles, width, &o)); *out = o; });
+}
+int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct **out) {
+    return guard([&] {
+        if (!x || !w || !out) throw std::invalid_argument("[vecMatMul4] null argument");
+        Borrow bx(h->ctx, x);
+        const int d = (int)h->h.tile();
+        *out = h->h.vecMatMul4(view(bx, d, d, 2 * d), w).get().release();
+    });
+}
 int hb_hemmer_packed_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa, const hb_ct *b, int rb, int cb, int wb, int target, hb_ct **out) {
     return guard([&] {
         Borrow ba(h->ctx, a), bb(h->ctx, b);

@@ -490,6 +490,43 @@ CtxtTensor multMatMatCC(Env &e, const CtxtTensor &op1, const CtxtTensor &op2, in
     return ccmmCore(e, std::move(a), std::move(b), op1.getHeight(), op1.getWidth(), op2.getWidth(), op1.getBlockWidth(), target_level);
 }
 
+// out[j][h][i] = sum over r of A[r][h][i] * B[r][h][j] for the tiles of `heads` heads (members in that order): blocks of two matrices, or query tiles
+// against key tiles of another number.  As ccmmPrepare and ccmmCore, but every tile's copies are made once for all the pairs that it is in
+// (nq + nk sets of them instead of 2 nq nk), the first term is one of the sum, and the sum over k and r is relinearised and rescaled once.  The reference has no
+// such product and so no order of rotations to keep: kFaithful takes the copies of kDirect.
+CtxtTensor multCross(Env &e, const CtxtTensor &op1, const CtxtTensor &op2, int heads, int inner, int target_level) {
+    const auto whole = [&](const CtxtTensor &t) { return heads > 0 && inner > 0 && t.get().getBatch() % ((i64)heads * inner) == 0; };
+    if (!whole(op1) || !whole(op2)) throw std::invalid_argument("[multCross] a batch does not split into that many heads and inner tiles");
+    const i64 num_rows = op1.getHeight(), num_cols = op2.getWidth(), width = op1.getBlockWidth(), num_k = ceil_pow2(op1.getWidth());
+    const int lvl = target_level + 2;
+    Ciphertext a, b, acc;
+    ccmmPrepare(e, op1, op2, target_level, a, b);
+    const TileTensorShape sa(num_rows, num_k, width), sb(num_k, num_cols, width);
+    const i64 rows_tmp = num_k > num_rows ? num_k : ceil_pow2(num_rows), cols_tmp = num_k > num_cols ? num_k : ceil_pow2(num_cols);
+    e.ev.tensorAccumulateCross(acc, e.ev.levelDownOne(a), e.ev.levelDownOne(b), inner, heads);
+    const Hoisted ha = e.ev.decompose(a), hb = e.ev.decompose(b);
+    const bool lazy = e.mode == kLazy;
+    const i64 group = lazy ? std::min(loop_group(a), loop_group(b)) : std::min(direct_group(a), direct_group(b));
+    for (i64 i0 = 1; i0 < num_k; i0 += group) {
+        const i64 count = std::min(num_k - i0, group);
+        Ciphertext ak, bk;
+        if (lazy) {
+            std::vector<WrappedCopy> wa, wb;
+            for (i64 i = i0; i < i0 + count; ++i) {
+                wa.push_back(wrapped_copy(e, false, sa, i, lvl, i, i - cols_tmp));
+                wb.push_back(wrapped_copy(e, true, sb, i, lvl, i * width, (i - rows_tmp) * width));
+            }
+            ak = assemble_lazy(e, a, ha, wa);
+            bk = assemble_lazy(e, b, hb, wb);
+        } else {
+            ak = direct_copies(e, a, ha, i0, count, [&](i64 i) { return std::make_pair(i, i - cols_tmp); }, [&](i64 w) -> const Plaintext & { return col_wrap(e, sa, w, lvl); });
+            bk = direct_copies(e, b, hb, i0, count, [&](i64 i) { return std::make_pair(i * width, (i - rows_tmp) * width); }, [&](i64 w) -> const Plaintext & { return row_wrap(e, sb, w, lvl); });
+        }
+        e.ev.tensorAccumulateCross(acc, ak, bk, (int)count * inner, heads);
+    }
+    return CtxtTensor(TileTensorShape(num_rows, num_cols, width), e.ev.rescale(e.ev.relinearize(acc)));
+}
+
 // multMatMat<Plaintext> (HEMMer::singleMatMul) -- MatrixUtils.cpp:1448-1570: ciphertext x plaintext without reuse.  The right
 // operand is decoded, tau-transformed in the clear (diagonalToRow<Plaintext>, :1072-1098), encoded at target + 2 and then
 // shifted by slot rotations of the plaintext; its row wrap uses plaintext x mask products as the reference does.

@@ -297,6 +297,66 @@ class Hemmer:
             raise HBError(rc, g().decode())
         return [CtxtTensor(Handle(self.lib, C.c_void_p(outs[t]), "ct"), *weights_by_tile[0][0].shape) for t in range(tiles)]
 
+    def matmul_reuse_experts(self, pre, inputs, sizes, weights, order=None):
+        """matmul_reuse_groups grouped by expert: weights[e][t][b] (None for an expert without inputs), the first sizes[0] positions at expert 0
+        and so on, position p with input order[p] (None: p); `pre` holds the copies of `inputs` inputs of as many K-groups as the weights have,
+        K-groups innermost.  Member p * tiles + t of the result is output tile t of position p."""
+        first = next(w for w, n in zip(weights, sizes) if n)[0][0]
+        pts = [[[w.ct for w in row] for row in rows] if n else None for rows, n in zip(weights, sizes)]
+        return CtxtTensor(self.lib.matmul_acc_grouped(pre, inputs, sizes, pts, first.width, order=order), *first.shape)
+
+    # ---- tiles against tiles of another number ----
+    def cross_matmul(self, a, b, heads=1, inner=1, target_level=4):
+        """out[j][h][i] = sum_r a[r][h][i] @ b[r][h][j] for the tiles of `heads` heads, batch members in that order."""
+        ct = self._call("cross_matmul", a.ct.ptr, *self._shp(a), b.ct.ptr, *self._shp(b), C.c_int(heads), C.c_int(inner), C.c_int(target_level))
+        return CtxtTensor(ct, a.rows, b.cols, a.width)
+
+    def cross_scores(self, query, key, heads=1, target_level=4):
+        """cross_matmul with the transposed key tiles: member (j * heads + h) * nq + i is query tile i times key tile j transposed."""
+        ct = self._call("cross_scores", query.ct.ptr, key.ct.ptr, *self._shp(query), C.c_int(heads), C.c_int(target_level))
+        return CtxtTensor(ct, query.rows, key.rows, query.width)
+
+    # ---- weights in 4 bits ----
+    @property
+    def tile(self):
+        """Side of the tile two of which fill a ciphertext."""
+        d = 1
+        while 2 * d * d < self.lib.slots:
+            d <<= 1
+        return d
+
+    def encode_diagonal_to_row4_q4(self, qweight, rows, cols, level=0):
+        """The operands that encode_diagonal_to_row4 makes of a rows x cols matrix, from its 4-bit form (Lib.qweight): [column tile][K-group]."""
+        d = self.tile
+        kb, nb = -(-rows // (4 * d)), -(-cols // d)
+        pts = self.lib.encode_q4(qweight, d, 0, kb * nb, level or self.lib.L)
+        return [[PtxtTensor(p, d, d, 2 * d) for p in pts[j * kb:(j + 1) * kb]] for j in range(nb)]
+
+    def encrypt_vectors(self, x, level, nonces):
+        """Rows of x spread over the columns of the tiles as matvec_q4 takes them: one member per vector and K-group of 4 tile entries."""
+        x, d = np.atleast_2d(np.asarray(x, dtype=np.float64)), self.tile
+        kb = -(-x.shape[1] // (4 * d))
+        parts = np.zeros((x.shape[0] * kb, 4, d))
+        for v, row in enumerate(x):
+            padded = np.zeros(kb * 4 * d)
+            padded[: row.size] = row
+            parts[v * kb:(v + 1) * kb] = padded.reshape(kb, 4, d)
+        halves = np.stack([parts[:, 0] + 1j * parts[:, 2], parts[:, 1] + 1j * parts[:, 3]], axis=2)     # [member][row][half]
+        msgs = np.zeros((parts.shape[0], self.lib.slots), dtype=np.complex128)
+        msgs[:, : 2 * d * d] = np.repeat(halves, d, axis=2).reshape(parts.shape[0], -1)
+        return CtxtTensor(self.lib.encrypt_many(msgs, level, nonces), d, d, 2 * d)
+
+    def matvec_q4(self, x, qweight):
+        """Encrypted vectors times a 4-bit matrix: one member per vector and column tile, one level below x; decrypt_vectors reads them."""
+        return CtxtTensor(self._call("matvec_q4", x.ct.ptr, qweight.ptr), *x.shape)
+
+    def decrypt_vectors(self, y, cols):
+        """The vectors that matvec_q4 made, [vectors][cols]."""
+        d = self.tile
+        nb, members = -(-cols // d), self.lib.ct_meta(y.ct)[2]
+        z = self.lib.decrypt_many([(y.ct, k) for k in range(members)])[:, : 2 * d].real
+        return (2.0 * (z[:, :d] + z[:, d:])).reshape(members // nb, nb * d)[:, :cols]
+
     def matmul_pre_rev(self, b, target_level=4):
         return CtxtTensor(self._call("matmul_pre_rev", b.ct.ptr, *self._shp(b), C.c_int(target_level)), *b.shape)
 

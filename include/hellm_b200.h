@@ -132,6 +132,22 @@ int hb_hemmer_matmul_reuse_groups(hb_hemmer *h, const hb_ct *pre, int btotal, in
 /* the same for `tiles` weights (pts[t * bcount + b]) that meet the same copies: out[t], t < tiles */
 int hb_hemmer_matmul_reuse_groups_tiles(hb_hemmer *h, const hb_ct *pre, int btotal, int b0, const hb_pt *const *pts, int bcount, int tiles,
                                         int width, hb_ct **out);
+/* Products grouped by expert (hb_matmul_acc_grouped): position p takes input order[p] (NULL: p) and the weights of the expert whose run of
+ * sizes[e] positions it lies in; copy k of K-group b of input i at batch position (k * inputs + i) * bcount + b of `pre`; member p * tiles + t of out. */
+int hb_hemmer_matmul_reuse_grouped(hb_hemmer *h, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts,
+                                   const hb_pt *const *pts, int bcount, int tiles, int width, hb_ct **out);
+/* Tiles against tiles of another number: out[j][hd][i] = sum over r < inner of a[r][hd][i] * b[r][hd][j] for `heads` heads, members in that order, at
+ * target_level; a needs target_level + 3 at least.  The shifted copies of a tile are made once for all its pairs.  cross_scores: b = the transposed key
+ * tiles, inner = 1 (schedule 2 transposes at target_level + 4, the others at the key's level).  No counterpart in the reference, whose sequences are one tile
+ * long. */
+int hb_hemmer_cross_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa, const hb_ct *b, int rb, int cb, int wb, int heads, int inner,
+                           int target_level, hb_ct **out);
+int hb_hemmer_cross_scores(hb_hemmer *h, const hb_ct *query, const hb_ct *key, int rows, int cols, int width, int heads, int target_level, hb_ct **out);
+/* Encrypted vectors times a matrix in 4 bits (hb_matvec_q4), rescaled and summed over the rows.  x: ceil(rows / 4 d) members a vector (d: the tile two of
+ * which fill a ciphertext), entry 4 d b + s of the vector in all columns of row s % d of member b: s < d left half, real part; s < 2 d right half, real
+ * part; s < 3 d left half, imaginary part; then right half, imaginary part.  out: one member per vector and column tile, in every row
+ * y / 2 = Re(left half) + Re(right half), one level below x. */
+int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct **out);
 /* HEMMer::matMulPreRev, matMulCCReUse (HEMMer.cpp:1114-1124; MatrixUtils.cpp:1641-1679) */
 int hb_hemmer_matmul_pre_rev(hb_hemmer *h, const hb_ct *b, int rows, int cols, int width, int target_level, hb_ct **out);
 int hb_hemmer_matmul_cc_reuse(hb_hemmer *h, const hb_ct *pre, const hb_ct *b, int rows, int cols, int width, hb_ct **out);
