@@ -22,8 +22,9 @@ struct ExpertList {
     int pos0;                                 // member positions before this launch's first
     int input[kExpertPositions];              // which input a position has
 };
-// CTAs of four warps that an SM holds: their registers have the sums
-template <int M, int T> constexpr int kExpertCtas = M * T > 8 ? 2 : M * T > 3 ? 3 : 4;
+// CTAs of four warps that an SM holds.  Blocks of nine to twelve sums a polynomial keep some words outside the registers with three CTAs; with two they do not and are slower (eight positions
+// at two of three experts, twelve tiles 9.9 / 9.6 ms, five at four, six tiles 1.95 / 1.77).
+template <int M, int T> constexpr int kExpertCtas = M * T > 3 ? 3 : 4;
 constexpr int kExpertRing = 4;
 template <int M, int T> constexpr size_t expert_smem() { return (size_t)4 * kExpertRing * (2 * M + T) * 256; }
 // pre [copies][inputs][bcount][2][n][N].  Four warps side by side, 32 residues each.  grid = (N / 128 * blocks, n)
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(128, kExpertCtas<M, T>) k_matmul_experts(u64 *
             if (q + t < tn) o[((size_t)(p + i) * el.out_tiles + q + t) * 2 * poly + k * poly] = sum.finish(m);
         });
     };
-    // as many positions as there are; modulo long primes as many sums at once as find room in the registers
+    // as many positions as there are; modulo long primes, whose sums take more registers, one position and at most four tiles at a time
     constexpr std::integral_constant<int, 1> one{};
     constexpr std::integral_constant<int, (M > 1 ? 2 : 1)> two{};
     if (m.fp) {
@@ -146,11 +147,8 @@ __global__ void __launch_bounds__(128, kExpertCtas<M, T>) k_matmul_experts(u64 *
     } else {
         constexpr int TT = T > 4 ? T / 2 : T;
         constexpr std::integral_constant<int, TT> some{};
-        for (int q = 0; q < T; q += TT) {
-            int p = 0;
-            if constexpr (kExpertCtas<M, T> == 2) for (; p + 1 < pn; p += 2) body(two, some, p, q, PieceSums{});
-            for (; p < pn; ++p) body(one, some, p, q, PieceSums{});
-        }
+        for (int q = 0; q < T; q += TT)
+            for (int p = 0; p < pn; ++p) body(one, some, p, q, PieceSums{});
     }
 }
 

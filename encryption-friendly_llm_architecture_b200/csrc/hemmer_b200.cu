@@ -1034,7 +1034,7 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
             auto begin = [&] { el.experts = 0; el.tiles = tn; el.bcount = bcount; el.out_tiles = tiles; el.tile0 = tile0; el.first_pos[0] = 0; el.pos0 = (int)next; };
             auto flush = [&] {
                 if (!el.experts) return;
-                const int M = expert_positions(el.experts, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; }), T = expert_tiles(M, tn);
+                const int M = expert_positions(el.experts, tn, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; }), T = expert_tiles(M, tn);
                 el.first_block[0] = 0;
                 for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + M - 1) / M * ((tn + T - 1) / T);
                 auto go = [&](auto m, auto t) { launch_experts<decltype(m)::value, decltype(t)::value>(c, el, pre, r->d, copies, inputs, gal); };

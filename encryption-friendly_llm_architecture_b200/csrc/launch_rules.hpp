@@ -91,20 +91,21 @@ constexpr int streamed_polynomials(int terms, int parts) {
     return line > 10 ? line : 10;
 }
 
-// Products grouped by expert: positions (M) and output tiles (T) of a block.  A lane keeps 2 M T sums, and a block of fewer positions than M does their work alone,
-// but in the registers of M.
+// Products grouped by expert: positions (M) and output tiles (T) of a block.  A lane keeps 2 M T sums; a block of fewer positions than M does the work of those it has.
 constexpr int expert_tiles(int M, int tiles) { // even blocks of at most eight, six or four tiles; there are none of five and seven
     const int most = M == 1 ? 8 : M == 2 ? 6 : 4, blocks = (tiles + most - 1) / most, t = (tiles + blocks - 1) / blocks;
     return t == 5 || t == 7 ? t + 1 : t;
 }
-template <class SIZE> constexpr int expert_positions(int experts, SIZE &&size) {
+// The products count, those of tiles past the end with them; among equals the blocks, which start one by one, and the words copied.  Experts of 128 copies at
+// level 5, us with one, two and three positions: 3 positions of 12 tiles 2175 2026 1844, 4 of 12 2887 2495 2640, 8 of 6 3063 2674 2885, 5 of 1 873 775 708, 1 of 8 482 559 547.
+template <class SIZE> constexpr int expert_positions(int experts, int tiles, SIZE &&size) {
     long cost[4] = {};
-    for (int e = 0; e < experts; ++e)
-        for (int M = 1; M <= 3; ++M) {
-            const int n = size(e), rest = n % M;
-            const int whole[4] = {0, 100, 165, 228}, part[4][3] = {{}, {}, {0, 108, 0}, {0, 115, 190}};
-            cost[M] += (long)(n / M) * whole[M] + part[M][rest];
-        }
+    for (int M = 1; M <= 3; ++M) {
+        const int T = expert_tiles(M, tiles);
+        auto block = [&](int p) { return 42 * p * T + 2 * p + T + 20 + (p < M && p == 1 ? 5 : 0); };
+        for (int e = 0; e < experts; ++e) cost[M] += (long)(size(e) / M) * block(M) + (size(e) % M ? block(size(e) % M) : 0);
+        cost[M] *= (tiles + T - 1) / T;
+    }
     return cost[3] < cost[2] && cost[3] < cost[1] ? 3 : cost[2] < cost[1] ? 2 : 1;
 }
 

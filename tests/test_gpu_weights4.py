@@ -90,6 +90,24 @@ def test_operands_of_other_tiles(gpu_small, tile):
         assert np.array_equal(g.pt_export(got[k]), g.pt_export(g.encode(_slots(w, tile, k % kb, k // kb, True, g.slots), 1))), k
 
 
+@pytest.mark.parametrize("ring", ["small", "full"])
+@pytest.mark.parametrize("bits", [0, 6, 12, 16, 40, 100])
+def test_operands_of_large_scales(request, ring, bits):
+    """Coefficients on both sides of the magnitudes after which they are reduced another way (2^44, 2^50), and past 63 bits, where they are what hb_encode makes of them."""
+    g = request.getfixturevalue("gpu_" + ring)
+    d = _tile(g)
+    codes, scales, _ = _matrix(4 * d + 5, d + 3, 16, bits)
+    scales = (scales.astype(np.float64) * 2.0**bits).astype(np.float32)
+    scales[0, 1] = np.float32(2.0**bits * 3)  # a few coefficients' worth above the others
+    code = np.empty((2 * codes.shape[0], codes.shape[1]))
+    code[0::2], code[1::2] = codes & 15, codes >> 4
+    w = (code[: 4 * d + 5] - 8) * np.repeat(scales.astype(np.float64), 16, axis=0)[: 4 * d + 5]
+    qw = g.qweight(codes, scales, 4 * d + 5, 16)
+    got = g.encode_q4(qw, d, 0, 4, 2)
+    for j, b in np.ndindex(2, 2):
+        assert np.array_equal(g.pt_export(got[j * 2 + b]), g.pt_export(g.encode(_slots(w, d, b, j, True, g.slots), 2))), (j, b)
+
+
 def _operand_sums(g, x, operands, kb, nb, at):
     """sum_b x[v][b] (.) p[j][b] in Python's integers"""
     n = x.shape[2]
