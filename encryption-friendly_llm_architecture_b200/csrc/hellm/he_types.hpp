@@ -306,6 +306,9 @@ class Evaluator {
     }
     // products grouped by expert: pts[(e * tiles + t) * bcount + b], member p * tiles + t of the result; order empty: position p has input p
     Ciphertext matmulGrouped(const Ciphertext &pre, int inputs, const std::vector<int32_t> &order, const std::vector<int32_t> &sizes, const std::vector<const hb_pt *> &pts, int bcount, int tiles, i64 row_step) const {
+        i64 positions = 0;
+        for (int32_t k : sizes) positions += k;
+        if ((!order.empty() && (i64)order.size() != positions) || (i64)pts.size() != (i64)sizes.size() * tiles * bcount) throw std::invalid_argument("[matmulGrouped] an order or weights of another number");
         hb_ct *o = nullptr;
         check(c_, hb_matmul_acc_grouped(c_, pre.raw(), inputs, order.empty() ? nullptr : order.data(), sizes.data(), (int)sizes.size(), pts.data(), bcount, tiles, row_step, &o));
         return Ciphertext(c_, o);

@@ -223,7 +223,7 @@ int hb_hemmer_cross_scores(hb_hemmer *h, const hb_ct *query, const hb_ct *key, i
 }
 int hb_hemmer_matmul_reuse_grouped(hb_hemmer *h, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts, const hb_pt *const *pts, int bcount, int tiles, int width,
                                    hb_ct **out) {
-    return guard([&] { hb_ct *o = nullptr; check(h->ctx, hb_matmul_acc_grouped(h->ctx, pre, inputs, order, sizes, experts, pts, bcount, tiles, width, &o)); *out = o; });
+    return guard([&] { check(h->ctx, hb_matmul_acc_grouped(h->ctx, pre, inputs, order, sizes, experts, pts, bcount, tiles, width, out)); });
 }
 int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct **out) {
     return guard([&] {

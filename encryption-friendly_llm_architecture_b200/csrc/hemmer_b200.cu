@@ -1264,11 +1264,13 @@ void embed_inverse(hb_ctx *c, i64 *coef, const double *re, const double *im, int
     }
 }
 // ---- plaintext operands from 4-bit weights ----
-constexpr size_t kMatvecBytes = (size_t)48 << 20;
+constexpr size_t kMatvecBytes = (size_t)48 << 20; // operands of a launch of k_matvec, which reads them from L2 (126 MB, with the words of x)
 struct Tiles4 { int kb, nb; }; // K-groups of four row tiles, column tiles
 Tiles4 tiles4(const hb_ctx *c, const hb_qweight *w, int d) {
     if (d < 1 || (i64)2 * d * d > c->h->slots) fail(HB_E_SHAPE, "4-bit weights: two tiles of that side do not fit the slots");
-    return {(int)((w->w.rows + (i64)4 * d - 1) / ((i64)4 * d)), (int)((w->w.cols + (i64)d - 1) / d)};
+    const i64 kb = (w->w.rows + (i64)4 * d - 1) / ((i64)4 * d), nb = (w->w.cols + (i64)d - 1) / d;
+    if (kb * nb > INT32_MAX) fail(HB_E_LIMIT, "4-bit weights: too many blocks"); // their numbers are ints
+    return {(int)kb, (int)nb};
 }
 Blocks4 blocks4(const hb_qweight *w, int d, int kb, bool diagonal, int first) {
     const u64 two32 = (u64)1 << 32, per = 2 * (u64)d, group = (u64)w->w.group;
@@ -1283,17 +1285,15 @@ void coefficients4(hb_ctx *c, const hb_qweight *w, const Blocks4 &b, int count, 
         launch(c, k_embed_inv_rows, dim3(16, (unsigned)count), kEmbThreads, 0, coef, (const double2 *)v.p, sc, c->emb_tb);
     } else launch(c, k_weight_small, dim3((unsigned)count), 256, 0, coef, w->w, b, c->logn - 1, sc, c->emb_tb);
 }
-// residues of the limbs l0 .. l0 + limbs - 1, transform order, as those limbs of the members of `to`
+// residues of the limbs l0 .. l0 + limbs - 1, transform order, one after the other in the members of `to`
 void transform4(hb_ctx *c, const PtList &to, const i64 *coef, int count, int l0, int limbs) {
     LimbMap map{};
     map.n = limbs;
     for (int i = 0; i < limbs; ++i) map.prime[i] = (unsigned char)(l0 + i);
-    if (c->logn != 16) { launch(c, k_coef_small, dim3((unsigned)limbs, (unsigned)count), 256, sizeof(u64) << c->logn, to, l0, coef, map, c->pc, c->tb, c->logn); return; }
-    PtList rows = to;
-    for (int i = 0; i < count; ++i) rows.p[i] += (size_t)l0 * c->N;
+    if (c->logn != 16) { launch(c, k_coef_small, dim3((unsigned)limbs, (unsigned)count), 256, sizeof(u64) << c->logn, to, coef, map, c->pc, c->tb, c->logn); return; }
     auto passes = [&](auto *cols, auto *second) {
-        launch(c, cols, dim3(16, (unsigned)(count * limbs)), 256, 0, to, l0, coef, map, c->pc, c->tb.t16);
-        launch(c, second, dim3(16, (unsigned)(count * limbs)), 256, 0, (const u64 *)nullptr, rows, (u64 *)nullptr, rows, map, c->pc, c->tb.t16);
+        launch(c, cols, dim3(16, (unsigned)(count * limbs)), 256, 0, to, coef, map, c->pc, c->tb.t16);
+        launch(c, second, dim3(16, (unsigned)(count * limbs)), 256, 0, (const u64 *)nullptr, to, (u64 *)nullptr, to, map, c->pc, c->tb.t16);
     };
     if (c->tb.t16.pm) passes(k_coef_cols<LongPm>, ntt16v2_fwd_rows<4, LongPm, PtList>);
     else passes(k_coef_cols<LongShoup>, ntt16v2_fwd_rows<4, LongShoup, PtList>);
@@ -1775,7 +1775,7 @@ int hb_matvec_q4(hb_ctx *c, const hb_ct *x, const hb_qweight *w, int tile, hb_ct
                     for (int k = 0; k < blocks; k += kBlocks4) {
                         const int some = std::min(kBlocks4, blocks - k);
                         PtList to{};
-                        for (int i = 0; i < some; ++i) to.p[i] = p.p + ((size_t)(k + i) * limbs - l0) * N;
+                        for (int i = 0; i < some; ++i) to.p[i] = p.p + (size_t)(k + i) * limbs * N;
                         transform4(c, to, (const i64 *)coef.p + (size_t)k * N, some, l0, limbs);
                     }
                     const MatvecShape s{vectors, t.kb, m, t.nb, j, n, l0};

@@ -49,7 +49,9 @@ struct PtList {
     __device__ __forceinline__ size_t off(int li, int period) const { return (size_t)(at(li / period, li % period, kN16) - (u64 *)nullptr); } // from a null base: the address of ntt16.cuh
 };
 // ---- slots -> coefficients: k_embed_inv_cols and k_embed_inv_small with the slots made on the way ----
-// half-transformed slots v [count][2^15].  grid = (16, count)
+// half-transformed slots v [count][2^15].  12 blocks of 768 x 768: 14.5 us, one wave of CTAs whose time is the latency of codes and scales and of two rounds of butterflies (10 us
+// of it, the time of the row pass); 36 blocks 36 us.  The slots written first and read again by the column pass: 366 us for 36 plaintexts at level 5, 226 with them made here and
+// the reduction in the column pass below.  grid = (16, count)
 __global__ void __launch_bounds__(kEmbThreads) k_weight_cols(double2 *v, const __grid_constant__ Weights4 w, const __grid_constant__ Blocks4 b, EmbedTables tb) {
     __shared__ double2 sm[kEmbRows * 8];
     const int lane = threadIdx.x & 7, sub = threadIdx.x >> 3, col = blockIdx.x * 8 + lane;
@@ -93,17 +95,19 @@ __global__ void __launch_bounds__(256) k_weight_small(i64 *coef, const __grid_co
     }
 }
 // ---- coefficients -> residues in transform order ----
-// The column pass of ntt16v2_fwd_cols on coefficients coef [count][2^16], reduced on the way: a pass over the residues of every limb less.  Limbs l0 .. of the members of `to`; map
-// names their primes.  32 members at level 5, with the reduction apart: 97 us, 45 with it (the butterflies hide behind nothing: FP64 bound).  grid = (16, count * map.n)
+// The column pass of ntt16v2_fwd_cols on coefficients coef [count][2^16], reduced on the way: a pass over the residues of every limb less (64 limbs: 19 us, the pass and the
+// reduction apart 15 and 17; 216 limbs of 36 members 52 us).  Bound by the FP64 instructions of the butterflies and the wait between its two rounds.  One test of the
+// magnitudes of all sixteen coefficients stands before the reductions, which would wait for a branch each.  map names the primes of the limbs of a member.
+// grid = (16, count * map.n)
 template <class LONG>
-__global__ void __launch_bounds__(256, 4) k_coef_cols(const __grid_constant__ PtList to, int l0, const i64 *coef, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, Ntt16Tables tb) {
+__global__ void __launch_bounds__(256, 4) k_coef_cols(const __grid_constant__ PtList to, const i64 *coef, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, Ntt16Tables tb) {
     __shared__ u64 sm[4096];
     const int member = blockIdx.y / map.n, li = blockIdx.y % map.n, pi = map.prime[li];
     const PrimeConst m = pc[pi];
     const ulonglong2 *tab = tb.fwd + (size_t)pi * Ntt16Layout::kEntries;
     const int tid = threadIdx.x, lane = tid & 15, sub = tid >> 4;
     const i64 *p = coef + (size_t)member * kN16 + blockIdx.x * 16 + lane;
-    u64 *o = to.at(member, l0 + li, kN16) + blockIdx.x * 16 + lane;
+    u64 *o = to.at(member, li, kN16) + blockIdx.x * 16 + lane;
     i64 a[16];
     u64 large = 0; // the magnitudes' bits: as a rule the coefficients are far below 2^44
     pdl_wait();
@@ -150,13 +154,13 @@ __global__ void __launch_bounds__(256, 4) k_coef_cols(const __grid_constant__ Pt
     }
 }
 // the whole transform of a small ring's limb: ntt_small on coefficients.  grid = (map.n, count)
-__global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtList to, int l0, const i64 *coef, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, NttTables tb, int logn) {
+__global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtList to, const i64 *coef, const __grid_constant__ LimbMap map, const PrimeConst *__restrict__ pc, NttTables tb, int logn) {
     extern __shared__ u64 sm_dyn[];
     const int N = 1 << logn, pi = map.prime[blockIdx.x];
     const PrimeConst m = pc[pi];
     const u64 q = m.q, q2 = q << 1;
     const i64 *p = coef + (size_t)blockIdx.y * N;
-    u64 *o = to.at(blockIdx.y, l0 + blockIdx.x, N);
+    u64 *o = to.at(blockIdx.y, blockIdx.x, N);
     const u64 *w = tb.psi + (size_t)pi * N, *ws = tb.psi_sh + (size_t)pi * N;
     pdl_wait();
     for (int i = threadIdx.x; i < N; i += 256) sm_dyn[i] = reduce_i64_any(p[i], m);
@@ -176,8 +180,9 @@ __global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtLi
 }
 // ---- products ----
 // out[v][j] = sum_b x[v][b] (.) p[j][b]: x [vectors][kb][2][n][N], operands p [columns][kb][limbs][N] of the limbs l0 .. and the columns j0 .., out [vectors][nb][2][n][N].  A thread has one
-// coefficient of both polynomials of V vectors and of C columns: 2 V + C words for 2 V C products, as many in flight.  Bound by the words of x and of the results.  The blocks of one
-// range of coefficients run side by side.  grid = (N / 256 * blocks, limbs)
+// coefficient of both polynomials of V vectors and of C columns: 2 V + C words for 2 V C products, as many in flight.  The blocks of one
+// range of coefficients run side by side.  Four vectors, 2048 x 2048, 4 K-groups: 40 us a limb, 68 MB of results and 17 MB of x in it (13 us of HBM), the rest the wait for the words of a
+// K-group (FP64 36 % active).  The words of the next K-group in flight during the products: 517 us for the whole call without, 557 to 661 with, since the registers cost warps.  grid = (N / 256 * blocks, limbs)
 struct MatvecShape { int vectors, kb, columns, nb, j0, n, l0; };
 template <int V, int C>
 __global__ void __launch_bounds__(256, 2) k_matvec(u64 *out, const u64 *x, const u64 *p, MatvecShape s, const PrimeConst *__restrict__ pc, int N) {

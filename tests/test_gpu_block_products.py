@@ -2,6 +2,8 @@
 4-bit weights, encrypted vectors times a 4-bit matrix, and a run of them together.
 
 Decrypted values may be off by 2^-14, the bound that every decrypted product of this repository is held to; sums over r tiles by r times that."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -132,6 +134,18 @@ def test_matvec_refuses_other_batches(pkg, fast):
     ct = h.encrypt_vectors(rng.uniform(-1, 1, (1, 100)), 3, [1])
     with pytest.raises(pkg.HBError):
         h.matvec_q4(ct, qw)
+
+
+def test_grouped_refuses_null_arguments(fast):
+    h = fast
+    f, pre = h._fn("matmul_reuse_grouped"), h.lib.ct_create(2, 2, 2, 1)
+    p = h.lib.encode(np.ones(4), 2)
+    arr, sizes, out = (C.c_void_p * 1)(p.ptr.value), (C.c_int32 * 1)(2), C.c_void_p()
+    args = lambda pre, sizes, arr, out: (h.h, pre, C.c_int(2), None, sizes, C.c_int(1), arr, C.c_int(1), C.c_int(1), C.c_int(2 * D), out)
+    assert f(*args(pre.ptr, sizes, arr, None)) != 0 and f(*args(None, sizes, arr, C.byref(out))) != 0
+    assert f(*args(pre.ptr, None, arr, C.byref(out))) != 0 and f(*args(pre.ptr, sizes, None, C.byref(out))) != 0
+    assert out.value is None and f(*args(pre.ptr, sizes, arr, C.byref(out))) == 0
+    type(p)(h.lib, out, "ct")
 
 
 def test_a_block_of_them(fast):
