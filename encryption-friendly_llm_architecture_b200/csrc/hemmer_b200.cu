@@ -1736,14 +1736,13 @@ int hb_encode_q4(hb_ctx *c, const hb_qweight *w, int tile, int diagonal, int fir
         if (first < 0 || count < 1 || (i64)first + count > (i64)t.kb * t.nb) fail(HB_E_ARG, "encode_q4: blocks that are not there");
         std::vector<hb_pt *> r((size_t)count, nullptr);
         try {
-            for (hb_pt *&p : r) p = new_pt(c, level, 1);
             ALG(c, (size_t)count * (level + 1));
             for (int k = 0; k < count; k += kBlocks4) {
                 const int m = std::min(kBlocks4, count - k);
                 TmpBytes coef(c, (size_t)m * c->N * sizeof(i64));
-                PtList to{};
-                for (int i = 0; i < m; ++i) to.p[i] = r[(size_t)(k + i)]->d;
                 coefficients4(c, w, blocks4(w, tile, t.kb, diagonal != 0, first + k), m, level, (i64 *)coef.p);
+                PtList to{}; // the plaintexts are made while the device is at work
+                for (int i = 0; i < m; ++i) to.p[i] = (r[(size_t)(k + i)] = new_pt(c, level, 1))->d;
                 transform4(c, to, (const i64 *)coef.p, m, 0, level + 1);
             }
         } catch (...) { for (hb_pt *p : r) hb_pt_free(p); throw; }

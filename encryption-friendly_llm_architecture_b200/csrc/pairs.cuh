@@ -6,9 +6,9 @@
 // word is read once for four products.  Its lanes are LR x LC blocks of TR x TC pairs, side by side for 32 / (LR LC) residues; the words of all its tiles come
 // through a ring of stages in shared memory that belongs to the warp alone (16-byte asynchronous copies, several groups ahead), from which every lane reads the
 // tiles of its block.  The ring runs on from one range of residues to the next.
-// 8 groups, 6 heads, 4 query and 8 key tiles at level 5: 1.27 ms (5.4 GB: 0.83 ms of HBM; FP64 0.45), bound by the copies and reads of the ring, which wait for one another in the
-// load-store unit.  Rings of 2, 3, 4, 6 and 8 stages: 1.95, 1.35, 1.30, 1.49 and 1.50 ms (with more copies in flight reads wait behind them).  One query tile with four key tiles: 267 us, 99 % of
-// the bandwidth.  Pair by pair the first takes 2.2 ms.  Twice as many pairs a warp (8 x 4, 168 registers): 1.5 ms.
+// 8 groups, 6 heads, 4 query and 8 key tiles at level 5: 1.27 ms, with 5.4 GB (0.83 ms of HBM), 0.4 ms of FP64 and the 60-bit limb, a sixth of the products and a quarter of the time, which
+// overlap in part.  Words straight to registers: 2.2 ms.  Rings of 2, 3, 4, 6 and 8 stages: 1.95, 1.35, 1.30, 1.49 and 1.50 ms (the reads of the ring wait behind the copies in flight).  Twice
+// as many pairs a warp (8 x 4, 168 registers): 1.5 ms; boxes of 64 residues by tensor-map copies and a ring of the CTA: 1.54 ms.  One query tile with four key tiles: 267 us, 99 % of the bandwidth.
 // The middle sum comes from one product of the sums, (b1 + a1)(b2 + a2), from which the outer two are taken off at the end: three products a pair.
 #pragma once
 #include "kernels.cuh"
