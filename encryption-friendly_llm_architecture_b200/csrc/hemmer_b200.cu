@@ -1074,8 +1074,9 @@ template <int TR, int TC, int LR, int LC> void launch_pairs(hb_ctx *c, int varia
         c->smem_opt_in_pairs[variant] = true;
     }
     const int n = level + 1, blocks = ((sides.nr + T::kRows - 1) / T::kRows) * ((sides.nc + T::kCols - 1) / T::kCols);
-    int run = 1; // ranges of a CTA: more of them, and the ring runs dry less often; but every SM wants several CTAs
-    while (run < 16 && c->N / (16 * T::kX * run) >= 1 && (i64)c->N / (16 * T::kX * run) * blocks * s.heads * n >= 148 * 8) run *= 2;
+    // ranges of a CTA: more of them, and the ring runs dry less often; but with few CTAs an SM those of the 60-bit limb end late (eight against eight tiles, two heads: 963 us with at least 8 an SM, 895 with 32)
+    int run = 1;
+    while (run < 16 && c->N / (16 * T::kX * run) >= 1 && (i64)c->N / (16 * T::kX * run) * blocks * s.heads * n >= 148 * 32) run *= 2;
     launch(c, k_tensor_pairs<TR, TC, LR, LC>, dim3((unsigned)(c->N / (8 * T::kX * run)) * (unsigned)blocks, (unsigned)(s.heads * n)), 256, T::kSmem, d, sides, s, run, n, c->qmap(level), c->pc, c->N,
            accumulate ? 1 : 0);
 }
