@@ -1265,7 +1265,9 @@ void embed_inverse(hb_ctx *c, i64 *coef, const double *re, const double *im, int
     }
 }
 // ---- plaintext operands from 4-bit weights ----
-constexpr size_t kMatvecBytes = (size_t)48 << 20; // operands of a launch of k_matvec, which reads them from L2 (126 MB, with the words of x)
+// Operands that a launch of k_matvec reads: an upper bound of the call's memory.  Fewer of them, that stay in L2, are slower, since their passes are launches of one or two waves each: 2048 x 2048
+// (33 MB a limb), at most 48, 210 and 512 MB: four vectors at level 5 518, 479 and 479 us, one at level 12 687, 637 and 615.
+constexpr size_t kMatvecBytes = (size_t)512 << 20;
 struct Tiles4 { int kb, nb; }; // K-groups of four row tiles, column tiles
 Tiles4 tiles4(const hb_ctx *c, const hb_qweight *w, int d) {
     if (d < 1 || (i64)2 * d * d > c->h->slots) fail(HB_E_SHAPE, "4-bit weights: two tiles of that side do not fit the slots");
@@ -1762,7 +1764,7 @@ int hb_matvec_q4(hb_ctx *c, const hb_ct *x, const hb_qweight *w, int tile, hb_ct
         hb_ct *r = new_ct(c, x->level, 2, vectors * t.nb, 2);
         try {
             ALG(c, x->limbs() + r->limbs());
-            // columns whose operands make one launch (a column of many K-groups several), and as many limbs at once as stay in L2 with them: x is read once per set of columns
+            // columns whose operands make one launch (a column of many K-groups several), and as many limbs at once as the bound allows: x is read once per set of columns
             const int columns = std::max(1, kBlocks4 / t.kb), N = c->N;
             for (int j = 0; j < t.nb; j += columns) {
                 const int m = std::min(columns, t.nb - j), blocks = m * t.kb, at_once = (int)std::clamp<size_t>(kMatvecBytes / ((size_t)blocks * N * 8), 1, (size_t)n);

@@ -181,8 +181,8 @@ __global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtLi
 // ---- products ----
 // out[v][j] = sum_b x[v][b] (.) p[j][b]: x [vectors][kb][2][n][N], operands p [columns][kb][limbs][N] of the limbs l0 .. and the columns j0 .., out [vectors][nb][2][n][N].  A thread has one
 // coefficient of both polynomials of V vectors and of C columns: 2 V + C words for 2 V C products, as many in flight.  The blocks of one
-// range of coefficients run side by side.  Four vectors, 2048 x 2048, 4 K-groups: 40 us a limb, 68 MB of results and 17 MB of x in it (13 us of HBM), the rest the wait for the words of a
-// K-group (FP64 36 % active).  The words of the next K-group in flight during the products: 517 us for the whole call without, 557 to 661 with, since the registers cost warps.  grid = (N / 256 * blocks, limbs)
+// range of coefficients run side by side.  Four vectors, 2048 x 2048, 4 K-groups: 40 us a limb, 68 MB of results and 17 MB of x in it (13 us of HBM, 18 with the operands), the rest the wait for the words of a
+// K-group (FP64 36 % active).  The words of the next K-group in flight during the products: 518 us for the whole call without, 557 to 661 with (at 48 MB of operands a launch), since the registers cost warps.  grid = (N / 256 * blocks, limbs)
 struct MatvecShape { int vectors, kb, columns, nb, j0, n, l0; };
 template <int V, int C>
 __global__ void __launch_bounds__(256, 2) k_matvec(u64 *out, const u64 *x, const u64 *p, MatvecShape s, const PrimeConst *__restrict__ pc, int N) {
