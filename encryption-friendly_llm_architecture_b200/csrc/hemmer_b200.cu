@@ -1302,7 +1302,7 @@ void transform4(hb_ctx *c, const PtList &to, const i64 *coef, int count, int l0,
     else passes(k_coef_cols<LongShoup>, ntt16v2_fwd_rows<4, LongShoup, PtList>);
 }
 template <int V, int C> void launch_matvec(hb_ctx *c, u64 *out, const u64 *x, const u64 *p, const MatvecShape &s, int limbs) {
-    launch(c, k_matvec<V, C>, dim3((unsigned)(c->N / 256) * (unsigned)(((s.vectors + V - 1) / V) * ((s.columns + C - 1) / C)), (unsigned)limbs), 256, 0, out, x, p, s, c->pc, c->N);
+    launch(c, k_matvec<V, C>, dim3((unsigned)(c->N / 128) * (unsigned)(((s.vectors + V - 1) / V) * ((s.columns + C - 1) / C)), (unsigned)limbs), 128, 0, out, x, p, s, c->pc, c->N);
 }
 // slot values of the residues t [count][2][N]: member b, slot s at re[(b * slots + s) * stride], im likewise
 void embed_forward(hb_ctx *c, double *re, double *im, int stride, const u64 *t, const DecItem *items, int count) {

@@ -181,14 +181,15 @@ __global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtLi
 // ---- products ----
 // out[v][j] = sum_b x[v][b] (.) p[j][b]: x [vectors][kb][2][n][N], operands p [columns][kb][limbs][N] of the limbs l0 .. and the columns j0 .., out [vectors][nb][2][n][N].  A thread has one
 // coefficient of both polynomials of V vectors and of C columns: 2 V + C words for 2 V C products, as many in flight.  The blocks of one
-// range of coefficients run side by side.  Four vectors, 2048 x 2048, 4 K-groups: 40 us a limb, 68 MB of results and 17 MB of x in it (13 us of HBM, 18 with the operands), the rest the wait for the words of a
-// K-group (FP64 36 % active).  The words of the next K-group in flight during the products: 518 us for the whole call without, 557 to 661 with (at 48 MB of operands a launch), since the registers cost warps.  grid = (N / 256 * blocks, limbs)
+// range of coefficients run side by side.  Four vectors, 2048 x 2048, 4 K-groups: 36 us a limb, 68 MB of results and 17 MB of x in it (13 us of HBM, 18 with the operands), the rest the wait for
+// the words of a K-group (FP64 36 % active).  The whole call in CTAs of 128 threads and two K-groups a turn against 256 threads and one: four vectors 479 -> 463 us, one 325 -> 298,
+// one of 32 K-groups 736 -> 620; with the words of the next K-group in flight as well 505, 321 and 708, since the registers cost warps.  grid = (N / 128 * blocks, limbs)
 struct MatvecShape { int vectors, kb, columns, nb, j0, n, l0; };
 template <int V, int C>
-__global__ void __launch_bounds__(256, 2) k_matvec(u64 *out, const u64 *x, const u64 *p, MatvecShape s, const PrimeConst *__restrict__ pc, int N) {
+__global__ void __launch_bounds__(128, V == 1 ? 5 : 3) k_matvec(u64 *out, const u64 *x, const u64 *p, MatvecShape s, const PrimeConst *__restrict__ pc, int N) {
     const int bv = (s.vectors + V - 1) / V, blocks = bv * ((s.columns + C - 1) / C), blk = blockIdx.x % blocks, v0 = blk % bv * V, c0 = blk / bv * C, l = s.l0 + blockIdx.y, limbs = gridDim.y;
     const PrimeConst m = pc[l];
-    const u32 at = blockIdx.x / blocks * 256 + threadIdx.x;
+    const u32 at = blockIdx.x / blocks * 128 + threadIdx.x;
     const size_t poly = (size_t)s.n * N, limb = (size_t)limbs * N;
     const u64 *xp[V], *pp[C];
 #pragma unroll
@@ -202,8 +203,7 @@ __global__ void __launch_bounds__(256, 2) k_matvec(u64 *out, const u64 *x, const
         for (int i = 0; i < V; ++i)
 #pragma unroll
             for (int j = 0; j < C; ++j) { a[i][j][0].zero(); a[i][j][1].zero(); }
-#pragma unroll 1
-        for (int b = 0; b < s.kb; ++b) {
+        auto group = [&](int b) {
             u64 xv[V][2], pv[C];
 #pragma unroll
             for (int i = 0; i < V; ++i) { xv[i][0] = xp[i][0]; xv[i][1] = xp[i][poly]; xp[i] += 2 * poly; }
@@ -219,7 +219,11 @@ __global__ void __launch_bounds__(256, 2) k_matvec(u64 *out, const u64 *x, const
             for (int i = 0; i < V; ++i)
 #pragma unroll
                 for (int j = 0; j < C; ++j) { a[i][j][0].product(xv[i][0], pv[j]); a[i][j][1].product(xv[i][1], pv[j]); }
-        }
+        };
+        int b = 0;
+#pragma unroll 1
+        for (; b + 1 < s.kb; b += 2) { group(b); group(b + 1); } // FP64 sums change registers at every product
+        if (b < s.kb) group(b);
 #pragma unroll
         for (int i = 0; i < V; ++i)
 #pragma unroll
