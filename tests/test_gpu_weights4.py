@@ -169,6 +169,32 @@ def test_matvec_largest_residues(gpu_small, kb):
     assert np.array_equal(g.ct_export(g.matvec_q4(ct, qw, 1))[..., at].astype(object), _operand_sums(g, x, operands, kb, 2, at))
 
 
+OTHER_PRIMES = [dict(log_n=10, q_bits=43), dict(log_n=11, q_bits=59), dict(log_n=16, q_bits=44), dict(log_n=16, q0_bits=59), dict(log_n=16, q0_bits=58, q_bits=50, p_bits=58)]
+
+
+@pytest.mark.parametrize("prm", OTHER_PRIMES)
+def test_other_primes(pkg, prm):
+    """Primes of other lengths, and 60-bit ones whose transforms take Shoup products; coefficients of the usual size and large ones."""
+    g = pkg.open_gpu(pkg.make_params(num_special=3, hamming_weight=32, max_level=3, dnum=3, **prm))
+    try:
+        d = _tile(g)
+        codes, scales, w = _matrix(4 * d + 3, d + 1, 16, 3)
+        for factor in (1.0, 2.0**9):
+            qw = g.qweight(codes, (scales * np.float32(factor)).astype(np.float32), 4 * d + 3, 16)
+            got = g.encode_q4(qw, d, 0, 4, 3)
+            for j, b in np.ndindex(2, 2):
+                assert np.array_equal(g.pt_export(got[j * 2 + b]), g.pt_export(g.encode(_slots(factor * w, d, b, j, True, g.slots), 3))), (factor, j, b)
+        x = rand_ct_residues(g, 3, 2, 6, 9)
+        x[:2] = np.array([int(q) - 1 for q in g.primes[:4]], dtype=np.uint64)[None, None, :, None]
+        ct = g.ct_create(3, 2, 6, 1)
+        g.ct_import(ct, x)
+        at = np.unique(np.concatenate([[0, g.N - 1], np.random.default_rng(1).integers(0, g.N, 15)]))
+        operands = g.encode_q4(qw, d, 0, 4, 3, diagonal=False)
+        assert np.array_equal(g.ct_export(g.matvec_q4(ct, qw, d))[..., at].astype(object), _operand_sums(g, x, operands, 2, 2, at))
+    finally:
+        g.close()
+
+
 def test_recorded_encoding_and_matvec(gpu_small):
     """Neither copies from the host, so both can be recorded; the weights are kept as they were."""
     g, d = gpu_small, _tile(gpu_small)
