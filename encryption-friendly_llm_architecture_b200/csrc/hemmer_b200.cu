@@ -1034,9 +1034,14 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
             auto begin = [&] { el.experts = 0; el.tiles = tn; el.bcount = bcount; el.out_tiles = tiles; el.tile0 = tile0; el.first_pos[0] = 0; el.pos0 = (int)next; };
             auto flush = [&] {
                 if (!el.experts) return;
-                const int M = expert_positions(el.experts, tn, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; }), T = expert_tiles(M, tn);
-                el.first_block[0] = 0;
-                for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + M - 1) / M * ((tn + T - 1) / T);
+                int M = expert_positions(el.experts, tn, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; }), T = expert_tiles(M, tn);
+                auto lay = [&] {
+                    el.first_block[0] = 0;
+                    for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + M - 1) / M * ((tn + T - 1) / T);
+                };
+                lay();
+                const i64 each = (i64)(c->N / 128) * n;
+                if (each * el.first_block[el.experts] < 148 * 3) { M = 1; T = expert_tiles_few(el.first_pos[el.experts], tn, each); lay(); }
                 auto go = [&](auto m, auto t) { launch_experts<decltype(m)::value, decltype(t)::value>(c, el, pre, r->d, copies, inputs, gal); };
                 auto by_tiles = [&](auto m) {
                     constexpr int MM = decltype(m)::value;

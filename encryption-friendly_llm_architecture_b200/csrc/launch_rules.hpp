@@ -109,4 +109,12 @@ template <class SIZE> constexpr int expert_positions(int experts, int tiles, SIZ
     return cost[3] < cost[2] && cost[3] < cost[1] ? 3 : cost[2] < cost[1] ? 2 : 1;
 }
 
+// Small rings: where the blocks of all positions leave SMs without work, single positions and as many tiles (four at most) as still fill them.  `each`: CTAs of a block.  2^12
+// coefficients, 32 copies, us with the rule above alone and with this: 4 positions of 6 tiles, 3 K-groups, level 1 84 -> 60; 8 of 12 tiles, 2 K-groups, level 0 86 -> 75; 3 of one tile, level 1 22 -> 18.
+constexpr int expert_tiles_few(int positions, int tiles, long each) {
+    int T = tiles < 4 ? tiles : 4;
+    while (T > 1 && positions * ((tiles + T - 1L) / T) * each < 148 * 3) --T;
+    return T;
+}
+
 } // namespace hb

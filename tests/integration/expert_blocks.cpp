@@ -39,5 +39,12 @@ int main() {
             const int one = expert_positions(1, tiles, [&](int) { return p; }), many = expert_positions(7, tiles, [&](int e) { return e % 2 ? p : 0; });
             CHECK(one == many, "%d positions of %d tiles: %d alone, %d thrice\n", p, tiles, one, many);
         }
+    for (int p = 1; p < 300; ++p)
+        for (int tiles = 1; tiles < 40; ++tiles)
+            for (long each : {8L, 16L, 64L, 512L}) {
+                const int T = expert_tiles_few(p, tiles, each);
+                CHECK(T >= 1 && T <= 4 && T <= tiles, "%d positions of %d tiles, %ld CTAs each: %d\n", p, tiles, each, T);
+                CHECK(T == 1 || p * ((tiles + T - 1L) / T) * each >= 148 * 3, "%d positions of %d tiles, %ld CTAs each: %d do not fill the GPU\n", p, tiles, each, T);
+            }
     return bad != 0;
 }
