@@ -45,8 +45,11 @@ Message paint(const Env &e, const TileTensorShape &s, const Placement &pl, i64 r
             if (!pred(r, c)) continue;
             for (const auto &o : pl.origins)
                 for (i64 dr = 0; dr < pl.row_scale; ++dr)
-                    for (i64 dc = 0; dc < pl.col_scale; ++dc)
-                        m.re[(size_t)((o.first + pl.row_scale * r + dr) * w + o.second + pl.col_scale * c + dc)] = value;
+                    for (i64 dc = 0; dc < pl.col_scale; ++dc) {
+                        const i64 at = (o.first + pl.row_scale * r + dr) * w + o.second + pl.col_scale * c + dc;
+                        if (at >= e.slots) throw std::invalid_argument("[masks] tiles of that shape reach past the slots"); // e.g. 20 rows or columns, which no grid is a multiple of
+                        m.re[(size_t)at] = value;
+                    }
         }
     return m;
 }
