@@ -140,7 +140,8 @@ class HEMMer {
     CtxtTensor ccMatMulCore(Ciphertext sigma_a, Ciphertext tau_b, i64 rows, i64 inner, i64 cols, i64 width, int target_level);
     // Products of tiles with tiles of another number (the reference's sequences are one tile long): for every head h, query tile i and key tile j the
     // product sum over r < inner of a[r][h][i] * b[r][h][j], members in that order; the result's are [j][h][i], so that scores can be the left operand
-    // of the product with the values (inner = key tiles).  crossScores transposes the key tiles first.
+    // of the product with the values (inner = key tiles).  Rows of a and columns of b divide the inner side of the tiles (rounded up to a power of two); tiles with
+    // a shorter one are padded with zeros.  crossScores transposes the key tiles first.
     CtxtTensor crossMatMul(const CtxtTensor &a, const CtxtTensor &b, int heads = 1, int inner = 1, int target_level = 4);
     CtxtTensor crossScores(const CtxtTensor &query, const CtxtTensor &key, int heads = 1, int target_level = 4);
     // Encrypted vectors times a matrix in 4 bits (hb_qweight): x has ceil(rows / 4 tile) members a vector, entry 4 tile b + s of it in all columns of row

@@ -501,6 +501,10 @@ CtxtTensor multCross(Env &e, const CtxtTensor &op1, const CtxtTensor &op2, int h
     const auto whole = [&](const CtxtTensor &t) { return heads > 0 && inner > 0 && t.get().getBatch() % ((i64)heads * inner) == 0; };
     if (!whole(op1) || !whole(op2)) throw std::invalid_argument("[multCross] a batch does not split into that many heads and inner tiles");
     const i64 num_rows = op1.getHeight(), num_cols = op2.getWidth(), width = op1.getBlockWidth(), num_k = ceil_pow2(op1.getWidth());
+    // sigma and tau turn rows and columns by up to the tile's side, the sum has num_k terms: a side longer than the inner one meets columns of the wrong row
+    // (32 x 16 times 16 x 16 is off by whole entries, as in the reference's formula).  The caller pads the inner side with zeros.
+    if (width < 1 || e.slots % width || num_rows < 1 || num_cols < 1 || num_k > width || num_k > e.slots / width || num_k % num_rows || num_k % num_cols)
+        throw std::invalid_argument("[multCross] rows and columns must divide the inner side, rounded up to a power of two, which fits the block width and the slots");
     const int lvl = target_level + 2;
     Ciphertext a, b, acc;
     ccmmPrepare(e, op1, op2, target_level, a, b);

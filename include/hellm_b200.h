@@ -137,7 +137,8 @@ int hb_hemmer_matmul_reuse_groups_tiles(hb_hemmer *h, const hb_ct *pre, int btot
 int hb_hemmer_matmul_reuse_grouped(hb_hemmer *h, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts,
                                    const hb_pt *const *pts, int bcount, int tiles, int width, hb_ct **out);
 /* Tiles against tiles of another number: out[j][hd][i] = sum over r < inner of a[r][hd][i] * b[r][hd][j] for `heads` heads, members in that order, at
- * target_level; a needs target_level + 3 at least.  The shifted copies of a tile are made once for all its pairs.  cross_scores: b = the transposed key
+ * target_level; a needs target_level + 3 at least.  ra and cb divide ca, rounded up to a power of two, which is wb at most: tiles whose inner side is shorter
+ * than their rows or columns are padded with zeros (HB_E_ARG otherwise).  The shifted copies of a tile are made once for all its pairs.  cross_scores: b = the transposed key
  * tiles, inner = 1 (schedule 2 transposes at target_level + 4, the others at the key's level).  No counterpart in the reference, whose sequences are one tile
  * long. */
 int hb_hemmer_cross_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa, const hb_ct *b, int rb, int cb, int wb, int heads, int inner,
