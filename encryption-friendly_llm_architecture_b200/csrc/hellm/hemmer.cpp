@@ -110,6 +110,8 @@ CtxtTensor HEMMer::ccMatMulCore(Ciphertext sa, Ciphertext tb, i64 rows, i64 inne
 }
 CtxtTensor HEMMer::crossMatMul(const CtxtTensor &a, const CtxtTensor &b, int heads, int inner, int t) { HB_ENV; return sched::multCross(env, a, b, heads, inner, t); }
 CtxtTensor HEMMer::crossScores(const CtxtTensor &query, const CtxtTensor &key, int heads, int t) {
+    // transpose() takes a tile whose rows are fewer than the block width for the first of two, and paints the second one's masks into the next row if there is no room for it
+    if (key.getHeight() != key.getBlockWidth() && key.getHeight() + key.getWidth() > key.getBlockWidth()) throw std::invalid_argument("[crossScores] a key tile alone has as many rows as its block width: pad it with zeros");
     CtxtTensor turned(key.getShape(), eval_.view(key.get(), 0, key.get().getBatch()));
     transposeInplace(turned, schedule_ == sched::kLazy ? t + 3 : 0); // in the fast schedule at the lowest level that leaves enough for the product
     return crossMatMul(query, turned, heads, 1, t);

@@ -76,3 +76,11 @@ def test_empty_tiles(pkg, hemmer, shape):
     with pytest.raises(pkg.HBError) as e:
         h.cross_matmul(pkg.CtxtTensor(a, *shape), pkg.CtxtTensor(a, shape[1], shape[0], shape[2]), target_level=2)
     assert e.value.code == -1
+
+
+@pytest.mark.parametrize("shape", [(16, 32, 32), (4, 8, 8), (1, 16, 16)])
+def test_scores_of_a_key_tile_alone_with_fewer_rows(pkg, hemmer, shape):
+    h = hemmer
+    with pytest.raises(pkg.HBError) as e:
+        h.cross_scores(pkg.CtxtTensor(h.lib.ct_create(8, 2, 1, 1), *shape), pkg.CtxtTensor(h.lib.ct_create(8, 2, 1, 1), *shape), target_level=2)
+    assert e.value.code == -1
