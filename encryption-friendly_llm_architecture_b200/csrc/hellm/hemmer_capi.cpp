@@ -214,12 +214,15 @@ int hb_hemmer_cross_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa,
         *out = h->h.crossMatMul(view(ba, ra, ca, wa), view(bb, rb, cb, wb), heads, inner, target).get().release();
     });
 }
-int hb_hemmer_cross_scores(hb_hemmer *h, const hb_ct *query, const hb_ct *key, int rows, int cols, int width, int heads, int target, hb_ct **out) {
+int hb_hemmer_cross_scores_shaped(hb_hemmer *h, const hb_ct *query, int rq, int cq, int wq, const hb_ct *key, int rk, int ck, int wk, int heads, int target, hb_ct **out) {
     return guard([&] {
         if (!query || !key || !out) throw std::invalid_argument("[crossScores] null argument");
         Borrow bq(h->ctx, query), bk(h->ctx, key);
-        *out = h->h.crossScores(view(bq, rows, cols, width), view(bk, rows, cols, width), heads, target).get().release();
+        *out = h->h.crossScores(view(bq, rq, cq, wq), view(bk, rk, ck, wk), heads, target).get().release();
     });
+}
+int hb_hemmer_cross_scores(hb_hemmer *h, const hb_ct *query, const hb_ct *key, int rows, int cols, int width, int heads, int target, hb_ct **out) {
+    return hb_hemmer_cross_scores_shaped(h, query, rows, cols, width, key, rows, cols, width, heads, target, out);
 }
 int hb_hemmer_matmul_reuse_grouped(hb_hemmer *h, const hb_ct *pre, int inputs, const int32_t *order, const int32_t *sizes, int experts, const hb_pt *const *pts, int bcount, int tiles, int width,
                                    hb_ct **out) {

@@ -313,7 +313,7 @@ class Hemmer:
 
     def cross_scores(self, query, key, heads=1, target_level=4):
         """cross_matmul with the transposed key tiles: member (j * heads + h) * nq + i is query tile i times key tile j transposed."""
-        ct = self._call("cross_scores", query.ct.ptr, key.ct.ptr, *self._shp(query), C.c_int(heads), C.c_int(target_level))
+        ct = self._call("cross_scores_shaped", query.ct.ptr, *self._shp(query), key.ct.ptr, *self._shp(key), C.c_int(heads), C.c_int(target_level))
         return CtxtTensor(ct, query.rows, key.rows, query.width)
 
     # ---- weights in 4 bits ----

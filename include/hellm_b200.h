@@ -144,6 +144,8 @@ int hb_hemmer_matmul_reuse_grouped(hb_hemmer *h, const hb_ct *pre, int inputs, c
 int hb_hemmer_cross_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa, const hb_ct *b, int rb, int cb, int wb, int heads, int inner,
                            int target_level, hb_ct **out);
 int hb_hemmer_cross_scores(hb_hemmer *h, const hb_ct *query, const hb_ct *key, int rows, int cols, int width, int heads, int target_level, hb_ct **out);
+/* the same with key tiles of another number of rows.  A key tile that is not one of a pair (wk below rk + ck) has wk rows. */
+int hb_hemmer_cross_scores_shaped(hb_hemmer *h, const hb_ct *query, int rq, int cq, int wq, const hb_ct *key, int rk, int ck, int wk, int heads, int target_level, hb_ct **out);
 /* Encrypted vectors times a matrix in 4 bits (hb_matvec_q4), rescaled and summed over the rows.  x: ceil(rows / 4 d) members a vector (d: the tile two of
  * which fill a ciphertext), entry 4 d b + s of the vector in all columns of row s % d of member b: s < d left half, real part; s < 2 d right half, real
  * part; s < 3 d left half, imaginary part; then right half, imaginary part.  out: one member per vector and column tile, in every row

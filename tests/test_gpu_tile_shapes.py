@@ -1,6 +1,7 @@
 """Products of tiles with tiles of another number, for tiles of every shape: those that are multiplied, against products in 64 bits, and those that are refused.
 
 Decrypted values may be off by 2^-14, the bound that every decrypted product of this repository is held to."""
+import ctypes as C
 import itertools
 
 import numpy as np
@@ -83,4 +84,39 @@ def test_scores_of_a_key_tile_alone_with_fewer_rows(pkg, hemmer, shape):
     h = hemmer
     with pytest.raises(pkg.HBError) as e:
         h.cross_scores(pkg.CtxtTensor(h.lib.ct_create(8, 2, 1, 1), *shape), pkg.CtxtTensor(h.lib.ct_create(8, 2, 1, 1), *shape), target_level=2)
+    assert e.value.code == -1
+
+
+@pytest.mark.parametrize("rows,keys", [(32, 16), (16, 32), (8, 16), (32, 8), (16, 16), (1, 32)])
+def test_scores_of_tiles_with_other_numbers_of_rows(pkg, hemmer, rows, keys):
+    h, rng = hemmer, np.random.default_rng(rows + keys)
+    q, k = [rng.uniform(-1, 1, (rows, 32)) for _ in range(2)], [rng.uniform(-1, 1, (keys, 32)) for _ in range(2)]
+    got = h.cross_scores(_tensor(pkg, h, q, 64, 1), _tensor(pkg, h, k, 64, 2), target_level=2)
+    assert got.shape == (rows, keys, 64)
+    for x, a, b in zip(_tiles(h, got, rows, keys, 2), q, k):
+        assert np.abs(x - a @ b.T).max() < TOL
+
+
+def test_rows_behind_a_shorter_key_tile_are_not_keys(pkg, hemmer):
+    """The shape says how many rows are keys, whatever the slots behind them hold."""
+    h, rng = hemmer, np.random.default_rng(1)
+    q, k = [rng.uniform(-1, 1, (32, 32)) for _ in range(2)], [rng.uniform(-1, 1, (32, 32)) for _ in range(2)]
+    whole = _tensor(pkg, h, k, 64, 2)
+    got = h.cross_scores(_tensor(pkg, h, q, 64, 1), pkg.CtxtTensor(whole.ct, 16, 32, 64), target_level=2)
+    for x, a, b in zip(_tiles(h, got, 32, 32, 2), q, k):
+        assert np.abs(x[:, :16] - a @ b[:16].T).max() < TOL
+
+
+def test_scores_through_the_entry_with_one_shape(pkg, hemmer):
+    h, rng = hemmer, np.random.default_rng(2)
+    q, k = (_tensor(pkg, h, [rng.uniform(-1, 1, (16, 32)) for _ in range(2)], 64, n) for n in (1, 2))
+    one = h._call("cross_scores", q.ct.ptr, k.ct.ptr, *h._shp(q), C.c_int(1), C.c_int(2))
+    assert np.array_equal(h.lib.ct_export(one), h.lib.ct_export(h.cross_scores(q, k, target_level=2).ct))
+
+
+@pytest.mark.parametrize("query,key", [((32, 32, 64), (32, 16, 64)), ((32, 32, 64), (32, 32, 32)), ((16, 16, 32), (32, 16, 32)), ((32, 32, 64), (20, 32, 64))])
+def test_scores_of_tiles_that_do_not_meet(pkg, hemmer, query, key):
+    h = hemmer
+    with pytest.raises(pkg.HBError) as e:
+        h.cross_scores(pkg.CtxtTensor(h.lib.ct_create(8, 2, 1, 1), *query), pkg.CtxtTensor(h.lib.ct_create(8, 2, 1, 1), *key), target_level=2)
     assert e.value.code == -1
