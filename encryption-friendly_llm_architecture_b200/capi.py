@@ -155,6 +155,12 @@ class Lib:
                                              C.c_int(codes.shape[1]), C.c_int(group), C.byref(out)))
         return Handle(self, out, "qweight")
 
+    def qweight_meta(self, w):
+        """(rows, columns, rows of a group) of a weight matrix in 4 bits."""
+        r, c, g = C.c_int(), C.c_int(), C.c_int()
+        self._chk(self._fn("qweight_meta")(w.ptr, C.byref(r), C.byref(c), C.byref(g)))
+        return r.value, c.value, g.value
+
     def encode_q4(self, w, tile, first, count, level, diagonal=True):
         """Plaintext operands of the blocks first .. first + count - 1 of a 4-bit weight matrix (K-groups of four row tiles innermost)."""
         out = (C.c_void_p * max(0, count))()

@@ -327,8 +327,10 @@ class Hemmer:
 
     def encode_diagonal_to_row4_q4(self, qweight, rows, cols, level=0):
         """The operands that encode_diagonal_to_row4 makes of a rows x cols matrix, from its 4-bit form (Lib.qweight): [column tile][K-group]."""
-        d = self.tile
+        d, there = self.tile, self.lib.qweight_meta(qweight)
         kb, nb = -(-rows // (4 * d)), -(-cols // d)
+        if kb != -(-there[0] // (4 * d)):  # the blocks are numbered by the matrix's own rows
+            raise ValueError(f"a matrix of {there[0]} rows, not {rows}")
         pts = self.lib.encode_q4(qweight, d, 0, kb * nb, level or self.lib.L)
         return [[PtxtTensor(p, d, d, 2 * d) for p in pts[j * kb:(j + 1) * kb]] for j in range(nb)]
 
