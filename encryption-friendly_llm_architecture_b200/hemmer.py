@@ -16,6 +16,8 @@ from .capi import Handle, Lib, HBError
 class CtxtTensor:
     """HETensor<Ciphertext> (HETensor.hpp:46-86): a ciphertext handle plus its tile shape."""
 
+    per_vector = None  # members of one vector, of encrypt_vectors and matvec_q4
+
     def __init__(self, ct: Handle, rows: int, cols: int, width: int | None = None):
         if width is None:
             width = 1
@@ -346,16 +348,25 @@ class Hemmer:
         halves = np.stack([parts[:, 0] + 1j * parts[:, 2], parts[:, 1] + 1j * parts[:, 3]], axis=2)     # [member][row][half]
         msgs = np.zeros((parts.shape[0], self.lib.slots), dtype=np.complex128)
         msgs[:, : 2 * d * d] = np.repeat(halves, d, axis=2).reshape(parts.shape[0], -1)
-        return CtxtTensor(self.lib.encrypt_many(msgs, level, nonces), d, d, 2 * d)
+        out = CtxtTensor(self.lib.encrypt_many(msgs, level, nonces), d, d, 2 * d)
+        out.per_vector = kb
+        return out
 
     def matvec_q4(self, x, qweight):
         """Encrypted vectors times a 4-bit matrix: one member per vector and column tile, one level below x; decrypt_vectors reads them."""
-        return CtxtTensor(self._call("matvec_q4", x.ct.ptr, qweight.ptr), *x.shape)
+        d, (rows, cols, _) = self.tile, self.lib.qweight_meta(qweight)
+        if x.per_vector not in (None, -(-rows // (4 * d))):  # a batch of the right size all the same may be other vectors
+            raise HBError(-3, f"vectors of {x.per_vector} members, a matrix of {rows} rows")
+        out = CtxtTensor(self._call("matvec_q4", x.ct.ptr, qweight.ptr), *x.shape)
+        out.per_vector = -(-cols // d)
+        return out
 
     def decrypt_vectors(self, y, cols):
         """The vectors that matvec_q4 made, [vectors][cols]."""
         d = self.tile
         nb, members = -(-cols // d), self.lib.ct_meta(y.ct)[2]
+        if y.per_vector not in (None, nb):
+            raise ValueError(f"vectors of {y.per_vector} column tiles, not {cols} columns")
         z = self.lib.decrypt_many([(y.ct, k) for k in range(members)])[:, : 2 * d].real
         return (2.0 * (z[:, :d] + z[:, d:])).reshape(members // nb, nb * d)[:, :cols]
 

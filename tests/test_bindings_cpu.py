@@ -1,6 +1,7 @@
 """What the Python layer checks of its arguments before it calls the library: with a stand-in for the library."""
 from types import SimpleNamespace
 
+import numpy as np
 import pytest
 
 
@@ -26,3 +27,44 @@ def test_operands_of_as_many_blocks(pkg, rows, cols, tiles):
     h = _hemmer(pkg, qweight_meta=lambda w: (100, 40, 16), encode_q4=lambda *a: calls.append(a) or [None] * a[3])
     got = h.encode_diagonal_to_row4_q4(None, rows, cols)
     assert len(got) == tiles and all(len(row) == 2 for row in got) and calls[0][2:4] == (0, 2 * tiles)
+
+
+def _vectors(pkg, cols):
+    """(layer, calls): 100 x 40 matrices, two K-groups of 64 rows and three column tiles"""
+    calls = []
+    h = _hemmer(pkg, qweight_meta=lambda w: (100, cols, 16), encrypt_many=lambda msgs, level, nonces: len(msgs), ct_meta=lambda ct: (3, 2, ct, 1),
+                decrypt_many=lambda members: np.zeros((len(members), 512), dtype=complex))
+    h._call = lambda name, x, w: calls.append(name) or 6
+    return h, calls
+
+
+class _Ct(int):
+    ptr = None
+
+
+def test_vectors_of_another_length(pkg):
+    """Two vectors of 60 entries are two members, which a matrix of 100 rows would take for one vector of 100; one of 200 are four, two vectors of it."""
+    h, calls = _vectors(pkg, 40)
+    w = SimpleNamespace(ptr=None)
+    for x in (np.ones((2, 60)), np.ones((1, 200)), np.ones((4, 1))):
+        ct = h.encrypt_vectors(x, 3, None)
+        ct.ct = _Ct(ct.ct)
+        with pytest.raises(pkg.HBError):
+            h.matvec_q4(ct, w)
+    assert not calls
+    for x in (np.ones((2, 100)), np.ones((1, 70)), np.ones((3, 128))):
+        ct = h.encrypt_vectors(x, 3, None)
+        ct.ct = _Ct(ct.ct)
+        h.matvec_q4(ct, w)
+    h.matvec_q4(pkg.CtxtTensor(_Ct(2), 16, 16, 32), w)  # made another way: the library counts its members
+    assert len(calls) == 4
+
+
+def test_results_of_another_width(pkg):
+    """Six members: two vectors of three column tiles, not three of two."""
+    h, _ = _vectors(pkg, 40)
+    y = h.matvec_q4(pkg.CtxtTensor(_Ct(4), 16, 16, 32), SimpleNamespace(ptr=None))
+    for cols in (32, 16, 1, 96):
+        with pytest.raises(ValueError):
+            h.decrypt_vectors(y, cols)
+    assert h.decrypt_vectors(y, 40).shape == (2, 40) and h.decrypt_vectors(pkg.CtxtTensor(6, 16, 16, 32), 32).shape == (3, 32)
