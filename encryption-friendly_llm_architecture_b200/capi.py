@@ -401,7 +401,7 @@ class Lib:
         (None: p); member p * tiles + t of the result.  pts[e] may be None where sizes[e] is 0."""
         sizes = [int(n) for n in sizes]
         there = [rows for rows, n in zip(pts, sizes) if n]
-        if len(pts) != len(sizes) or not there:
+        if len(pts) != len(sizes) or not there or not there[0]:
             raise ValueError("one list of weights per expert, and an expert with inputs")
         tiles, bcount = len(there[0]), len(there[0][0])
         if any(len(rows) != tiles or any(len(row) != bcount for row in rows) for rows in there):

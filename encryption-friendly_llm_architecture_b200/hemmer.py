@@ -303,7 +303,10 @@ class Hemmer:
         """matmul_reuse_groups grouped by expert: weights[e][t][b] (None for an expert without inputs), the first sizes[0] positions at expert 0
         and so on, position p with input order[p] (None: p); `pre` holds the copies of `inputs` inputs of as many K-groups as the weights have,
         K-groups innermost.  Member p * tiles + t of the result is output tile t of position p."""
-        first = next(w for w, n in zip(weights, sizes) if n)[0][0]
+        used = [w for w, n in zip(weights, sizes) if n]
+        if len(weights) != len(sizes) or not used or not used[0] or not used[0][0]:
+            raise ValueError("one list of weights per expert, and an expert with inputs")
+        first = used[0][0][0]
         pts = [[[w.ct for w in row] for row in rows] if n else None for rows, n in zip(weights, sizes)]
         return CtxtTensor(self.lib.matmul_acc_grouped(pre, inputs, sizes, pts, first.width, order=order), *first.shape)
 

@@ -68,3 +68,25 @@ def test_results_of_another_width(pkg):
         with pytest.raises(ValueError):
             h.decrypt_vectors(y, cols)
     assert h.decrypt_vectors(y, 40).shape == (2, 40) and h.decrypt_vectors(pkg.CtxtTensor(6, 16, 16, 32), 32).shape == (3, 32)
+
+
+def _weights(tiles, groups):
+    return [[SimpleNamespace(ct=SimpleNamespace(ptr=SimpleNamespace(value=1)), width=32, shape=(16, 16, 32)) for _ in range(groups)] for _ in range(tiles)]
+
+
+@pytest.mark.parametrize("sizes,weights", [([0, 0], [None, None]), ([], []), ([1], [_weights(2, 1), _weights(2, 1)]), ([1, 0], [_weights(2, 1)]), ([1], [[]]), ([1], [[[]]])])
+def test_experts_without_inputs_or_weights(pkg, sizes, weights):
+    """As many lists of weights as sizes, one of them with positions and with weights."""
+    calls = []
+    h = _hemmer(pkg, matmul_acc_grouped=lambda *a, **k: calls.append(a))
+    with pytest.raises(ValueError):
+        h.matmul_reuse_experts(None, 2, sizes, weights)
+    assert not calls
+    h.matmul_reuse_experts(None, 2, [0, 2], [None, _weights(2, 1)])
+    assert len(calls) == 1
+
+
+def test_an_expert_with_an_empty_list(pkg):
+    lib = object.__new__(pkg.capi.Lib)
+    with pytest.raises(ValueError):
+        lib.matmul_acc_grouped(None, 2, [1], [[]], 8)
