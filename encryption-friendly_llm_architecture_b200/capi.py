@@ -46,6 +46,14 @@ def _nonces(nonces, count):
     return nonces
 
 
+def _i32(v):
+    """A whole number as the C entries take it; ctypes would drop the bits that do not fit."""
+    v = int(v)
+    if not -2**31 <= v < 2**31:
+        raise ValueError(f"{v} does not fit 32 bits")
+    return C.c_int32(v)
+
+
 def _f64(a):
     return None if a is None else a.ctypes.data_as(c_f64p)
 
@@ -151,8 +159,8 @@ class Lib:
         if rows < 1 or group < 1 or codes.shape[0] != (rows + 1) // 2 or scales.shape != ((rows + group - 1) // group, codes.shape[1]):
             raise ValueError(f"{rows} rows in groups of {group}: codes {codes.shape}, scales {scales.shape}")
         out = C.c_void_p()
-        self._chk(self._fn("qweight_create")(self.ctx, codes.ctypes.data_as(C.POINTER(C.c_uint8)), scales.ctypes.data_as(C.POINTER(C.c_float)), C.c_int(rows),
-                                             C.c_int(codes.shape[1]), C.c_int(group), C.byref(out)))
+        self._chk(self._fn("qweight_create")(self.ctx, codes.ctypes.data_as(C.POINTER(C.c_uint8)), scales.ctypes.data_as(C.POINTER(C.c_float)), _i32(rows),
+                                             _i32(codes.shape[1]), _i32(group), C.byref(out)))
         return Handle(self, out, "qweight")
 
     def qweight_meta(self, w):
@@ -164,12 +172,12 @@ class Lib:
     def encode_q4(self, w, tile, first, count, level, diagonal=True):
         """Plaintext operands of the blocks first .. first + count - 1 of a 4-bit weight matrix (K-groups of four row tiles innermost)."""
         out = (C.c_void_p * max(0, count))()
-        self._chk(self._fn("encode_q4")(self.ctx, w.ptr, C.c_int(tile), C.c_int(1 if diagonal else 0), C.c_int(first), C.c_int(count), C.c_int(level), out))
+        self._chk(self._fn("encode_q4")(self.ctx, w.ptr, _i32(tile), C.c_int(1 if diagonal else 0), _i32(first), _i32(count), _i32(level), out))
         return [Handle(self, C.c_void_p(p), "pt") for p in out]
 
     def matvec_q4(self, x, w, tile):
         """Encrypted vectors (their K-groups innermost in the batch) times a 4-bit weight matrix, un-rescaled."""
-        return self._op("matvec_q4", x.ptr, w.ptr, C.c_int(tile))
+        return self._op("matvec_q4", x.ptr, w.ptr, _i32(tile))
 
     def decode(self, pt):
         re = np.zeros(self.slots); im = np.zeros(self.slots)
@@ -393,7 +401,7 @@ class Lib:
     def tensor_acc_cross(self, a, b, groups, heads=1, acc=None):
         """out[j][h][i] = sum_g tensor(a[g][h][i], b[g][h][j]); with `acc` the sum goes there, and `acc` comes back."""
         out = C.c_void_p(acc.ptr.value if acc is not None else None)
-        self._chk(self._fn("tensor_acc_cross")(self.ctx, a.ptr, b.ptr, C.c_int(groups), C.c_int(heads), C.byref(out)))
+        self._chk(self._fn("tensor_acc_cross")(self.ctx, a.ptr, b.ptr, _i32(groups), _i32(heads), C.byref(out)))
         return acc if acc is not None else Handle(self, out, "ct")
 
     def matmul_acc_grouped(self, pre, inputs, sizes, pts, row_step, order=None):
@@ -412,8 +420,8 @@ class Lib:
         for e, (rows, n) in enumerate(zip(pts, sizes)):
             if n:
                 arr[e * tiles * bcount:(e + 1) * tiles * bcount] = [p.ptr.value for row in rows for p in row]
-        which = None if order is None else (C.c_int32 * len(order))(*[int(i) for i in order])
-        return self._op("matmul_acc_grouped", pre.ptr, C.c_int(inputs), which, (C.c_int32 * len(sizes))(*sizes), C.c_int(len(sizes)), arr, C.c_int(bcount), C.c_int(tiles),
+        which = None if order is None else (C.c_int32 * len(order))(*[_i32(i) for i in order])
+        return self._op("matmul_acc_grouped", pre.ptr, _i32(inputs), which, (C.c_int32 * len(sizes))(*[_i32(n) for n in sizes]), C.c_int(len(sizes)), arr, C.c_int(bcount), C.c_int(tiles),
                         C.c_int64(row_step))
 
     def rotate_sum(self, xs, steps):

@@ -90,3 +90,21 @@ def test_an_expert_with_an_empty_list(pkg):
     lib = object.__new__(pkg.capi.Lib)
     with pytest.raises(ValueError):
         lib.matmul_acc_grouped(None, 2, [1], [[]], 8)
+
+
+@pytest.mark.parametrize("far", [2**32, 2**32 + 1, 2**31, -2**31 - 1])
+def test_whole_numbers_beyond_32_bits(pkg, far):
+    """ctypes drops the bits that do not fit: input 2^32 would be input 0, a group of 2^32 + 1 rows one of a single row, whose scales are not there."""
+    calls = []
+    lib = object.__new__(pkg.capi.Lib)
+    lib._fn = lambda name: lambda *a: calls.append(name) or 0
+    lib._op = lambda name, *a: calls.append(name)
+    lib.ctx, lib.alive = None, False
+    x = SimpleNamespace(ptr=SimpleNamespace(value=None))
+    w, codes, scales = [[x]], np.zeros((2, 3), dtype=np.uint8), np.zeros((1, 3), dtype=np.float32)
+    for call in (lambda n: lib.matmul_acc_grouped(x, 2, [1], [w], 8, order=[n]), lambda n: lib.matmul_acc_grouped(x, n, [1], [w], 8), lambda n: lib.matmul_acc_grouped(x, 2, [n], [w], 8),
+                 lambda n: lib.tensor_acc_cross(x, x, n), lambda n: lib.tensor_acc_cross(x, x, 1, heads=n), lambda n: lib.matvec_q4(x, x, n), lambda n: lib.encode_q4(x, n, 0, 1, 1),
+                 lambda n: lib.encode_q4(x, 1, n, 1, 1), lambda n: lib.encode_q4(x, 1, 0, 1, n), lambda n: lib.qweight(codes, scales, 4, abs(n))):
+        with pytest.raises(ValueError):
+            call(far)
+        assert not calls
