@@ -1034,27 +1034,26 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
             auto begin = [&] { el.experts = 0; el.tiles = tn; el.bcount = bcount; el.out_tiles = tiles; el.tile0 = tile0; el.first_pos[0] = 0; el.pos0 = (int)next; };
             auto flush = [&] {
                 if (!el.experts) return;
-                int M = expert_positions(el.experts, tn, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; }), T = expert_tiles(M, tn);
-                auto lay = [&] {
-                    el.first_block[0] = 0;
-                    for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + M - 1) / M * ((tn + T - 1) / T);
-                };
-                lay();
-                const i64 each = (i64)(c->N / 128) * n;
-                if (each * el.first_block[el.experts] < 148 * 3) { M = 1; T = expert_tiles_few(el.first_pos[el.experts], tn, each); lay(); }
-                auto go = [&](auto m, auto t) { launch_experts<decltype(m)::value, decltype(t)::value>(c, el, pre, r->d, copies, inputs, gal); };
+                const ExpertBlocks b = expert_blocks(el.experts, tn, (long)(c->N / 128) * n, [&](int e) { return el.first_pos[e + 1] - el.first_pos[e]; });
+                el.first_block[0] = 0;
+                for (int e = 0; e < el.experts; ++e) el.first_block[e + 1] = el.first_block[e] + (el.first_pos[e + 1] - el.first_pos[e] + b.M - 1) / b.M * ((tn + b.T - 1) / b.T);
                 auto by_tiles = [&](auto m) {
-                    constexpr int MM = decltype(m)::value;
-                    switch (T) {
-                    case 1: go(m, std::integral_constant<int, 1>{}); break;
-                    case 2: go(m, std::integral_constant<int, 2>{}); break;
-                    case 3: go(m, std::integral_constant<int, 3>{}); break;
-                    case 4: go(m, std::integral_constant<int, 4>{}); break;
-                    case 6: if constexpr (MM < 3) go(m, std::integral_constant<int, 6>{}); break;
-                    default: if constexpr (MM < 2) go(m, std::integral_constant<int, 8>{});
+                    auto go = [&](auto t) {
+                        constexpr int M = decltype(m)::value, T = decltype(t)::value;
+                        if constexpr (expert_kernel(M, T)) launch_experts<M, T>(c, el, pre, r->d, copies, inputs, gal);
+                        else fail(HB_E_LIMIT, "matmul_acc_grouped: blocks without a kernel"); // the rule makes none
+                    };
+                    switch (b.T) {
+                    case 1: go(std::integral_constant<int, 1>{}); break;
+                    case 2: go(std::integral_constant<int, 2>{}); break;
+                    case 3: go(std::integral_constant<int, 3>{}); break;
+                    case 4: go(std::integral_constant<int, 4>{}); break;
+                    case 6: go(std::integral_constant<int, 6>{}); break;
+                    case 8: go(std::integral_constant<int, 8>{}); break;
+                    default: go(std::integral_constant<int, 0>{});
                     }
                 };
-                if (M == 1) by_tiles(std::integral_constant<int, 1>{}); else if (M == 2) by_tiles(std::integral_constant<int, 2>{}); else by_tiles(std::integral_constant<int, 3>{});
+                if (b.M == 1) by_tiles(std::integral_constant<int, 1>{}); else if (b.M == 2) by_tiles(std::integral_constant<int, 2>{}); else by_tiles(std::integral_constant<int, 3>{});
             };
             begin();
             for (int e = 0; e < experts; ++e)

@@ -116,5 +116,16 @@ constexpr int expert_tiles_few(int positions, int tiles, long each) {
     while (T > 1 && positions * ((tiles + T - 1L) / T) * each < 148 * 3) --T;
     return T;
 }
+// The blocks of a launch: M positions and T tiles.
+struct ExpertBlocks { int M, T; };
+template <class SIZE> constexpr ExpertBlocks expert_blocks(int experts, int tiles, long each, SIZE &&size) {
+    const int M = expert_positions(experts, tiles, size), T = expert_tiles(M, tiles);
+    long positions = 0, groups = 0;
+    for (int e = 0; e < experts; ++e) { positions += size(e); groups += (size(e) + M - 1) / M; }
+    if (each * groups * ((tiles + T - 1) / T) >= 148 * 3) return {M, T};
+    return {1, expert_tiles_few((int)positions, tiles, each)};
+}
+// Blocks that there are kernels for.
+constexpr bool expert_kernel(int M, int T) { return T >= 1 && (M == 1 ? T <= 8 && T != 5 && T != 7 : M == 2 ? T <= 6 && T != 5 : M == 3 && T <= 4); }
 
 } // namespace hb
