@@ -1071,17 +1071,16 @@ hb_ct *do_matmul_experts(hb_ctx *c, const hb_ct *pre, int inputs, const int32_t 
     return r;
 }
 // ---- tensor products of all pairs of tiles ----
-template <int TR, int TC, int LR, int LC> void launch_pairs(hb_ctx *c, int variant, u64 *d, const PairSides &sides, const PairShape &s, int level, bool accumulate) {
-    using T = PairTile<TR, TC, LR, LC>;
-    if (!c->smem_opt_in_pairs[variant]) {
-        CK(cudaFuncSetAttribute(k_tensor_pairs<TR, TC, LR, LC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
-        c->smem_opt_in_pairs[variant] = true;
+template <int V> void launch_pairs(hb_ctx *c, u64 *d, const PairSides &sides, const PairShape &s, int level, bool accumulate) {
+    constexpr PairBlock B = kPairBlocks[V];
+    using T = PairTile<B.tr, B.tc, B.lr, B.lc>;
+    auto *const kernel = k_tensor_pairs<B.tr, B.tc, B.lr, B.lc>;
+    if (!c->smem_opt_in_pairs[V]) {
+        CK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)T::kSmem));
+        c->smem_opt_in_pairs[V] = true;
     }
-    const int n = level + 1, blocks = ((sides.nr + T::kRows - 1) / T::kRows) * ((sides.nc + T::kCols - 1) / T::kCols);
-    // ranges of a CTA: more of them, and the ring runs dry less often; but with few CTAs an SM those of the 60-bit limb end late (eight against eight tiles, two heads: 963 us with at least 8 an SM, 895 with 32)
-    int run = 1;
-    while (run < 16 && c->N / (16 * T::kX * run) >= 1 && (i64)c->N / (16 * T::kX * run) * blocks * s.heads * n >= 148 * 32) run *= 2;
-    launch(c, k_tensor_pairs<TR, TC, LR, LC>, dim3((unsigned)(c->N / (8 * T::kX * run)) * (unsigned)blocks, (unsigned)(s.heads * n)), 256, T::kSmem, d, sides, s, run, n, c->qmap(level), c->pc, c->N,
+    const int n = level + 1, run = pair_ranges(B, c->N, sides.nr, sides.nc, s.heads, n);
+    launch(c, kernel, dim3((unsigned)(c->N / (8 * T::kX * run)) * (unsigned)pair_blocks(B, sides.nr, sides.nc), (unsigned)(s.heads * n)), 256, T::kSmem, d, sides, s, run, n, c->qmap(level), c->pc, c->N,
            accumulate ? 1 : 0);
 }
 // acc[j][h][i] (+)= sum_g tensor(a[g][h][i], b[g][h][j])
@@ -1102,16 +1101,15 @@ hb_ct *do_tensor_pairs(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, in
     try {
         const bool keys = s.nk > s.nq;
         const PairSides sides{keys ? b->d : a->d, keys ? a->d : b->d, std::max(s.nq, s.nk), std::min(s.nq, s.nk), keys ? 1 : 0};
-        const int rows = sides.nr > 2 ? 4 : sides.nr, cols = sides.nc > 2 ? 4 : sides.nc;
-        auto go = [&](auto tr, auto tc, auto lr, auto lc, int variant) {
-            launch_pairs<decltype(tr)::value, decltype(tc)::value, decltype(lr)::value, decltype(lc)::value>(c, variant, r->d, sides, s, a->level, acc != nullptr);
-        };
-        constexpr std::integral_constant<int, 1> one{};
-        constexpr std::integral_constant<int, 2> two{};
-        constexpr std::integral_constant<int, 4> four{};
-        if (cols == 1) { if (rows == 1) go(one, one, one, one, 0); else if (rows == 2) go(two, one, one, one, 1); else go(four, one, one, one, 2); }
-        else if (cols == 2) { if (rows == 2) go(two, two, one, one, 3); else go(two, two, two, one, 4); }
-        else go(two, two, two, two, 5);
+        auto go = [&](auto v) { launch_pairs<decltype(v)::value>(c, r->d, sides, s, a->level, acc != nullptr); };
+        switch (pair_block(sides.nr, sides.nc)) {
+        case 0: go(std::integral_constant<int, 0>{}); break;
+        case 1: go(std::integral_constant<int, 1>{}); break;
+        case 2: go(std::integral_constant<int, 2>{}); break;
+        case 3: go(std::integral_constant<int, 3>{}); break;
+        case 4: go(std::integral_constant<int, 4>{}); break;
+        default: go(std::integral_constant<int, 5>{});
+        }
     } catch (...) { if (!acc) hb_ct_free(r); throw; }
     return r;
 }

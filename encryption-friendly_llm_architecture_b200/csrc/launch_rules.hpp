@@ -128,4 +128,18 @@ template <class SIZE> constexpr ExpertBlocks expert_blocks(int experts, int tile
 // Blocks that there are kernels for.
 constexpr bool expert_kernel(int M, int T) { return T >= 1 && (M == 1 ? T <= 8 && T != 5 && T != 7 : M == 2 ? T <= 6 && T != 5 : M == 3 && T <= 4); }
 
+// Tensor products of all pairs of tiles: a warp's block is lr x lc lane blocks of tr x tc pairs, side by side for 32 / (lr lc) residues.  The block is the smallest that holds the
+// tiles of both sides, four of each at most; nr and nc: tiles of the sides, nr at least nc.
+struct PairBlock { int tr, tc, lr, lc; };
+constexpr PairBlock kPairBlocks[] = {{1, 1, 1, 1}, {2, 1, 1, 1}, {4, 1, 1, 1}, {2, 2, 1, 1}, {2, 2, 2, 1}, {2, 2, 2, 2}};
+constexpr int pair_block(int nr, int nc) { return nc == 1 ? (nr > 2 ? 2 : nr - 1) : nc > 2 ? 5 : nr > 2 ? 4 : 3; }
+constexpr int pair_blocks(PairBlock b, int nr, int nc) { return (nr + b.tr * b.lr - 1) / (b.tr * b.lr) * ((nc + b.tc * b.lc - 1) / (b.tc * b.lc)); } // blocks of all pairs
+// ranges of a CTA: more of them, and the ring runs dry less often; but with few CTAs an SM those of the 60-bit limb end late (eight against eight tiles, two heads: 963 us with at least 8 an SM, 895 with 32)
+constexpr int pair_ranges(PairBlock b, int N, int nr, int nc, int heads, int limbs) {
+    const int X = 32 / (b.lr * b.lc);
+    int run = 1;
+    while (run < 16 && N / (16 * X * run) >= 1 && (long)N / (16 * X * run) * pair_blocks(b, nr, nc) * heads * limbs >= 148 * 32) run *= 2;
+    return run;
+}
+
 } // namespace hb

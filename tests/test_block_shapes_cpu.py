@@ -5,7 +5,7 @@ import subprocess
 import pytest
 
 from conftest import PKG_NAME, ROOT
-from test_gpu_block_shapes import EXPERTS, RINGS
+from test_gpu_block_shapes import EXPERTS, PAIRS, RINGS
 
 
 @pytest.fixture(scope="module")
@@ -46,3 +46,12 @@ def test_sums_of_experts_past_every_reduction(blocks):
     for m in (2, 3):
         products = {n for mm, _, _, _, n in _expert_blocks(blocks) if mm == m and n}
         assert {127, 128, 129} <= products
+
+
+def test_every_run_of_ranges(blocks):
+    lines = [" ".join(map(str, ["pairs", 1 << RINGS[ring]["log_n"], level + 1, heads, nq, nk])) for ring, level, _, heads, nq, nk, _ in PAIRS]
+    reached = {tuple(b) for b in blocks(lines)}
+    assert reached == {(block, run) for block in range(6) for run in (1, 2, 4, 8, 16)}
+    several = [case for case, (_, run) in zip(PAIRS, blocks(lines)) if run >= 4]
+    assert {1, 2, 3, 5} <= {case[2] for case in several}   # one group: every copy begins a range; and numbers that are no multiple of the ring's four stages
+    assert any(case[6] for case in several)
