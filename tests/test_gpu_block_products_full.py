@@ -10,9 +10,18 @@ TOL = 2.0 ** -14
 D = 128
 
 
+@pytest.fixture(scope="module")
+def ring(pkg):
+    """A context of its own: the methods add rotation keys, which tests of missing ones must not find."""
+    g = pkg.open_gpu()
+    g.keygen()
+    yield g
+    g.close()
+
+
 @pytest.fixture(scope="module", params=[0, 1, 2])
-def hemmer(request, pkg, gpu_full):
-    h = pkg.open_hemmer(gpu_full)
+def hemmer(request, pkg, ring):
+    h = pkg.open_hemmer(ring)
     h.set_schedule(request.param)
     yield h
     h.close()

@@ -35,6 +35,16 @@ EXPERTS = [
 ]
 
 
+@pytest.fixture(autouse=True)
+def _memory_goes_back(request):
+    """The cases are large, and tests that fill the GPU come after them."""
+    import torch
+    yield
+    g = request.getfixturevalue("gpu_" + request.node.callspec.params["ring"])
+    g._chk(g._fn("release_cached")(g.ctx))
+    torch.cuda.empty_cache()
+
+
 def _view(handle):
     """The device words of a handle, for torch."""
     import torch
