@@ -6,9 +6,9 @@
 // 16-byte asynchronous copies a few steps ahead: lines of 32 residues, of rotated weights the line that holds the residues wanted (a rotation permutes aligned
 // runs of 32 as units, and within them), from which every lane reads its own.  The blocks of one range of residues, over all experts, run side by side, so that
 // copies and weights come from L2 for all but the first of them.
-// Two of three experts, twelve tiles, two K-groups of 128 copies, 8 positions at level 5: 9.6 ms (1.1 of HBM, 4.3 of FP64 at four instructions a product); five positions, one
-// K-group, six tiles: 1.77 ms.  FP64 is 60 % active and 67 % of the issue slots are taken: a product costs 12.7 instructions, 5.7 of them FP64 (the 60-bit limb's nine
-// and the conversions in it), 1.7 moves, the rest addresses and copies, and 168 registers leave three warps a scheduler.  Rings of 2, 3, 4 and 6 stages: 16.4, 10.4, 9.6 and 10.7 ms.  Sums that
+// Two of three experts, twelve tiles, two K-groups of 128 copies, 8 positions at level 5: 9.9 ms (1.1 of HBM, 5.2 of FP64 at four instructions a product, nine modulo the 60-bit prime); five positions, one
+// K-group, six tiles: 1.83 ms.  FP64 is 60 % active and 67 % of the issue slots are taken: a product costs 12.7 instructions, 5.7 of them FP64 (the 60-bit limb's nine
+// and the conversions in it), 1.7 moves, the rest addresses and copies, and 168 registers leave three warps a scheduler.  Rings of 2, 3, 4 and 6 stages, in one run: 16.4, 10.4, 9.6 and 10.7 ms.  Sums that
 // are kept as a double and modulo 2^64 (one FP64 instruction, three integer ones) for all, half or a third of the tiles: 13.2, 11.9 and 11.4 ms.
 #pragma once
 #include "pieces.cuh"

@@ -1267,7 +1267,8 @@ void embed_inverse(hb_ctx *c, i64 *coef, const double *re, const double *im, int
     }
 }
 // ---- plaintext operands from 4-bit weights ----
-// Operands that a launch of k_matvec reads: an upper bound of the call's memory.  Fewer of them, that stay in L2, are slower, since their passes are launches of one or two waves each: 2048 x 2048
+// Operands that a launch of k_matvec reads, as far as one limb of one column of blocks is not more (from 1024 K-groups of a full ring); the coefficients of the launch's blocks come on
+// top.  Fewer of them, that stay in L2, are slower, since their passes are launches of one or two waves each: 2048 x 2048
 // (33 MB a limb), at most 48, 210 and 512 MB: four vectors at level 5 518, 479 and 479 us, one at level 12 687, 637 and 615.
 constexpr size_t kMatvecBytes = (size_t)512 << 20;
 struct Tiles4 { int kb, nb; }; // K-groups of four row tiles, column tiles
@@ -1766,7 +1767,7 @@ int hb_matvec_q4(hb_ctx *c, const hb_ct *x, const hb_qweight *w, int tile, hb_ct
         hb_ct *r = new_ct(c, x->level, 2, vectors * t.nb, 2);
         try {
             ALG(c, x->limbs() + r->limbs());
-            // columns whose operands make one launch (a column of many K-groups several), and as many limbs at once as the bound allows: x is read once per set of columns
+            // columns whose operands make one launch (a column of many K-groups several), and as many limbs at once as kMatvecBytes holds: x is read once per set of columns
             const int columns = std::max(1, kBlocks4 / t.kb), N = c->N;
             for (int j = 0; j < t.nb; j += columns) {
                 const int m = std::min(columns, t.nb - j), blocks = m * t.kb, at_once = (int)std::clamp<size_t>(kMatvecBytes / ((size_t)blocks * N * 8), 1, (size_t)n);
@@ -1783,6 +1784,7 @@ int hb_matvec_q4(hb_ctx *c, const hb_ct *x, const hb_qweight *w, int tile, hb_ct
                         transform4(c, to, (const i64 *)coef.p + (size_t)k * N, some, l0, limbs);
                     }
                     const MatvecShape s{vectors, t.kb, m, t.nb, j, n, l0};
+                    // eight sums of a polynomial, four for one vector; vectors and columns past the end are multiplied and not stored (k_matvec has what that costs)
                     if (vectors == 1) launch_matvec<1, 4>(c, r->d, x->d, p.p, s, limbs);
                     else if (vectors == 2) launch_matvec<2, 4>(c, r->d, x->d, p.p, s, limbs);
                     else launch_matvec<4, 2>(c, r->d, x->d, p.p, s, limbs);

@@ -6,9 +6,10 @@
 // word is read once for four products.  Its lanes are LR x LC blocks of TR x TC pairs, side by side for 32 / (LR LC) residues; the words of all its tiles come
 // through a ring of stages in shared memory that belongs to the warp alone (16-byte asynchronous copies, several groups ahead), from which every lane reads the
 // tiles of its block.  The ring runs on from one range of residues to the next.
-// 8 groups, 6 heads, 4 query and 8 key tiles at level 5: 1.27 ms, with 5.4 GB (0.83 ms of HBM), 0.4 ms of FP64 and the 60-bit limb, a sixth of the products and a quarter of the time, which
-// overlap in part.  Words straight to registers: 2.2 ms.  Rings of 2, 3, 4, 6 and 8 stages: 1.95, 1.35, 1.30, 1.49 and 1.50 ms (the reads of the ring wait behind the copies in flight).  Twice
-// as many pairs a warp (8 x 4, 168 registers): 1.5 ms; boxes of 64 residues by tensor-map copies and a ring of the CTA: 1.54 ms.  One query tile with four key tiles: 267 us, 99 % of the bandwidth.
+// 8 groups, 6 heads, 4 query and 8 key tiles at level 5: 1.35 to 1.43 ms from box to box, with 5.4 GB (0.83 ms of HBM), 0.4 ms of FP64 and the 60-bit limb, a sixth of the products and a
+// quarter of the time, which overlap in part: the grid has one limb after the other, so the CTAs of an SM have the same kind of work.  Into an accumulator, whose words are loaded only where they
+// are added: 2.8 ms, with 1.8 GB more.  Words straight to registers: 2.2 ms.  Rings of 2, 3, 4, 6 and 8 stages, in one run: 1.95, 1.35, 1.30, 1.49 and 1.50 ms (the reads of the ring wait behind the copies in flight).  Twice
+// as many pairs a warp (8 x 4, 168 registers): 1.5 ms; boxes of 64 residues by tensor-map copies and a ring of the CTA: 1.54 ms.  One query tile with four key tiles: 270 us, 98 % of the bandwidth.
 // The middle sum comes from one product of the sums, (b1 + a1)(b2 + a2), from which the outer two are taken off at the end: three products a pair.
 #pragma once
 #include "kernels.cuh"

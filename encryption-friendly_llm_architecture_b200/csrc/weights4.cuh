@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(256) k_coef_small(const __grid_constant__ PtLi
 // coefficient of both polynomials of V vectors and of C columns: 2 V + C words for 2 V C products, as many in flight.  The blocks of one
 // range of coefficients run side by side.  Four vectors, 2048 x 2048, 4 K-groups: 36 us a limb, 68 MB of results and 17 MB of x in it (13 us of HBM, 18 with the operands), the rest the wait for
 // the words of a K-group (FP64 36 % active).  The whole call in CTAs of 128 threads and two K-groups a turn against 256 threads and one: four vectors 479 -> 463 us, one 325 -> 298,
-// one of 32 K-groups 736 -> 620; with the words of the next K-group in flight as well 505, 321 and 708, since the registers cost warps.  grid = (N / 128 * blocks, limbs)
+// one of 32 K-groups 736 -> 620; with the words of the next K-group in flight as well 505, 321 and 708, since the registers cost warps.
+// Three vectors take the block of four (2048 x 2048, level 5: 437 us for three, 458 for four), five that of eight (608 and 674).  grid = (N / 128 * blocks, limbs)
 struct MatvecShape { int vectors, kb, columns, nb, j0, n, l0; };
 template <int V, int C>
 __global__ void __launch_bounds__(128, V == 1 ? 5 : 3) k_matvec(u64 *out, const u64 *x, const u64 *p, MatvecShape s, const PrimeConst *__restrict__ pc, int N) {
