@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import numpy as np
 
-from .capi import Handle, Lib, HBError
+from .capi import Handle, Lib, HBError, _i32
 
 
 class CtxtTensor:
@@ -313,12 +313,12 @@ class Hemmer:
     # ---- tiles against tiles of another number ----
     def cross_matmul(self, a, b, heads=1, inner=1, target_level=4):
         """out[j][h][i] = sum_r a[r][h][i] @ b[r][h][j] for the tiles of `heads` heads, batch members in that order."""
-        ct = self._call("cross_matmul", a.ct.ptr, *self._shp(a), b.ct.ptr, *self._shp(b), C.c_int(heads), C.c_int(inner), C.c_int(target_level))
+        ct = self._call("cross_matmul", a.ct.ptr, *self._shp(a), b.ct.ptr, *self._shp(b), _i32(heads), _i32(inner), _i32(target_level))
         return CtxtTensor(ct, a.rows, b.cols, a.width)
 
     def cross_scores(self, query, key, heads=1, target_level=4):
         """cross_matmul with the transposed key tiles: member (j * heads + h) * nq + i is query tile i times key tile j transposed."""
-        ct = self._call("cross_scores_shaped", query.ct.ptr, *self._shp(query), key.ct.ptr, *self._shp(key), C.c_int(heads), C.c_int(target_level))
+        ct = self._call("cross_scores_shaped", query.ct.ptr, *self._shp(query), key.ct.ptr, *self._shp(key), _i32(heads), _i32(target_level))
         return CtxtTensor(ct, query.rows, key.rows, query.width)
 
     # ---- weights in 4 bits ----

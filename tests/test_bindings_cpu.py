@@ -108,3 +108,18 @@ def test_whole_numbers_beyond_32_bits(pkg, far):
         with pytest.raises(ValueError):
             call(far)
         assert not calls
+
+
+@pytest.mark.parametrize("far", [2**32 + 1, 2**31])
+def test_heads_and_tiles_beyond_32_bits(pkg, far):
+    calls = []
+    h = _hemmer(pkg)
+    h._call = lambda name, *a: calls.append(name)
+    t = pkg.CtxtTensor(SimpleNamespace(ptr=None), 16, 16, 32)
+    for call in (lambda: h.cross_matmul(t, t, heads=far), lambda: h.cross_matmul(t, t, inner=far), lambda: h.cross_matmul(t, t, target_level=far), lambda: h.cross_scores(t, t, heads=far),
+                 lambda: h.cross_scores(t, t, target_level=far)):
+        with pytest.raises(ValueError):
+            call()
+    assert not calls
+    h.cross_matmul(t, t), h.cross_scores(t, t)
+    assert len(calls) == 2
