@@ -424,6 +424,44 @@ class Lib:
         return self._op("matmul_acc_grouped", pre.ptr, _i32(inputs), which, (C.c_int32 * len(sizes))(*[_i32(n) for n in sizes]), C.c_int(len(sizes)), arr, C.c_int(bcount), C.c_int(tiles),
                         C.c_int64(row_step))
 
+    # ---- normalisation: members are [column tile][token tile] ----
+    def norm_squares(self, x, groups, mean=None, pad=0):
+        """sum_t tensor(x[t][b] - mean[b], itself) - pad * tensor(mean[b], mean[b]), un-relinearised."""
+        return self._op("norm_squares", x.ptr, mean.ptr if mean is not None else None, _i32(groups), _i32(pad))
+
+    def norm_scale(self, x, factor, groups, mean=None):
+        """tensor(x[t][b] - mean[b], factor[b] or factor[t][b]), un-relinearised."""
+        return self._op("norm_scale", x.ptr, mean.ptr if mean is not None else None, factor.ptr, _i32(groups))
+
+    def norm_affine(self, x, groups, gamma=None, beta=None):
+        """x[t][b] (.) gamma[t] + K beta[t], un-rescaled; without gamma x[t][b] + beta[t], which needs no rescale.  Lists of one plaintext per column tile."""
+        groups = _i32(groups)
+        for p in (gamma, beta):
+            if p is not None and len(p) != groups.value:
+                raise ValueError(f"{groups.value} column tiles, {len(p)} plaintexts")
+        lists = [None if p is None else (C.c_void_p * len(p))(*[q.ptr.value for q in p]) for p in (gamma, beta)]
+        return self._op("norm_affine", x.ptr, *lists, groups)
+
+    def norm_grad_sums(self, dy, xhat, groups, g=None):
+        """(rows, rowsum, cols, colsum): tensor sums of g (None: dy) with xhat over the column tiles, of dy with xhat over the token tiles, and plain sums of g and dy."""
+        outs = [C.c_void_p() for _ in range(4)]
+        self._chk(self._fn("norm_grad_sums")(self.ctx, dy.ptr, g.ptr if g is not None else None, xhat.ptr, _i32(groups), *[C.byref(o) for o in outs]))
+        return tuple(Handle(self, o, "ct") for o in outs)
+
+    def norm_grad_input(self, g, mean, xhat, dot, groups):
+        """K (g[t][b] - mean[b]) - tensor(xhat[t][b], dot[b]), un-relinearised."""
+        return self._op("norm_grad_input", g.ptr, mean.ptr, xhat.ptr, dot.ptr, _i32(groups))
+
+    def square_sum_many(self, xs):
+        """The sum of tensor(x, x) over all members of all handles: one member, un-relinearised."""
+        return self._op("square_sum_many", (C.c_void_p * len(xs))(*[x.ptr.value for x in xs]), _i32(len(xs)))
+
+    def scale_many(self, xs, factor):
+        """tensor(x, factor) for all members of all handles, a handle for each; the factor is one member."""
+        outs = (C.c_void_p * len(xs))()
+        self._chk(self._fn("scale_many")(self.ctx, (C.c_void_p * len(xs))(*[x.ptr.value for x in xs]), _i32(len(xs)), factor.ptr, outs))
+        return [Handle(self, C.c_void_p(p), "ct") for p in outs]
+
     def rotate_sum(self, xs, steps):
         """sum_t rot(xs[t], steps[t]) with one ModDown for the whole sum."""
         n = len(xs)

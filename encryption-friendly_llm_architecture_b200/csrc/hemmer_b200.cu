@@ -7,6 +7,7 @@
 #include "kernels.cuh"
 #include "pairs.cuh"
 #include "experts.cuh"
+#include "norms.cuh"
 #include "ntt.cuh"
 #include "convcols.cuh"
 #include "convmma.cuh"
@@ -1113,6 +1114,182 @@ hb_ct *do_tensor_pairs(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, in
     } catch (...) { if (!acc) hb_ct_free(r); throw; }
     return r;
 }
+// ---- sums of squares, products with one factor, gradients of a layer norm ----
+// rescaled pairs of one level
+void norm_operand(const hb_ctx *c, const hb_ct *x, const hb_ct *like, const std::string &what) {
+    if (!x) fail(HB_E_ARG, what + ": null argument");
+    own(c, x);
+    if (x->np != 2 || x->spow != 1) fail(HB_E_SHAPE, what + ": operands must be rescaled 2-poly ciphertexts");
+    if (x->level != like->level) fail(HB_E_LEVEL, what + ": level mismatch");
+}
+// members of a column tile
+int norm_batch(const hb_ct *x, int groups, const std::string &what) {
+    if (groups < 1 || x->batch % groups) fail(HB_E_SHAPE, what + ": the batch does not split into that many column tiles");
+    return x->batch / groups;
+}
+// one that all column tiles share
+void norm_shared(const hb_ctx *c, const hb_ct *m, const hb_ct *x, int batch, const std::string &what) {
+    norm_operand(c, m, x, what);
+    if (m->batch != batch) fail(HB_E_SHAPE, what + ": one member per member of a column tile");
+}
+void norm_blocks(i64 blocks, const std::string &what) { if (blocks > INT32_MAX) fail(HB_E_LIMIT, what + ": too many members"); }
+// the scale of a level as a whole number, modulo every prime: a term of a product's scale from one without a factor
+Scalars whole_scale(const hb_ctx *c, int level) {
+    Scalars k{};
+    const u64 whole = (u64)std::rint(c->h->scale[(size_t)level]);
+    for (int i = 0; i <= level; ++i) k.v[i] = whole % c->h->q[(size_t)i];
+    return k;
+}
+hb_ct *do_norm_squares(hb_ctx *c, const hb_ct *x, const hb_ct *mean, int groups, int pad) {
+    norm_operand(c, x, x, "norm_squares");
+    const int batch = norm_batch(x, groups, "norm_squares"), n = x->level + 1, N = c->N;
+    if (mean) norm_shared(c, mean, x, batch, "norm_squares");
+    if (pad < 0 || pad > c->h->slots || (pad && !mean)) fail(HB_E_ARG, "norm_squares: columns past the width are counted from 0 to the slots, and only beside a mean");
+    const i64 blocks = (i64)(N / 256) * batch * n;
+    norm_blocks(blocks, "norm_squares");
+    hb_ct *r = new_ct(c, x->level, 3, batch, 2);
+    try {
+        ALG(c, x->limbs() + (mean ? mean->limbs() : 0) + r->limbs());
+        const MemberRun run{x->d, (size_t)2 * n * N};
+        auto go = [&](auto *kernel) { launch(c, kernel, dim3((unsigned)blocks), 256, 0, r->d, run, mean ? mean->d : nullptr, groups, batch, (u64)pad, n, c->pc, N, 0); };
+        if (mean) go(k_square_sums<MemberRun, true>); else go(k_square_sums<MemberRun, false>);
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
+hb_ct *do_norm_scale(hb_ctx *c, const hb_ct *x, const hb_ct *mean, const hb_ct *factor, int groups) {
+    norm_operand(c, x, x, "norm_scale");
+    const int batch = norm_batch(x, groups, "norm_scale"), n = x->level + 1, N = c->N;
+    if (mean) norm_shared(c, mean, x, batch, "norm_scale");
+    norm_operand(c, factor, x, "norm_scale");
+    if (factor->batch != batch && factor->batch != x->batch) fail(HB_E_SHAPE, "norm_scale: a factor per member, or per member of a column tile");
+    const i64 blocks = (i64)(N / 256) * x->batch * n;
+    norm_blocks(blocks, "norm_scale");
+    hb_ct *r = new_ct(c, x->level, 3, x->batch, 2);
+    try {
+        ALG(c, x->limbs() + (mean ? mean->limbs() : 0) + factor->limbs() + r->limbs());
+        const MemberRun run{x->d, (size_t)2 * n * N};
+        const OutRun to{r->d, (size_t)3 * n * N};
+        auto go = [&](auto *kernel) { launch(c, kernel, dim3((unsigned)blocks), 256, 0, to, run, mean ? mean->d : nullptr, factor->d, batch, factor->batch, n, c->pc, N); };
+        if (mean) go(k_scale_members<MemberRun, OutRun, true>); else go(k_scale_members<MemberRun, OutRun, false>);
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
+hb_ct *do_norm_affine(hb_ctx *c, const hb_ct *x, const hb_pt *const *gamma, const hb_pt *const *beta, int groups) {
+    norm_operand(c, x, x, "norm_affine");
+    const int batch = norm_batch(x, groups, "norm_affine"), n = x->level + 1, N = c->N;
+    if (!gamma && !beta) fail(HB_E_ARG, "norm_affine: factors, addends or both");
+    for (const hb_pt *const *p : {gamma, beta})
+        for (int t = 0; p && t < groups; ++t) {
+            if (!p[t]) fail(HB_E_ARG, "norm_affine: null plaintext");
+            own(c, p[t]);
+            if (p[t]->level != x->level) fail(HB_E_LEVEL, "norm_affine: plaintext level differs from the ciphertexts'");
+            if (p[t]->spow != 1) fail(HB_E_SHAPE, "norm_affine: plaintext not rescaled");
+        }
+    norm_blocks((i64)(N / 256) * x->batch * n, "norm_affine");
+    hb_ct *r = new_ct(c, x->level, 2, x->batch, gamma ? 2 : 1);
+    try {
+        ALG(c, x->limbs() + r->limbs() + (size_t)groups * n * ((gamma ? 1 : 0) + (beta ? 1 : 0)));
+        const Scalars K = whole_scale(c, x->level);
+        for (int t0 = 0; t0 < groups; t0 += kNormTiles) {
+            const int some = std::min(kNormTiles, groups - t0);
+            AffineList a{};
+            a.tile0 = t0; a.batch = batch;
+            for (int t = 0; t < some; ++t) { a.gamma[t] = gamma ? gamma[t0 + t]->d : nullptr; a.beta[t] = beta ? beta[t0 + t]->d : nullptr; }
+            launch(c, k_affine, dim3((unsigned)(N / 256 * some * batch * n)), 256, 0, r->d, x->d, a, K, n, c->pc, N);
+        }
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
+// rows, rowsum, cols, colsum
+struct GradSums { hb_ct *r[4] = {}; };
+GradSums do_norm_grad_sums(hb_ctx *c, const hb_ct *dy, const hb_ct *g, const hb_ct *xhat, int groups) {
+    norm_operand(c, dy, dy, "norm_grad_sums");
+    const int batch = norm_batch(dy, groups, "norm_grad_sums"), n = dy->level + 1, N = c->N;
+    if (!g) g = dy;
+    for (const hb_ct *y : {g, xhat}) {
+        norm_operand(c, y, dy, "norm_grad_sums");
+        if (y->batch != dy->batch) fail(HB_E_SHAPE, "norm_grad_sums: batches differ");
+    }
+    norm_blocks((i64)(N / 256) * std::max(groups, batch) * n, "norm_grad_sums");
+    GradSums s;
+    try {
+        for (int k = 0; k < 4; ++k) s.r[k] = new_ct(c, dy->level, k % 2 ? 2 : 3, k < 2 ? batch : groups, k % 2 ? 1 : 2);
+        ALG(c, (g == dy ? 2 : 3) * dy->limbs() + (size_t)5 * (batch + groups) * n);
+        launch(c, k_grad_sums_one, dim3((unsigned)(N / 256 * batch * n)), 256, 0, s.r[0]->d, s.r[1]->d, g->d, xhat->d, groups, batch, 1, n, c->pc, N);
+        launch(c, k_grad_sums_one, dim3((unsigned)(N / 256 * groups * n)), 256, 0, s.r[2]->d, s.r[3]->d, dy->d, xhat->d, batch, 1, batch, n, c->pc, N);
+    } catch (...) { for (hb_ct *r : s.r) hb_ct_free(r); throw; }
+    return s;
+}
+hb_ct *do_norm_grad_input(hb_ctx *c, const hb_ct *g, const hb_ct *mean, const hb_ct *xhat, const hb_ct *dot, int groups) {
+    norm_operand(c, g, g, "norm_grad_input");
+    const int batch = norm_batch(g, groups, "norm_grad_input"), n = g->level + 1, N = c->N;
+    norm_operand(c, xhat, g, "norm_grad_input");
+    if (xhat->batch != g->batch) fail(HB_E_SHAPE, "norm_grad_input: batches differ");
+    for (const hb_ct *m : {mean, dot}) norm_shared(c, m, g, batch, "norm_grad_input");
+    const i64 blocks = (i64)(N / 256) * g->batch * n;
+    norm_blocks(blocks, "norm_grad_input");
+    hb_ct *r = new_ct(c, g->level, 3, g->batch, 2);
+    try {
+        ALG(c, 2 * g->limbs() + 2 * mean->limbs() + r->limbs());
+        launch(c, k_grad_input, dim3((unsigned)blocks), 256, 0, r->d, g->d, mean->d, xhat->d, dot->d, batch, whole_scale(c, g->level), n, c->pc, N);
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
+// handles of one level, and the members of all of them
+i64 list_members(hb_ctx *c, const hb_ct *const *xs, int count, const std::string &what) {
+    if (!xs || count < 1) fail(HB_E_ARG, what + ": no ciphertexts");
+    if (!xs[0]) fail(HB_E_ARG, what + ": null argument");
+    i64 members = 0;
+    for (int k = 0; k < count; ++k) { norm_operand(c, xs[k], xs[0], what); members += xs[k]->batch; }
+    return members;
+}
+hb_ct *do_square_sum_many(hb_ctx *c, const hb_ct *const *xs, int count) {
+    const i64 members = list_members(c, xs, count, "square_sum_many");
+    const int n = xs[0]->level + 1, N = c->N;
+    hb_ct *r = new_ct(c, xs[0]->level, 3, 1, 2);
+    try {
+        ALG(c, (size_t)members * 2 * n + r->limbs());
+        MemberList list;
+        int some = 0, first = 1;
+        auto flush = [&] {
+            if (!some) return;
+            launch(c, k_square_sums<MemberList, false>, dim3((unsigned)(N / 256 * n)), 256, 0, r->d, list, nullptr, some, 1, 0ull, n, c->pc, N, first ? 0 : 1);
+            some = first = 0;
+        };
+        for (int k = 0; k < count; ++k)
+            for (int i = 0; i < xs[k]->batch; ++i) {
+                list.p[some++] = xs[k]->d + (size_t)i * 2 * n * N;
+                if (some == kListMembers) flush();
+            }
+        flush();
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
+void do_scale_many(hb_ctx *c, const hb_ct *const *xs, int count, const hb_ct *factor, std::vector<hb_ct *> &r) {
+    list_members(c, xs, count, "scale_many");
+    norm_operand(c, factor, xs[0], "scale_many");
+    if (factor->batch != 1) fail(HB_E_SHAPE, "scale_many: one factor");
+    const int n = xs[0]->level + 1, N = c->N;
+    MemberList list;
+    OutList to;
+    int some = 0;
+    auto flush = [&] {
+        if (some) launch(c, k_scale_members<MemberList, OutList, false>, dim3((unsigned)(N / 256 * some * n)), 256, 0, to, list, nullptr, factor->d, 1, 1, n, c->pc, N);
+        some = 0;
+    };
+    ALG(c, factor->limbs());
+    for (int k = 0; k < count; ++k) {
+        r.push_back(nullptr);
+        r.back() = new_ct(c, xs[k]->level, 3, xs[k]->batch, 2);
+        ALG(c, xs[k]->limbs() + r.back()->limbs());
+        for (int i = 0; i < xs[k]->batch; ++i) {
+            list.p[some] = xs[k]->d + (size_t)i * 2 * n * N;
+            to.p[some++] = r.back()->d + (size_t)i * 3 * n * N;
+            if (some == kListMembers) flush();
+        }
+    }
+    flush();
+}
 hb_ct *do_level_down(hb_ctx *c, const hb_ct *a, int target) {
     own(c, a);
     if (target > a->level || target < 0) fail(HB_E_LEVEL, "level_down: bad target");
@@ -2167,6 +2344,36 @@ int hb_assemble_masked_into(hb_ctx *c, const hb_ct *a, const hb_digits *dg, cons
         if (a->np != 2 || dg->level != a->level || dg->batch != a->batch) fail(HB_E_SHAPE, "assemble_masked: digits do not belong to this ciphertext");
         if (!k1s || !dst) fail(HB_E_ARG, "assemble_masked: no keys or no destination");
         do_assemble_mk(c, a, dg->d, k1s, k2s, groups, dst, first);
+    });
+}
+int hb_norm_squares(hb_ctx *c, const hb_ct *x, const hb_ct *mean, int groups, int pad, hb_ct **out) {
+    return guard(c, [&] { if (!out) fail(HB_E_ARG, "norm_squares: null argument"); *out = do_norm_squares(c, x, mean, groups, pad); });
+}
+int hb_norm_scale(hb_ctx *c, const hb_ct *x, const hb_ct *mean, const hb_ct *factor, int groups, hb_ct **out) {
+    return guard(c, [&] { if (!out) fail(HB_E_ARG, "norm_scale: null argument"); *out = do_norm_scale(c, x, mean, factor, groups); });
+}
+int hb_norm_affine(hb_ctx *c, const hb_ct *x, const hb_pt *const *gamma, const hb_pt *const *beta, int groups, hb_ct **out) {
+    return guard(c, [&] { if (!out) fail(HB_E_ARG, "norm_affine: null argument"); *out = do_norm_affine(c, x, gamma, beta, groups); });
+}
+int hb_norm_grad_sums(hb_ctx *c, const hb_ct *dy, const hb_ct *g, const hb_ct *xhat, int groups, hb_ct **rows, hb_ct **rowsum, hb_ct **cols, hb_ct **colsum) {
+    return guard(c, [&] {
+        if (!rows || !rowsum || !cols || !colsum) fail(HB_E_ARG, "norm_grad_sums: null argument");
+        const GradSums s = do_norm_grad_sums(c, dy, g, xhat, groups);
+        *rows = s.r[0]; *rowsum = s.r[1]; *cols = s.r[2]; *colsum = s.r[3];
+    });
+}
+int hb_norm_grad_input(hb_ctx *c, const hb_ct *g, const hb_ct *mean, const hb_ct *xhat, const hb_ct *dot, int groups, hb_ct **out) {
+    return guard(c, [&] { if (!out) fail(HB_E_ARG, "norm_grad_input: null argument"); *out = do_norm_grad_input(c, g, mean, xhat, dot, groups); });
+}
+int hb_square_sum_many(hb_ctx *c, const hb_ct *const *xs, int count, hb_ct **out) {
+    return guard(c, [&] { if (!out) fail(HB_E_ARG, "square_sum_many: null argument"); *out = do_square_sum_many(c, xs, count); });
+}
+int hb_scale_many(hb_ctx *c, const hb_ct *const *xs, int count, const hb_ct *factor, hb_ct **out) {
+    return guard(c, [&] {
+        if (!out) fail(HB_E_ARG, "scale_many: null argument");
+        std::vector<hb_ct *> r;
+        try { do_scale_many(c, xs, count, factor, r); } catch (...) { for (hb_ct *x : r) hb_ct_free(x); throw; }
+        std::copy(r.begin(), r.end(), out);
     });
 }
 int hb_tensor_acc_groups(hb_ctx *c, const hb_ct *a, const hb_ct *b, int groups, hb_ct **acc) { return guard(c, [&] { *acc = do_tensor(c, a, b, *acc, groups); }); }

@@ -283,6 +283,28 @@ int hb_tensor_acc_groups(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, int groups
  * members in that order, b groups * heads * nk, of one level; *acc (NULL: created) nk * heads * nq, the key tile outermost, so that scores
  * can be the left operand of a product with the values.  Pair by pair the residues of hb_tensor_acc_groups. */
 int hb_tensor_acc_cross(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, int groups, int heads, hb_ct **acc);
+/* Normalisation.  No counterparts in the reference, which composes them of HomEvaluator calls.  Members x[t][b]: `groups` column tiles, outermost,
+ * of batch(x) / groups token tiles each; all operands of a call are rescaled pairs of one level.  (x): tensor product; m, r, mean and dot
+ * have one member per token tile.  What has three polynomials, or a factor, comes back un-relinearised and un-rescaled (scale power 2).
+ *   hb_norm_squares     out[b] = sum_t (x[t][b] - m[b]) (x) (x[t][b] - m[b]) - pad m[b] (x) m[b].  mean NULL: the sum of x (x) x.  pad (0 to the slots, only beside
+ *                       a mean): columns of the last tile past the width, where x is 0 and the difference -m
+ *   hb_norm_scale       out[t][b] = (x[t][b] - m[b]) (x) r[b], or (x) r[t][b] when the factor has as many members as x.  mean NULL: x (x) r
+ *   hb_norm_affine      out[t][b] = x[t][b] (.) gamma[t] + K beta[t], K the level's scale as a whole number, so that both terms have the scale of
+ *                       a product; beta NULL: none.  gamma NULL: out = x + beta[t], not multiplied and so with x's own scale.  `groups` plaintexts each, of x's level
+ *   hb_norm_grad_sums   rows[b] = sum_t g[t][b] (x) xhat[t][b] and rowsum[b] = sum_t g[t][b]; cols[t] = sum_b dy[t][b] (x) xhat[t][b] and
+ *                       colsum[t] = sum_b dy[t][b], which after a sum over the rows are the gradients of gamma and beta.  g NULL: dy.  The plain sums are rescaled pairs
+ *   hb_norm_grad_input  out[t][b] = K (g[t][b] - mean[b]) - xhat[t][b] (x) dot[b]: with the row means of g and of g xhat, relinearised, rescaled and multiplied by
+ *                       the inverse deviation, the gradient of a layer norm's input */
+int hb_norm_squares(hb_ctx *ctx, const hb_ct *x, const hb_ct *mean, int groups, int pad, hb_ct **out);
+int hb_norm_scale(hb_ctx *ctx, const hb_ct *x, const hb_ct *mean, const hb_ct *factor, int groups, hb_ct **out);
+int hb_norm_affine(hb_ctx *ctx, const hb_ct *x, const hb_pt *const *gamma, const hb_pt *const *beta, int groups, hb_ct **out);
+int hb_norm_grad_sums(hb_ctx *ctx, const hb_ct *dy, const hb_ct *g, const hb_ct *xhat, int groups, hb_ct **rows, hb_ct **rowsum, hb_ct **cols, hb_ct **colsum);
+int hb_norm_grad_input(hb_ctx *ctx, const hb_ct *g, const hb_ct *mean, const hb_ct *xhat, const hb_ct *dot, int groups, hb_ct **out);
+/* Many tensors at once, handles of any batch but one level.  hb_square_sum_many: out (one member) = the sum of x (x) x over all members of all handles, each of them
+ * read once: the square of their global norm, slot by slot.  hb_scale_many: out[k] (a handle per handle) = xs[k] (x) factor, the factor one member.  Un-relinearised
+ * and un-rescaled. */
+int hb_square_sum_many(hb_ctx *ctx, const hb_ct *const *xs, int count, hb_ct **out);
+int hb_scale_many(hb_ctx *ctx, const hb_ct *const *xs, int count, const hb_ct *factor, hb_ct **out);
 /* acc += tensor(first half of the members of x, second half); *acc may be NULL on entry */
 int hb_tensor_acc_halves(hb_ctx *ctx, const hb_ct *x, hb_ct **acc);
 /* out = sum_k pre[k] (.) rot_rows(pt, k * row_step), un-rescaled -- HomEvaluator::matmul :595-601 */

@@ -1,0 +1,281 @@
+"""hb_norm_*, hb_square_sum_many and hb_scale_many against sums of products of Python's own integers, member by member.  All results are whole numbers:
+equal or wrong."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from conftest import open_oracle, rand_ct_residues
+from test_gpu_tile_products import _ct, _points, _pt, _rand
+
+pytestmark = pytest.mark.gpu
+
+
+def _primes(g, n):
+    return np.array([int(q) for q in g.primes[:n]], dtype=object)[:, None]
+
+
+def _pair(x, y):
+    return np.stack([x[0] * y[0], x[0] * y[1] + x[1] * y[0], x[1] * y[1]])
+
+
+def _check(g, handle, expected, at, level, polys, scale_pow):
+    assert g.ct_meta(handle) == (level, polys, len(expected), scale_pow)
+    got = g.ct_export(handle)[..., at].astype(object)
+    want = np.stack([e % _primes(g, level + 1) for e in expected])
+    assert np.array_equal(got, want)
+
+
+def _objects(res, at):
+    return res[..., at].astype(object)
+
+
+def _scale(g, level):
+    return int(np.rint(g.scales[level]))
+
+
+SHAPES = [  # column tiles, token tiles, level
+    (1, 1, 3), (2, 1, 0), (3, 2, 5), (4, 3, 2), (5, 1, 1), (6, 4, 3), (7, 5, 2), (8, 1, 8), (9, 2, 1), (12, 3, 3), (13, 2, 2), (1, 17, 1), (33, 1, 2), (2, 40, 1), (130, 1, 0),
+]
+
+
+@pytest.fixture(params=["small", "mid"])
+def ring(request, gpu_small, gpu_mid):
+    return gpu_small if request.param == "small" else gpu_mid
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("T,B,level", SHAPES)
+def test_squares(ring, T, B, level, edge):
+    g = ring
+    x, mean = _rand(g, level, T * B, 1, edge=edge), _rand(g, level, B, 2)
+    if edge:  # differences as large as they get, of either sign
+        mean[::2] = 0
+        mean[1::2] = x[0]
+        x[: B // 2] = 0
+    at = _points(g, np.random.default_rng(T * 100 + B), 12)
+    xo, mo = _objects(x, at), _objects(mean, at)
+    cx, cm = _ct(g, x), _ct(g, mean)
+    for pad in (0, 1, g.slots):
+        want = [sum(_pair(xo[t * B + b] - mo[b], xo[t * B + b] - mo[b]) for t in range(T)) - pad * _pair(mo[b], mo[b]) for b in range(B)]
+        _check(g, g.norm_squares(cx, T, mean=cm, pad=pad), want, at, level, 3, 2)
+    _check(g, g.norm_squares(cx, T), [sum(_pair(xo[t * B + b], xo[t * B + b]) for t in range(T)) for b in range(B)], at, level, 3, 2)
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("T,B,level", SHAPES)
+def test_scale(ring, T, B, level, edge):
+    g = ring
+    x, mean, r, rr = _rand(g, level, T * B, 1, edge=edge), _rand(g, level, B, 2), _rand(g, level, B, 3, edge=edge), _rand(g, level, T * B, 4)
+    if edge:
+        mean[::2] = 0
+        x[: B // 2] = 0
+    at = _points(g, np.random.default_rng(T * 100 + B), 12)
+    xo, mo, ro, rro = (_objects(v, at) for v in (x, mean, r, rr))
+    cx, cm, cr, crr = (_ct(g, v) for v in (x, mean, r, rr))
+    of = [(k, k % B) for k in range(T * B)]
+    _check(g, g.norm_scale(cx, cr, T, mean=cm), [_pair(xo[k] - mo[b], ro[b]) for k, b in of], at, level, 3, 2)
+    _check(g, g.norm_scale(cx, cr, T), [_pair(xo[k], ro[b]) for k, b in of], at, level, 3, 2)
+    _check(g, g.norm_scale(cx, crr, T, mean=cm), [_pair(xo[k] - mo[b], rro[k]) for k, b in of], at, level, 3, 2)
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("T,B,level", SHAPES)
+def test_affine(ring, T, B, level, edge):
+    g = ring
+    x = _rand(g, level, T * B, 1, edge=edge)
+    gamma, beta = (_rand(g, level, T, s, polys=1, edge=edge)[:, 0] for s in (2, 3))
+    at = _points(g, np.random.default_rng(T * 100 + B), 12)
+    xo, go, bo = (_objects(v, at) for v in (x, gamma, beta))
+    cx, pg, pb, K = _ct(g, x), [_pt(g, v) for v in gamma], [_pt(g, v) for v in beta], _scale(g, level)
+    of = [(k, k // B) for k in range(T * B)]
+    _check(g, g.norm_affine(cx, T, gamma=pg, beta=pb), [np.stack([xo[k][0] * go[t] + K * bo[t], xo[k][1] * go[t]]) for k, t in of], at, level, 2, 2)
+    _check(g, g.norm_affine(cx, T, gamma=pg), [np.stack([xo[k][0] * go[t], xo[k][1] * go[t]]) for k, t in of], at, level, 2, 2)
+    _check(g, g.norm_affine(cx, T, beta=pb), [np.stack([xo[k][0] + bo[t], xo[k][1]]) for k, t in of], at, level, 2, 1)
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("T,B,level", SHAPES)
+def test_grad_sums(ring, T, B, level, edge):
+    g = ring
+    dy, gg, xh = (_rand(g, level, T * B, s, edge=edge) for s in (1, 2, 3))
+    at = _points(g, np.random.default_rng(T * 100 + B), 12)
+    do, go, xo = (_objects(v, at) for v in (dy, gg, xh))
+    cd, cg, cx = (_ct(g, v) for v in (dy, gg, xh))
+    for handle, y in ((cg, go), (None, do)):
+        got = g.norm_grad_sums(cd, cx, T, g=handle)
+        _check(g, got[0], [sum(_pair(y[t * B + b], xo[t * B + b]) for t in range(T)) for b in range(B)], at, level, 3, 2)
+        _check(g, got[1], [sum(y[t * B + b] for t in range(T)) for b in range(B)], at, level, 2, 1)
+        _check(g, got[2], [sum(_pair(do[t * B + b], xo[t * B + b]) for b in range(B)) for t in range(T)], at, level, 3, 2)
+        _check(g, got[3], [sum(do[t * B + b] for b in range(B)) for t in range(T)], at, level, 2, 1)
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("T,B,level", SHAPES)
+def test_grad_input(ring, T, B, level, edge):
+    g = ring
+    gg, xh, mean, dot = _rand(g, level, T * B, 1, edge=edge), _rand(g, level, T * B, 2, edge=edge), _rand(g, level, B, 3), _rand(g, level, B, 4, edge=edge)
+    if edge:  # the largest differences, and factors of nothing
+        mean[::2] = 0
+        xh[: B // 2] = 0
+    at = _points(g, np.random.default_rng(T * 100 + B), 12)
+    go, xo, mo, ao = (_objects(v, at) for v in (gg, xh, mean, dot))
+    K, nothing = _scale(g, level), 0 * go[0][:1]
+    want = [np.concatenate([K * (go[k] - mo[k % B]), nothing]) - _pair(xo[k], ao[k % B]) for k in range(T * B)]
+    _check(g, g.norm_grad_input(*(_ct(g, v) for v in (gg, mean, xh, dot)), T), want, at, level, 3, 2)
+
+
+LISTS = [[1], [3], [1, 1], [1] * 7, [2, 5, 1], [1, 4, 1, 9, 2], [31, 2], [64], [130, 126], [255, 2], [257], [1] * 40 + [100] * 5]
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("sizes", LISTS, ids=lambda s: f"{len(s)}x{sum(s)}")
+def test_square_sum_many(ring, sizes, edge):
+    g, level = ring, 2 if sum(sizes) < 100 else 1
+    xs = [_rand(g, level, m, 10 + k, edge=edge) for k, m in enumerate(sizes)]
+    at = _points(g, np.random.default_rng(len(sizes)), 12)
+    want = sum(_pair(m, m) for x in xs for m in _objects(x, at))
+    handles = [_ct(g, x) for x in xs]
+    _check(g, g.square_sum_many(handles), [want], at, level, 3, 2)
+    _check(g, g.square_sum_many(handles + handles[:1]), [want + sum(_pair(m, m) for m in _objects(xs[0], at))], at, level, 3, 2)   # the same handle twice
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("sizes", LISTS, ids=lambda s: f"{len(s)}x{sum(s)}")
+def test_scale_many(ring, sizes, edge):
+    g, level = ring, 2 if sum(sizes) < 100 else 1
+    xs, f = [_rand(g, level, m, 10 + k, edge=edge) for k, m in enumerate(sizes)], _rand(g, level, 1, 9, edge=edge)
+    at = _points(g, np.random.default_rng(len(sizes)), 12)
+    handles, cf, fo = [_ct(g, x) for x in xs], _ct(g, f), _objects(f, at)[0]
+    got = g.scale_many(handles + handles[:1] + [cf], cf)   # the same handle twice, and the factor itself
+    assert len(got) == len(xs) + 2
+    for h, x in zip(got, xs + xs[:1] + [f]):
+        _check(g, h, [_pair(m, fo) for m in _objects(x, at)], at, level, 3, 2)
+    _check(g, cf, _objects(f, at), at, level, 2, 1)
+
+
+@pytest.mark.parametrize("n_bits", [(58, 58), (50, 50), (44, 60), (43, 60)])
+def test_primes_of_other_lengths(pkg, n_bits):
+    """Scaling primes that leave room for eight products of a sum, and those that go by pieces."""
+    g = pkg.open_gpu(pkg.make_params(log_n=10, max_level=4, dnum=3 if n_bits[0] < 50 else 5, num_special=3, q0_bits=60, q_bits=n_bits[0], p_bits=60, hamming_weight=32))
+    try:
+        level, T, B = 3, 19, 2
+        at = np.arange(g.N)
+        x, mean, r = _rand(g, level, T * B, 1, edge=True), _rand(g, level, B, 2), _rand(g, level, B, 3, edge=True)
+        mean[0] = 0
+        xo, mo, ro = (_objects(v, at) for v in (x, mean, r))
+        cx, cm, cr = (_ct(g, v) for v in (x, mean, r))
+        _check(g, g.norm_squares(cx, T, mean=cm, pad=7), [sum(_pair(xo[t * B + b] - mo[b], xo[t * B + b] - mo[b]) for t in range(T)) - 7 * _pair(mo[b], mo[b]) for b in range(B)], at, level, 3, 2)
+        _check(g, g.norm_scale(cx, cr, T, mean=cm), [_pair(xo[k] - mo[k % B], ro[k % B]) for k in range(T * B)], at, level, 3, 2)
+        rows, rowsum, cols, colsum = g.norm_grad_sums(cx, cx, T)
+        _check(g, rows, [sum(_pair(xo[t * B + b], xo[t * B + b]) for t in range(T)) for b in range(B)], at, level, 3, 2)
+        _check(g, colsum, [sum(xo[t * B + b] for b in range(B)) for t in range(T)], at, level, 2, 1)
+        _check(g, cols, [sum(_pair(xo[t * B + b], xo[t * B + b]) for b in range(B)) for t in range(T)], at, level, 3, 2)
+        K, nothing = _scale(g, level), 0 * xo[0][:1]
+        _check(g, g.norm_grad_input(cx, cm, cx, cr, T), [np.concatenate([K * (xo[k] - mo[k % B]), nothing]) - _pair(xo[k], ro[k % B]) for k in range(T * B)], at, level, 3, 2)
+        _check(g, g.square_sum_many([cx, cm]), [sum(_pair(v, v) for v in [*xo, *mo])], at, level, 3, 2)
+    finally:
+        g.close()
+
+
+def test_views_and_whole_calls_of_the_library_agree(gpu_small):
+    """Runs of members without a copy as operands, and the residues of hb_tensor, hb_sub and hb_add."""
+    g = gpu_small
+    T, B, level = 3, 2, 4
+    x, m, r = _ct(g, _rand(g, level, T * B + 3, 1)), _ct(g, _rand(g, level, B, 2)), _ct(g, _rand(g, level, B, 3))
+    view = g._op("batch_view", x.ptr, C.c_int(2), C.c_int(T * B))
+    acc = None
+    for t in range(T):
+        d = g.sub(g._op("batch_view", view.ptr, C.c_int(t * B), C.c_int(B)), m)
+        assert np.array_equal(g.ct_export(g.tensor(d, r)), g.ct_export(g.norm_scale(view, r, T, mean=m))[t * B:(t + 1) * B])
+        acc = g.tensor(d, d) if acc is None else g.add(acc, g.tensor(d, d))
+    assert np.array_equal(g.ct_export(acc), g.ct_export(g.norm_squares(view, T, mean=m)))
+
+
+def test_replayed_from_a_graph(gpu_small):
+    g = gpu_small
+    T, B, level = 4, 2, 3
+    res = {k: _rand(g, level, n, s) for s, (k, n) in enumerate([("x", T * B), ("y", T * B), ("m", B), ("r", B), ("f", 1)])}
+    h = {k: _ct(g, v) for k, v in res.items()}
+    pts = [_pt(g, v[0]) for v in _rand(g, level, T, 9, polys=1)]
+
+    def all_calls():
+        return [g.norm_squares(h["x"], T, mean=h["m"], pad=3), g.norm_scale(h["x"], h["r"], T, mean=h["m"]), g.norm_affine(h["x"], T, gamma=pts, beta=pts),
+                *g.norm_grad_sums(h["x"], h["y"], T), g.norm_grad_input(h["x"], h["m"], h["y"], h["r"], T), g.square_sum_many([h["x"], h["r"]]), *g.scale_many([h["x"], h["m"]], h["f"])]
+
+    want = [g.ct_export(o) for o in all_calls()]
+    g.graph_begin()
+    outs = all_calls()
+    graph = g.graph_end()
+    for k in h:   # other values while the graph does not run, then its own again
+        g.ct_import(h[k], np.zeros_like(res[k]))
+    g.graph_launch(graph)
+    assert all(not g.ct_export(o).any() for o in outs[:2] + outs[3:])   # the affine part keeps its addend
+    for k in h:
+        g.ct_import(h[k], res[k])
+    for _ in range(2):
+        g.graph_launch(graph)
+    for o, w in zip(outs, want):
+        assert np.array_equal(g.ct_export(o), w)
+
+
+def test_refusals(pkg, gpu_small, gpu_mid):
+    g, level, T, B = gpu_small, 3, 2, 2
+    x, m, f = _ct(g, _rand(g, level, T * B, 1)), _ct(g, _rand(g, level, B, 2)), _ct(g, _rand(g, level, 1, 3))
+    low, three, raw = _ct(g, _rand(g, level - 1, B, 4)), _ct(g, _rand(g, level, B, 5, polys=3), 2), _ct(g, _rand(g, level, B, 6), 2)
+    other = _ct(gpu_mid, _rand(gpu_mid, level, B, 7))
+    p, plow = [_pt(g, _rand(g, level, 1, 8, polys=1)[0, 0])] * 2, [_pt(g, _rand(g, level - 1, 1, 8, polys=1)[0, 0])] * 2
+    ARG, LEVEL, SHAPE = -1, -2, -3
+
+    def refused(code, call, *a, **k):
+        before = g.ct_export(x)
+        with pytest.raises(pkg.HBError) as e:
+            call(*a, **k)
+        assert e.value.code == code, e.value
+        assert np.array_equal(g.ct_export(x), before)
+
+    for groups in (0, -1, 3, 5):
+        refused(SHAPE, g.norm_squares, x, groups)
+        refused(SHAPE, g.norm_scale, x, m, groups)
+        refused(SHAPE, g.norm_grad_sums, x, x, groups)
+        refused(SHAPE, g.norm_grad_input, x, m, x, m, groups)
+    for groups in (3, 5):
+        refused(SHAPE, g.norm_affine, x, groups, gamma=p[:1] * groups)
+    refused(SHAPE, g._op, "norm_affine", x.ptr, None, None, C.c_int(0))
+    for bad, code in ((low, LEVEL), (three, SHAPE), (raw, SHAPE), (other, ARG), (x, SHAPE), (f, SHAPE)):
+        refused(code, g.norm_squares, x, T, mean=bad)
+        if bad is not x:   # a factor per member
+            refused(code, g.norm_scale, x, bad, T)
+        refused(code, g.norm_scale, x, m, T, mean=bad)
+        refused(code, g.norm_grad_input, x, bad, x, m, T)
+        refused(code, g.norm_grad_input, x, m, x, bad, T)
+        if bad is not x:
+            refused(code, g.norm_grad_input, x, m, bad, m, T)
+            refused(code, g.norm_grad_sums, x, bad, T)
+            refused(code, g.norm_grad_sums, x, x, T, g=bad)
+    refused(ARG, g.norm_squares, x, T, pad=1)
+    refused(ARG, g.norm_squares, x, T, mean=m, pad=-1)
+    refused(ARG, g.norm_squares, x, T, mean=m, pad=g.slots + 1)
+    refused(ARG, g.norm_affine, x, T)
+    refused(LEVEL, g.norm_affine, x, T, gamma=plow)
+    refused(LEVEL, g.norm_affine, x, T, gamma=p, beta=plow)
+    refused(ARG, g.square_sum_many, [])
+    refused(ARG, g.scale_many, [], f)
+    for bad, code in ((low, LEVEL), (three, SHAPE), (raw, SHAPE), (other, ARG)):
+        refused(code, g.square_sum_many, [x, bad])
+        refused(code, g.scale_many, [x, bad], f)
+    refused(SHAPE, g.scale_many, [x], m)
+    refused(LEVEL, g.scale_many, [x], _ct(g, _rand(g, level - 1, 1, 4)))
+    with pytest.raises(ValueError):
+        g.norm_affine(x, T, gamma=p[:1])
+    with pytest.raises(ValueError):
+        g.norm_squares(x, 2 ** 32 + 2)
+    # nulls through the C entries
+    out, null = C.c_void_p(), (C.c_void_p * 2)()
+    for name, args in (("norm_squares", (None, None, 1, 0)), ("norm_scale", (x.ptr, None, None, 2)), ("norm_grad_input", (x.ptr, None, x.ptr, m.ptr, 2)), ("norm_affine", (x.ptr, null, None, 2)),
+                       ("square_sum_many", (null, 2)), ("square_sum_many", (None, 2)), ("norm_grad_sums", (x.ptr, None, None, 2))):
+        extra = [C.byref(out)] * (4 if name == "norm_grad_sums" else 1)
+        assert g._fn(name)(g.ctx, *args, *extra) == ARG and not out.value
+        assert g._fn(name)(g.ctx, *args, *[None] * len(extra)) == ARG
+    assert g._fn("scale_many")(g.ctx, null, 2, f.ptr, null) == ARG
+    assert g._fn("scale_many")(g.ctx, (C.c_void_p * 1)(x.ptr.value), 1, f.ptr, None) == ARG
