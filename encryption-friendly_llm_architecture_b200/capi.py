@@ -12,6 +12,7 @@ import numpy as np
 c_u64p = C.POINTER(C.c_uint64)
 c_f64p = C.POINTER(C.c_double)
 c_i64p = C.POINTER(C.c_int64)
+_Int4 = C.c_int * 4
 
 
 class Params(C.Structure):
@@ -247,9 +248,9 @@ class Lib:
         return Handle(self, out, "ct")
 
     def ct_meta(self, ct):
-        v = [C.c_int() for _ in range(4)]
-        self._fn("ct_meta")(ct.ptr, *[C.byref(x) for x in v])
-        return tuple(x.value for x in v)  # level, n_poly, batch, scale_pow
+        v = _Int4()
+        self._fn("ct_meta")(ct.ptr, C.byref(v), C.byref(v, 4), C.byref(v, 8), C.byref(v, 12))
+        return tuple(v[:])  # level, n_poly, batch, scale_pow
 
     def pt_meta(self, pt):
         v = [C.c_int() for _ in range(2)]

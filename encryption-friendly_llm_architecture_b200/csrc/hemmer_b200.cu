@@ -1132,7 +1132,6 @@ void norm_shared(const hb_ctx *c, const hb_ct *m, const hb_ct *x, int batch, con
     norm_operand(c, m, x, what);
     if (m->batch != batch) fail(HB_E_SHAPE, what + ": one member per member of a column tile");
 }
-void norm_blocks(i64 blocks, const std::string &what) { if (blocks > INT32_MAX) fail(HB_E_LIMIT, what + ": too many members"); }
 // the scale of a level as a whole number, modulo every prime: a term of a product's scale from one without a factor
 Scalars whole_scale(const hb_ctx *c, int level) {
     Scalars k{};
@@ -1140,19 +1139,31 @@ Scalars whole_scale(const hb_ctx *c, int level) {
     for (int i = 0; i <= level; ++i) k.v[i] = whole % c->h->q[(size_t)i];
     return k;
 }
+// `each` members of every column, so many a CTA
+Walk walk(const hb_ctx *c, int each, int step, int n) { return {each, step, norm_chunk(each, (long)(c->N / kNormLanes) * n, step)}; }
+dim3 walk_grid(const hb_ctx *c, const Walk &w, int n, const std::string &what) {
+    const i64 z = (i64)w.step * ((w.each + w.chunk - 1) / w.chunk);
+    if (z > 65535) fail(HB_E_LIMIT, what + ": too many members");
+    return dim3((unsigned)(c->N / kNormLanes), (unsigned)n, (unsigned)z);
+}
 hb_ct *do_norm_squares(hb_ctx *c, const hb_ct *x, const hb_ct *mean, int groups, int pad) {
     norm_operand(c, x, x, "norm_squares");
     const int batch = norm_batch(x, groups, "norm_squares"), n = x->level + 1, N = c->N;
     if (mean) norm_shared(c, mean, x, batch, "norm_squares");
     if (pad < 0 || pad > c->h->slots || (pad && !mean)) fail(HB_E_ARG, "norm_squares: columns past the width are counted from 0 to the slots, and only beside a mean");
-    const i64 blocks = (i64)(N / 256) * batch * n;
-    norm_blocks(blocks, "norm_squares");
+    const int log_splits = norm_log_splits(groups, (long)(N / kNormLanes) * batch * n), chunk = norm_chunk(batch, (long)(N / kNormLanes << log_splits) * n, 1);
+    const dim3 grid((unsigned)(N / kNormLanes << log_splits), (unsigned)n, (unsigned)((batch + chunk - 1) / chunk));
     hb_ct *r = new_ct(c, x->level, 3, batch, 2);
     try {
         ALG(c, x->limbs() + (mean ? mean->limbs() : 0) + r->limbs());
         const MemberRun run{x->d, (size_t)2 * n * N};
-        auto go = [&](auto *kernel) { launch(c, kernel, dim3((unsigned)blocks), 256, 0, r->d, run, mean ? mean->d : nullptr, groups, batch, (u64)pad, n, c->pc, N, 0); };
-        if (mean) go(k_square_sums<MemberRun, true>); else go(k_square_sums<MemberRun, false>);
+        auto go = [&](auto *kernel) { launch(c, kernel, grid, 256, 0, r->d, run, mean ? mean->d : nullptr, SquareShape{groups, batch, chunk, log_splits, (u64)pad}, n, c->pc, N, 0); };
+        const int turn = norm_turn((groups + (1 << log_splits) - 1) >> log_splits);
+        if (!mean) go(k_square_sums<MemberRun, false, 4>);
+        else if (turn == 1) go(k_square_sums<MemberRun, true, 1>);
+        else if (turn == 2) go(k_square_sums<MemberRun, true, 2>);
+        else if (turn == 3) go(k_square_sums<MemberRun, true, 3>);
+        else go(k_square_sums<MemberRun, true, 4>);
     } catch (...) { hb_ct_free(r); throw; }
     return r;
 }
@@ -1162,15 +1173,18 @@ hb_ct *do_norm_scale(hb_ctx *c, const hb_ct *x, const hb_ct *mean, const hb_ct *
     if (mean) norm_shared(c, mean, x, batch, "norm_scale");
     norm_operand(c, factor, x, "norm_scale");
     if (factor->batch != batch && factor->batch != x->batch) fail(HB_E_SHAPE, "norm_scale: a factor per member, or per member of a column tile");
-    const i64 blocks = (i64)(N / 256) * x->batch * n;
-    norm_blocks(blocks, "norm_scale");
+    const Walk w = walk(c, groups, batch, n);
+    const dim3 grid = walk_grid(c, w, n, "norm_scale");
     hb_ct *r = new_ct(c, x->level, 3, x->batch, 2);
     try {
         ALG(c, x->limbs() + (mean ? mean->limbs() : 0) + factor->limbs() + r->limbs());
         const MemberRun run{x->d, (size_t)2 * n * N};
         const OutRun to{r->d, (size_t)3 * n * N};
-        auto go = [&](auto *kernel) { launch(c, kernel, dim3((unsigned)blocks), 256, 0, to, run, mean ? mean->d : nullptr, factor->d, batch, factor->batch, n, c->pc, N); };
-        if (mean) go(k_scale_members<MemberRun, OutRun, true>); else go(k_scale_members<MemberRun, OutRun, false>);
+        auto go = [&](auto *kernel) { launch(c, kernel, grid, 256, 0, to, run, mean ? mean->d : nullptr, factor->d, w, n, c->pc, N); };
+        const bool each = factor->batch != batch;
+        if (mean) { if (each) go(k_scale_members<MemberRun, OutRun, true, true>); else go(k_scale_members<MemberRun, OutRun, true, false>); }
+        else if (each) go(k_scale_members<MemberRun, OutRun, false, true>);
+        else go(k_scale_members<MemberRun, OutRun, false, false>);
     } catch (...) { hb_ct_free(r); throw; }
     return r;
 }
@@ -1185,7 +1199,6 @@ hb_ct *do_norm_affine(hb_ctx *c, const hb_ct *x, const hb_pt *const *gamma, cons
             if (p[t]->level != x->level) fail(HB_E_LEVEL, "norm_affine: plaintext level differs from the ciphertexts'");
             if (p[t]->spow != 1) fail(HB_E_SHAPE, "norm_affine: plaintext not rescaled");
         }
-    norm_blocks((i64)(N / 256) * x->batch * n, "norm_affine");
     hb_ct *r = new_ct(c, x->level, 2, x->batch, gamma ? 2 : 1);
     try {
         ALG(c, x->limbs() + r->limbs() + (size_t)groups * n * ((gamma ? 1 : 0) + (beta ? 1 : 0)));
@@ -1195,7 +1208,9 @@ hb_ct *do_norm_affine(hb_ctx *c, const hb_ct *x, const hb_pt *const *gamma, cons
             AffineList a{};
             a.tile0 = t0; a.batch = batch;
             for (int t = 0; t < some; ++t) { a.gamma[t] = gamma ? gamma[t0 + t]->d : nullptr; a.beta[t] = beta ? beta[t0 + t]->d : nullptr; }
-            launch(c, k_affine, dim3((unsigned)(N / 256 * some * batch * n)), 256, 0, r->d, x->d, a, K, n, c->pc, N);
+            a.tiles = some; a.chunk = norm_chunk(batch, (long)(N / kNormLanes) * n, some);
+            const dim3 grid((unsigned)(N / kNormLanes), (unsigned)n, (unsigned)(some * ((batch + a.chunk - 1) / a.chunk)));
+            if (gamma) launch(c, k_affine<true>, grid, 256, 0, r->d, x->d, a, K, n, c->pc, N); else launch(c, k_affine<false>, grid, 256, 0, r->d, x->d, a, K, n, c->pc, N);
         }
     } catch (...) { hb_ct_free(r); throw; }
     return r;
@@ -1210,13 +1225,31 @@ GradSums do_norm_grad_sums(hb_ctx *c, const hb_ct *dy, const hb_ct *g, const hb_
         norm_operand(c, y, dy, "norm_grad_sums");
         if (y->batch != dy->batch) fail(HB_E_SHAPE, "norm_grad_sums: batches differ");
     }
-    norm_blocks((i64)(N / 256) * std::max(groups, batch) * n, "norm_grad_sums");
     GradSums s;
     try {
         for (int k = 0; k < 4; ++k) s.r[k] = new_ct(c, dy->level, k % 2 ? 2 : 3, k < 2 ? batch : groups, k % 2 ? 1 : 2);
         ALG(c, (g == dy ? 2 : 3) * dy->limbs() + (size_t)5 * (batch + groups) * n);
-        launch(c, k_grad_sums_one, dim3((unsigned)(N / 256 * batch * n)), 256, 0, s.r[0]->d, s.r[1]->d, g->d, xhat->d, groups, batch, 1, n, c->pc, N);
-        launch(c, k_grad_sums_one, dim3((unsigned)(N / 256 * groups * n)), 256, 0, s.r[2]->d, s.r[3]->d, dy->d, xhat->d, batch, 1, batch, n, c->pc, N);
+        for (int t0 = 0; t0 < groups;) {
+            const int some = std::min(grad_tiles(groups), groups - t0);
+            auto go = [&](auto tiles, auto same) {
+                launch(c, k_grad_sums<decltype(tiles)::value, decltype(same)::value>, dim3((unsigned)(N / 128), (unsigned)n), 128, 0, s.r[0]->d, s.r[1]->d, s.r[2]->d, s.r[3]->d, dy->d, g->d, xhat->d,
+                       GradShape{batch, t0}, n, c->pc, N);
+            };
+            auto by_tiles = [&](auto same) {
+                switch (some) {
+                case 1: go(std::integral_constant<int, 1>{}, same); break;
+                case 2: go(std::integral_constant<int, 2>{}, same); break;
+                case 3: go(std::integral_constant<int, 3>{}, same); break;
+                case 4: go(std::integral_constant<int, 4>{}, same); break;
+                case 5: go(std::integral_constant<int, 5>{}, same); break;
+                case 6: go(std::integral_constant<int, 6>{}, same); break;
+                case 7: go(std::integral_constant<int, 7>{}, same); break;
+                default: go(std::integral_constant<int, 8>{}, same);
+                }
+            };
+            if (g == dy) by_tiles(std::true_type{}); else by_tiles(std::false_type{});
+            t0 += some;
+        }
     } catch (...) { for (hb_ct *r : s.r) hb_ct_free(r); throw; }
     return s;
 }
@@ -1226,12 +1259,12 @@ hb_ct *do_norm_grad_input(hb_ctx *c, const hb_ct *g, const hb_ct *mean, const hb
     norm_operand(c, xhat, g, "norm_grad_input");
     if (xhat->batch != g->batch) fail(HB_E_SHAPE, "norm_grad_input: batches differ");
     for (const hb_ct *m : {mean, dot}) norm_shared(c, m, g, batch, "norm_grad_input");
-    const i64 blocks = (i64)(N / 256) * g->batch * n;
-    norm_blocks(blocks, "norm_grad_input");
+    const Walk w = walk(c, groups, batch, n);
+    const dim3 grid = walk_grid(c, w, n, "norm_grad_input");
     hb_ct *r = new_ct(c, g->level, 3, g->batch, 2);
     try {
         ALG(c, 2 * g->limbs() + 2 * mean->limbs() + r->limbs());
-        launch(c, k_grad_input, dim3((unsigned)blocks), 256, 0, r->d, g->d, mean->d, xhat->d, dot->d, batch, whole_scale(c, g->level), n, c->pc, N);
+        launch(c, k_grad_input, grid, 256, 0, r->d, g->d, mean->d, xhat->d, dot->d, w, whole_scale(c, g->level), n, c->pc, N);
     } catch (...) { hb_ct_free(r); throw; }
     return r;
 }
@@ -1253,7 +1286,8 @@ hb_ct *do_square_sum_many(hb_ctx *c, const hb_ct *const *xs, int count) {
         int some = 0, first = 1;
         auto flush = [&] {
             if (!some) return;
-            launch(c, k_square_sums<MemberList, false>, dim3((unsigned)(N / 256 * n)), 256, 0, r->d, list, nullptr, some, 1, 0ull, n, c->pc, N, first ? 0 : 1);
+            const int log_splits = norm_log_splits(some, (long)(N / kNormLanes) * n);
+            launch(c, k_square_sums<MemberList, false, 4>, dim3((unsigned)(N / kNormLanes << log_splits), (unsigned)n), 256, 0, r->d, list, nullptr, SquareShape{some, 1, 1, log_splits, 0}, n, c->pc, N, first ? 0 : 1);
             some = first = 0;
         };
         for (int k = 0; k < count; ++k)
@@ -1274,7 +1308,8 @@ void do_scale_many(hb_ctx *c, const hb_ct *const *xs, int count, const hb_ct *fa
     OutList to;
     int some = 0;
     auto flush = [&] {
-        if (some) launch(c, k_scale_members<MemberList, OutList, false>, dim3((unsigned)(N / 256 * some * n)), 256, 0, to, list, nullptr, factor->d, 1, 1, n, c->pc, N);
+        const Walk w = walk(c, some, 1, n);
+        if (some) launch(c, k_scale_members<MemberList, OutList, false, false>, walk_grid(c, w, n, "scale_many"), 256, 0, to, list, nullptr, factor->d, w, n, c->pc, N);
         some = 0;
     };
     ALG(c, factor->limbs());

@@ -142,4 +142,26 @@ constexpr int pair_ranges(PairBlock b, int N, int nr, int nc, int heads, int lim
     return run;
 }
 
+// Members that a CTA takes one after the other where they share a factor: as many as leave `enough` CTAs, eight at most, but more where a grid of 65535 a column of
+// members would not reach them.  `each`: CTAs with one chunk for all members; `columns` of them side by side.
+constexpr int norm_chunk(int members, long each, long columns) {
+    int chunk = members < 8 ? members : 8;
+    while (chunk > 1 && each * columns * ((members + chunk - 1) / chunk) < 148 * 8) --chunk;
+    while (columns * ((members + chunk - 1L) / chunk) > 65535 && chunk < members) ++chunk;
+    return chunk;
+}
+// Parts of the members of a sum, as a power of two up to eight: more while there are CTAs missing and every part has some members left.  `each`: CTAs without parts.
+constexpr int norm_log_splits(int members, long each) {
+    int log = 0;
+    while (log < 3 && (each << log) < 148 * 4 && members >= 4 << log) ++log;
+    return log;
+}
+// Members that a sum of `members` multiplies a turn.  Calls at level 5, us, with two, three and four: 5 of 8 token tiles 84 80 -, 6 of 4 48 43 51, 12 of 4 - 69 68.
+constexpr int norm_turn(int members) { return members <= 4 ? members : members == 5 || members == 6 || members == 9 ? 3 : 4; }
+// Column tiles of a launch of the sums in both directions: even launches of at most eight.
+constexpr int grad_tiles(int tiles) {
+    const int launches = (tiles + 7) / 8;
+    return (tiles + launches - 1) / launches;
+}
+
 } // namespace hb

@@ -9,6 +9,7 @@
 // Sums are exact until one reduction at their end (FpAcc, PieceAcc).
 #pragma once
 #include "kernels.cuh"
+#include <type_traits>
 
 namespace hb {
 
@@ -16,27 +17,76 @@ namespace hb {
 struct FpField { // primes below 2^44: whole numbers in doubles, differences with their sign
     using Value = double;
     using Sum = FpAcc;
+    struct Plain { // of residues, as many between two reductions as a sum has room for products: below 2^49
+        double v;
+        __device__ __forceinline__ void zero() { v = 0.0; }
+        __device__ __forceinline__ void add(double x) { v += x; }
+        __device__ __forceinline__ u64 canonical(const PrimeConst &m) const { return canon_fp64(v, m.q_inv_f, (double)m.q); }
+        __device__ __forceinline__ void relax(const PrimeConst &m) { v = u52_to_double(canonical(m)); }
+    };
+    struct Lean { // of products that are reduced one by one: half the registers of a Sum, seven instructions a product instead of four
+        double v;
+        __device__ __forceinline__ void zero() { v = 0.0; }
+        __device__ __forceinline__ void add(const Lean &x, const PrimeConst &) { v += x.v; }
+        __device__ __forceinline__ void set(double a, double b, const PrimeConst &m) { v = mul_fp64_lazy(a, b, m.q_inv_f, (double)m.q); }
+        __device__ __forceinline__ void set(double a, double b, double c, double d, const PrimeConst &m) { v = mul_fp64_lazy(a, b, m.q_inv_f, (double)m.q) + mul_fp64_lazy(c, d, m.q_inv_f, (double)m.q); }
+        __device__ __forceinline__ u64 canonical(const PrimeConst &m) const { return canon_fp64(v, m.q_inv_f, (double)m.q); } // 64 products below 2^44 in magnitude: below 2^50
+        __device__ __forceinline__ void relax(const PrimeConst &m) { v = u52_to_double(canonical(m)); }
+    };
     const PrimeConst &m;
     __device__ __forceinline__ explicit FpField(const PrimeConst &m_) : m(m_) {}
     __device__ __forceinline__ double value(u64 x) const { return u52_to_double(x); }
     __device__ __forceinline__ double minus(double a, double b) const { return a - b; }
     __device__ __forceinline__ double negative(double a) const { return -a; }
-    __device__ __forceinline__ int room() const { return m.q < (1ull << 42) ? 128 : 8; } // products of a sum before it is reduced
+    static constexpr int kFewest = 8; // products of a sum before it is reduced, for the longest of these primes
+    __device__ __forceinline__ int room() const { return m.q < (1ull << 42) ? 128 : kFewest; }
 };
 struct PieceField { // 45 to 60 bits
     using Value = u64;
     using Sum = PieceAcc;
+    struct Plain { // of nine residues at most
+        u64 v;
+        __device__ __forceinline__ void zero() { v = 0; }
+        __device__ __forceinline__ void add(u64 x) { v += x; }
+        __device__ __forceinline__ u64 canonical(const PrimeConst &m) const { return canon_q(v, m.q, FoldQ{m.fold_shift, (1u << m.fold_shift) - 1u, m.fold_d}); }
+        __device__ __forceinline__ void relax(const PrimeConst &m) { v = canonical(m); }
+    };
+    struct Lean {
+        u64 v;
+        __device__ __forceinline__ void zero() { v = 0; }
+        __device__ __forceinline__ void add(const Lean &x, const PrimeConst &m) { v = add_mod(v, x.v, m.q); }
+        __device__ __forceinline__ void set(u64 a, u64 b, const PrimeConst &m) { PieceAcc s; s.zero(); s.mac(a, b); v = s.finish(m); }
+        __device__ __forceinline__ void set(u64 a, u64 b, u64 c, u64 d, const PrimeConst &m) { PieceAcc s; s.zero(); s.mac(a, b); s.mac(c, d); v = s.finish(m); }
+        __device__ __forceinline__ u64 canonical(const PrimeConst &) const { return v; }
+        __device__ __forceinline__ void relax(const PrimeConst &) {}
+    };
     const PrimeConst &m;
     __device__ __forceinline__ explicit PieceField(const PrimeConst &m_) : m(m_) {}
     __device__ __forceinline__ u64 value(u64 x) const { return x; }
     __device__ __forceinline__ u64 minus(u64 a, u64 b) const { return sub_mod(a, b, m.q); }
     __device__ __forceinline__ u64 negative(u64 a) const { return m.q - a; } // up to q: products stay below 2^120
-    __device__ __forceinline__ int room() const { return 8; }
+    static constexpr int kFewest = 8;
+    __device__ __forceinline__ int room() const { return kFewest; }
 };
 template <class F> __device__ __forceinline__ void by_prime(const PrimeConst &m, F &&f) {
     if (m.fp) f(FpField(m)); else f(PieceField(m));
 }
-__device__ __forceinline__ u64 twice_mod(u64 a, u64 q) { return add_mod(a, a, q); }
+
+// Two residues side by side: 16 bytes a load, and two chains of arithmetic a thread.
+struct Two { u64 v[2]; };
+__device__ __forceinline__ Two load2(const u64 *p) { const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(p); return {{x.x, x.y}}; }
+__device__ __forceinline__ void store2(u64 *p, const Two &x) { *reinterpret_cast<ulonglong2 *>(p) = make_ulonglong2(x.v[0], x.v[1]); }
+// a polynomial pair at two residues
+struct Pair {
+    Two p[2];
+    // at a short offset from an address that all threads share: whole pointers would take more registers than the words
+    __device__ __forceinline__ void load(const u64 *from, size_t poly, u32 at) { p[0] = load2(from + at); p[1] = load2(from + poly + at); }
+    template <class F, class V> __device__ __forceinline__ void values(const F &f, V (&v0)[2], V (&v1)[2]) const {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) { v0[e] = f.value(p[0].v[e]); v1[e] = f.value(p[1].v[e]); }
+    }
+};
+constexpr int kNormLanes = 512; // residues of a CTA: two a thread
 
 // Members one after the other, or wherever a list says.
 struct MemberRun {
@@ -59,133 +109,351 @@ struct OutList {
     __device__ __forceinline__ u64 *at(int i) const { return p[i]; }
 };
 
-// out[b] (+)= the sum over t < groups.  grid = N / 256 * batch * n, the residues of a limb side by side
-template <class MEMBERS, bool MEAN>
-__global__ void __launch_bounds__(256) k_square_sums(u64 *out, const __grid_constant__ MEMBERS x, const u64 *mean, int groups, int batch, u64 pad, int n, const PrimeConst *__restrict__ pc, int N, int accumulate) {
-    const u32 px = N / 256, row = blockIdx.x / px;
-    const int b = (int)row / n, l = (int)row % n;
-    const u32 i = blockIdx.x % px * 256 + threadIdx.x;
+// out[b] (+)= the sum over t < groups, for `chunk` token tiles one after the other.  Threads of a CTA: `splits` parts (a power of two) of the members by 512 / splits residues; the
+// parts are joined in shared memory, in order.  A register that has been multiplied is filled again at once, with the member four further on or the first one of the next token tile.
+// grid = (N splits / 512, n, chunks): quotients by sizes would take a fifth of the instructions
+struct SquareShape { int groups, batch, chunk, log_splits; u64 pad; };
+// U members are multiplied a turn; where a part has fewer left, the first turn takes the mean (or zeros) for the ones that are not there, whose squares are nothing: a product behind a
+// branch would make the sums change registers.
+template <class MEMBERS, bool MEAN, int U>
+__global__ void __launch_bounds__(256, U == 1 ? 3 : 2) k_square_sums(u64 *out, const __grid_constant__ MEMBERS x, const u64 *mean, SquareShape w, int n, const PrimeConst *__restrict__ pc, int N,
+                                                                                 int accumulate) {
+    __shared__ __align__(16) u64 parts[2][3][kNormLanes];
+    const int splits = 1 << w.log_splits, wide = 256 >> w.log_splits, lane = threadIdx.x & (wide - 1), part = threadIdx.x >> (8 - w.log_splits);
+    const int l = blockIdx.y, first = blockIdx.z * w.chunk, last = min(first + w.chunk, w.batch);
     const PrimeConst m = pc[l];
-    const size_t poly = (size_t)n * N, at = (size_t)l * N + i;
+    const size_t poly = (size_t)n * N;
+    const u32 at = (u32)(l * N) + (blockIdx.x * wide + lane) * 2;
+    const int count = (w.groups - part + splits - 1) >> w.log_splits, turns = (count + U - 1) / U, some = count - (turns - 1) * U; // members of this part, those of the first turn
+    Pair v[U], mr{};
+    auto load = [&](int u, int t, int b) { v[u].load(x.at((t + u * splits) * w.batch + b), poly, at); };
     pdl_wait();
+    // the first words do not wait for the constants of the prime
+    if (MEAN) mr.load(mean + (size_t)first * 2 * poly, poly, at);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (u < some) load(u, part, first);
+        else v[u] = mr;
+    }
     by_prime(m, [&](auto f) {
         using V = typename decltype(f)::Value;
-        typename decltype(f)::Sum s[3];
-        for (auto &k : s) k.zero();
-        V m0{}, m1{};
-        if (MEAN) { m0 = f.value(mean[b * 2 * poly + at]); m1 = f.value(mean[(b * 2 + 1) * poly + at]); }
-        for (int t = 0; t < groups; ++t) {
-            if (t && t % f.room() == 0) for (auto &k : s) k.relax(m);
-            const u64 *p = x.at(t * batch + b) + at;
-            V v0 = f.value(p[0]), v1 = f.value(p[poly]);
-            if (MEAN) { v0 = f.minus(v0, m0); v1 = f.minus(v1, m1); }
-            s[0].mac(v0, v0); s[1].mac(v0, v1); s[2].mac(v1, v1);
+        using Sum = typename decltype(f)::Sum;
+#pragma unroll 1
+        for (int b = first; b < last; ++b) {
+            Sum s[3][2];
+            V m0[2], m1[2];
+            if (MEAN) {
+                mr.values(f, m0, m1);
+                if (b + 1 < last) mr.load(mean + (size_t)(b + 1) * 2 * poly, poly, at);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                s[0][e].zero(); s[1][e].zero(); s[2][e].zero();
+            }
+            int t = part + some * splits, held = 0; // the next turn's first member; products of a sum
+#pragma unroll 1
+            for (int turn = 0; turn < turns; ++turn) {
+                if ((held += U) > f.room()) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) { s[k][0].relax(m); s[k][1].relax(m); }
+                    held = U;
+                }
+                const bool on = turn + 1 < turns;
+                const int t2 = on ? t : part, b2 = on ? b : b + 1, there = on ? U : b + 1 < last ? some : 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    V v0[2], v1[2];
+                    v[u].values(f, v0, v1);
+                    if (u < there) load(u, t2, b2);
+                    else if (U > 1) v[u] = mr;
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (MEAN) { v0[e] = f.minus(v0[e], m0[e]); v1[e] = f.minus(v1[e], m1[e]); }
+                        s[0][e].mac(v0[e], v0[e]); s[1][e].mac(v0[e], v1[e]); s[2][e].mac(v1[e], v1[e]);
+                    }
+                }
+                t += U * splits;
+            }
+            Two r[3];
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) r[k].v[e] = s[k][e].canonical(m);
+            if (MEAN && w.pad && part == 0) { // less the squares of the columns past the width
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[0][e].zero(); s[1][e].zero(); s[2][e].zero();
+                    s[0][e].mac(m0[e], m0[e]); s[1][e].mac(m0[e], m1[e]); s[2][e].mac(m1[e], m1[e]);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) r[k].v[e] = sub_mod(r[k].v[e], mul_mod_any(s[k][e].canonical(m), w.pad, m), m.q);
+                }
+            }
+            if (splits > 1) { // the buffers take turns: that of b - 1 is read before the barrier of b, which stands before the writes of b + 1
+                auto &buf = parts[b & 1];
+#pragma unroll
+                for (int k = 0; k < 3; ++k) store2(&buf[k][2 * threadIdx.x], r[k]);
+                __syncthreads();
+                if (part) continue;
+                for (int j = 1; j < splits; ++j)
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) {
+                        const Two y = load2(&buf[k][2 * (threadIdx.x + j * wide)]);
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) r[k].v[e] = add_mod(r[k].v[e], y.v[e], m.q);
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) r[1].v[e] = add_mod(r[1].v[e], r[1].v[e], m.q);
+            u64 *o = out + (size_t)b * 3 * poly + at;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) {
+                if (accumulate) {
+                    const Two y = load2(o + k * poly);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) r[k].v[e] = add_mod(r[k].v[e], y.v[e], m.q);
+                }
+                store2(o + k * poly, r[k]);
+            }
         }
-        u64 r[3] = {s[0].canonical(m), s[1].canonical(m), s[2].canonical(m)};
-        if (MEAN && pad) {
-            for (auto &k : s) k.zero();
-            s[0].mac(m0, m0); s[1].mac(m0, m1); s[2].mac(m1, m1);
-            for (int k = 0; k < 3; ++k) r[k] = sub_mod(r[k], mul_mod_any(s[k].canonical(m), pad, m), m.q);
-        }
-        r[1] = twice_mod(r[1], m.q);
-        u64 *o = out + (size_t)b * 3 * poly + at;
-        for (int k = 0; k < 3; ++k) o[k * poly] = accumulate ? add_mod(r[k], o[k * poly], m.q) : r[k];
     });
 }
-// out[i] = (x[i] - mean[i % batch]) (x) r[i % factors].  grid = N / 256 * members * n
-template <class MEMBERS, class OUT, bool MEAN>
-__global__ void __launch_bounds__(256) k_scale_members(const __grid_constant__ OUT out, const __grid_constant__ MEMBERS x, const u64 *mean, const u64 *r, int batch, int factors, int n, const PrimeConst *__restrict__ pc, int N) {
-    const u32 px = N / 256, row = blockIdx.x / px;
-    const int k = (int)row / n, l = (int)row % n;
-    const u32 i = blockIdx.x % px * 256 + threadIdx.x;
+// Members c, c + step, ... of a column c < step, `each` of them; a CTA takes a chunk of them one after the other.
+struct Walk { int each, step, chunk; };
+// out[i] = (x[i] - mean[c]) (x) r[c] for the members i = c, c + step, ... of column c < step: mean and factor are read once for a chunk of members.  EACH: a factor per member.
+// grid = (N / 512, n, step * chunks)
+template <class MEMBERS, class OUT, bool MEAN, bool EACH>
+__global__ void __launch_bounds__(256, 4) k_scale_members(const __grid_constant__ OUT out, const __grid_constant__ MEMBERS x, const u64 *mean, const u64 *r, Walk w, int n, const PrimeConst *__restrict__ pc, int N) {
+    const int l = blockIdx.y, c = (int)(blockIdx.z % (u32)w.step), first = (int)(blockIdx.z / (u32)w.step) * w.chunk, last = min(first + w.chunk, w.each);
     const PrimeConst m = pc[l];
-    const size_t poly = (size_t)n * N, at = (size_t)l * N + i;
+    const size_t poly = (size_t)n * N;
+    const u32 at = (u32)(l * N) + (blockIdx.x * 256 + threadIdx.x) * 2;
+    Pair rr, mr{}, xr, er{};
     pdl_wait();
+    // the first words do not wait for the constants of the prime, and those of the next member are in flight while this one is multiplied
+    if (!EACH) rr.load(r + (size_t)c * 2 * poly, poly, at);
+    if (MEAN) mr.load(mean + (size_t)c * 2 * poly, poly, at);
+    auto fetch = [&](int t) {
+        const int i = t * w.step + c;
+        xr.load(x.at(i), poly, at);
+        if (EACH) er.load(r + (size_t)i * 2 * poly, poly, at);
+    };
+    fetch(first);
     by_prime(m, [&](auto f) {
         using V = typename decltype(f)::Value;
-        const u64 *p = x.at(k) + at, *rp = r + (size_t)(k % factors) * 2 * poly + at;
-        V v0 = f.value(p[0]), v1 = f.value(p[poly]);
-        const V r0 = f.value(rp[0]), r1 = f.value(rp[poly]);
-        if (MEAN) {
-            const u64 *mp = mean + (size_t)(k % batch) * 2 * poly + at;
-            v0 = f.minus(v0, f.value(mp[0])); v1 = f.minus(v1, f.value(mp[poly]));
+        V r0[2], r1[2], m0[2], m1[2];
+        if (!EACH) rr.values(f, r0, r1);
+        if (MEAN) mr.values(f, m0, m1);
+#pragma unroll 1
+        for (int t = first; t < last; ++t) {
+            V v0[2], v1[2];
+            xr.values(f, v0, v1);
+            if (EACH) er.values(f, r0, r1);
+            if (t + 1 < last) fetch(t + 1);
+            Two d[3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (MEAN) { v0[e] = f.minus(v0[e], m0[e]); v1[e] = f.minus(v1[e], m1[e]); }
+                typename decltype(f)::Sum s[3];
+                s[0].zero(); s[1].zero(); s[2].zero();
+                s[0].mac(v0[e], r0[e]); s[1].mac(v0[e], r1[e]); s[1].mac(v1[e], r0[e]); s[2].mac(v1[e], r1[e]);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) d[k].v[e] = s[k].canonical(m);
+            }
+            u64 *o = out.at(t * w.step + c) + at;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) store2(o + k * poly, d[k]);
         }
-        typename decltype(f)::Sum s[3];
-        for (auto &e : s) e.zero();
-        s[0].mac(v0, r0); s[1].mac(v0, r1); s[1].mac(v1, r0); s[2].mac(v1, r1);
-        u64 *o = out.at(k) + at;
-        for (int e = 0; e < 3; ++e) o[e * poly] = s[e].canonical(m);
     });
 }
 // Plaintexts of the column tiles.
 constexpr int kNormTiles = 128; // of a launch
-struct AffineList { const u64 *gamma[kNormTiles], *beta[kNormTiles]; int tile0, batch; };
-// members of the tiles tile0 ..: out = x gamma + K beta on the first polynomial, x gamma on the second; without gammas x + beta.  grid = N / 256 * members * n
-__global__ void __launch_bounds__(256) k_affine(u64 *out, const u64 *x, const __grid_constant__ AffineList a, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc, int N) {
-    const u32 px = N / 256, row = blockIdx.x / px;
-    const int k = (int)row / n, l = (int)row % n, t = k / a.batch;
-    const u32 i = blockIdx.x % px * 256 + threadIdx.x;
+struct AffineList { const u64 *gamma[kNormTiles], *beta[kNormTiles]; int tile0, tiles, batch, chunk; };
+// members of the tiles tile0 ..: out = x gamma + K beta on the first polynomial, x gamma on the second; without gammas x + beta.  A CTA takes a chunk of one tile's members.
+// grid = (N / 512, n, tiles * chunks)
+template <bool GAMMA>
+__global__ void __launch_bounds__(256, 4) k_affine(u64 *out, const u64 *x, const __grid_constant__ AffineList a, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc, int N) {
+    const int l = blockIdx.y, t = (int)(blockIdx.z % (u32)a.tiles), first = (int)(blockIdx.z / (u32)a.tiles) * a.chunk, last = min(first + a.chunk, a.batch);
     const PrimeConst m = pc[l];
-    const size_t poly = (size_t)n * N, at = (size_t)l * N + i;
+    const size_t poly = (size_t)n * N;
+    const u32 at = (u32)(l * N) + (blockIdx.x * 256 + threadIdx.x) * 2;
+    const size_t from = ((size_t)a.tile0 + t) * a.batch * 2 * poly;
+    Two be{}, ga{};
+    Pair xr;
+    auto fetch = [&](int b) { xr.load(x + from + (size_t)b * 2 * poly, poly, at); };
     pdl_wait();
+    if (a.beta[t]) be = load2(a.beta[t] + at);
+    if (GAMMA) ga = load2(a.gamma[t] + at);
+    fetch(first);
     by_prime(m, [&](auto f) {
-        const u64 *p = x + (size_t)(a.tile0 * a.batch + k) * 2 * poly + at;
-        u64 *o = out + (size_t)(a.tile0 * a.batch + k) * 2 * poly + at;
-        if (!a.gamma[t]) {
-            o[0] = a.beta[t] ? add_mod(p[0], a.beta[t][at], m.q) : p[0];
-            o[poly] = p[poly];
-            return;
+        using V = typename decltype(f)::Value;
+        V g[2] = {};
+        if (GAMMA) {
+            const V k = f.value(K.v[l]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                g[e] = f.value(ga.v[e]);
+                typename decltype(f)::Sum s;
+                s.zero();
+                s.mac(f.value(be.v[e]), k);
+                be.v[e] = s.canonical(m);
+            }
         }
-        const auto g = f.value(a.gamma[t][at]);
-        typename decltype(f)::Sum s[2];
-        for (auto &e : s) e.zero();
-        s[0].mac(f.value(p[0]), g); s[1].mac(f.value(p[poly]), g);
-        if (a.beta[t]) s[0].mac(f.value(a.beta[t][at]), f.value(K.v[l]));
-        o[0] = s[0].canonical(m); o[poly] = s[1].canonical(m);
+#pragma unroll 1
+        for (int b = first; b < last; ++b) {
+            Two v0 = xr.p[0], v1 = xr.p[1];
+            if (b + 1 < last) fetch(b + 1);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (GAMMA) {
+                    typename decltype(f)::Sum s[2];
+                    s[0].zero(); s[1].zero();
+                    s[0].mac(f.value(v0.v[e]), g[e]); s[1].mac(f.value(v1.v[e]), g[e]);
+                    v0.v[e] = s[0].canonical(m); v1.v[e] = s[1].canonical(m);
+                }
+                v0.v[e] = add_mod(v0.v[e], be.v[e], m.q);
+            }
+            u64 *o = out + from + (size_t)b * 2 * poly + at;
+            store2(o, v0); store2(o + poly, v1);
+        }
     });
 }
-// Sums over one index: out[j] = sum_i y(i, j) (x) xhat(i, j) and sum[j] = sum_i y(i, j), member(i, j) = i * by_i + j * by_j.  grid = N / 256 * results * n
-__global__ void __launch_bounds__(256) k_grad_sums_one(u64 *out, u64 *sum, const u64 *y, const u64 *xhat, int terms, int by_i, int by_j, int n, const PrimeConst *__restrict__ pc, int N) {
-    const u32 px = N / 256, row = blockIdx.x / px;
-    const int j = (int)row / n, l = (int)row % n;
-    const u32 i = blockIdx.x % px * 256 + threadIdx.x;
+// Both directions in one pass over dy, g and xhat.  A thread has one residue of TT column tiles: their sums over b stay in its registers, a word each, the sums over t of one b are written (+= for
+// all but the first tiles of a call).  The words of W tiles are in flight; a register that has been multiplied is filled again at once.  SAME: g is dy.
+// grid = (N / 128, n)
+struct GradShape { int batch, tile0; };
+constexpr int grad_ctas(int TT, bool SAME) { return TT == 1 ? 7 : TT == 2 ? 5 : TT == 3 ? 4 : TT == 7 || (TT == 5 && !SAME) ? 2 : 3; }
+template <int TT, bool SAME>
+__global__ void __launch_bounds__(128, grad_ctas(TT, SAME)) k_grad_sums(u64 *rows, u64 *rowsum, u64 *cols, u64 *colsum, const u64 *dy, const u64 *g, const u64 *xhat, GradShape w, int n, const PrimeConst *__restrict__ pc, int N) {
+    constexpr int W = TT == 8 ? 2 : TT == 6 ? 3 : TT;
+    static_assert(TT % W == 0, "a tile's words have their place in the registers");
+    const int l = blockIdx.y;
     const PrimeConst m = pc[l];
-    const size_t poly = (size_t)n * N, at = (size_t)l * N + i;
+    // an address is one that all threads share, and a short offset: pointers of every tile and polynomial would take more registers than the sums
+    const size_t poly = (size_t)n * N, per_tile = (size_t)w.batch * 2 * poly;
+    const u32 at = (u32)(l * N) + blockIdx.x * 128 + threadIdx.x;
+    size_t from = (size_t)w.tile0 * per_tile;
+    u64 v[W][6];
+    auto fetch = [&](int t, size_t i) {
+        i += t * per_tile;
+        u64 (&y)[6] = v[t % W];
+        y[0] = (xhat + i)[at]; y[1] = (xhat + i + poly)[at]; y[2] = (dy + i)[at]; y[3] = (dy + i + poly)[at];
+        if (!SAME) { y[4] = (g + i)[at]; y[5] = (g + i + poly)[at]; }
+    };
     pdl_wait();
+#pragma unroll
+    for (int t = 0; t < W; ++t) fetch(t, from);
     by_prime(m, [&](auto f) {
-        typename decltype(f)::Sum s[3];
-        for (auto &e : s) e.zero();
-        u64 p0 = 0, p1 = 0;
-        for (int e = 0; e < terms; ++e) {
-            if (e && e % (f.room() / 2) == 0) for (auto &k : s) k.relax(m);
-            const size_t from = ((size_t)e * by_i + (size_t)j * by_j) * 2 * poly + at;
-            p0 = add_mod(p0, y[from], m.q); p1 = add_mod(p1, y[from + poly], m.q);
-            const auto y0 = f.value(y[from]), y1 = f.value(y[from + poly]), x0 = f.value(xhat[from]), x1 = f.value(xhat[from + poly]);
-            s[0].mac(y0, x0); s[1].mac(y0, x1); s[1].mac(y1, x0); s[2].mac(y1, x1);
+        using F = decltype(f);
+        using Rows = std::conditional_t<SAME, typename F::Lean, typename F::Sum>;
+        typename F::Lean c[TT][3];
+        typename F::Plain cs[TT][2];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+#pragma unroll
+            for (int k = 0; k < 3; ++k) c[t][k].zero();
+            cs[t][0].zero(); cs[t][1].zero();
         }
-        u64 *o = out + (size_t)j * 3 * poly + at;
-        for (int e = 0; e < 3; ++e) o[e * poly] = s[e].canonical(m);
-        sum[(size_t)j * 2 * poly + at] = p0; sum[((size_t)j * 2 + 1) * poly + at] = p1;
+        int held = 0;
+#pragma unroll 1
+        for (int b = 0; b < w.batch; ++b) {
+            if (held == F::kFewest) { // members of a plain sum; a lean one has room for 32
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) c[t][k].relax(m);
+                    cs[t][0].relax(m); cs[t][1].relax(m);
+                }
+                held = 0;
+            }
+            ++held;
+            Rows r[3];
+            typename F::Plain rs[2];
+#pragma unroll
+            for (int k = 0; k < 3; ++k) r[k].zero();
+            rs[0].zero(); rs[1].zero();
+            const bool on = b + 1 < w.batch;
+#pragma unroll
+            for (int t = 0; t < TT; ++t) {
+                const u64 (&y)[6] = v[t % W];
+                const auto x0 = f.value(y[0]), x1 = f.value(y[1]), d0 = f.value(y[2]), d1 = f.value(y[3]), g0 = SAME ? d0 : f.value(y[4]), g1 = SAME ? d1 : f.value(y[5]);
+                if (t + W < TT) fetch(t + W, from);
+                else if (on) fetch(t + W - TT, from + 2 * poly);
+                typename F::Lean p[3];
+                p[0].set(d0, x0, m); p[1].set(d0, x1, d1, x0, m); p[2].set(d1, x1, m);
+#pragma unroll
+                for (int k = 0; k < 3; ++k) c[t][k].add(p[k], m);
+                cs[t][0].add(d0); cs[t][1].add(d1);
+                if constexpr (SAME) {
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) r[k].add(p[k], m);
+                } else {
+                    if (t && t % (F::kFewest / 2) == 0 && f.room() / 2 < TT) {
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) r[k].relax(m);
+                    }
+                    r[0].mac(g0, x0); r[1].mac(g0, x1); r[1].mac(g1, x0); r[2].mac(g1, x1);
+                }
+                rs[0].add(g0); rs[1].add(g1);
+            }
+            from += 2 * poly;
+            const u64 res[5] = {r[0].canonical(m), r[1].canonical(m), r[2].canonical(m), rs[0].canonical(m), rs[1].canonical(m)};
+            u64 *const o = rows + (size_t)b * 3 * poly, *const os = rowsum + (size_t)b * 2 * poly;
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                u64 *p = (k < 3 ? o + k * poly : os + (k - 3) * poly) + at;
+                *p = w.tile0 ? add_mod(res[k], *p, m.q) : res[k];
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            u64 *const o = cols + (size_t)(w.tile0 + t) * 3 * poly + at, *const os = colsum + (size_t)(w.tile0 + t) * 2 * poly + at;
+#pragma unroll
+            for (int k = 0; k < 3; ++k) o[k * poly] = c[t][k].canonical(m);
+            os[0] = cs[t][0].canonical(m); os[poly] = cs[t][1].canonical(m);
+        }
     });
 }
-// grid = N / 256 * members * n
-__global__ void __launch_bounds__(256) k_grad_input(u64 *out, const u64 *g, const u64 *mean, const u64 *xhat, const u64 *dot, int batch, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc, int N) {
-    const u32 px = N / 256, row = blockIdx.x / px;
-    const int k = (int)row / n, l = (int)row % n, b = k % batch;
-    const u32 i = blockIdx.x % px * 256 + threadIdx.x;
+// members c, c + step, ... of token tile c < step share mean and dot, which are read once for a chunk of them.  grid = (N / 512, n, step * chunks)
+__global__ void __launch_bounds__(256, 3) k_grad_input(u64 *out, const u64 *g, const u64 *mean, const u64 *xhat, const u64 *dot, Walk w, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc,
+                                                       int N) {
+    const int l = blockIdx.y, c = (int)(blockIdx.z % (u32)w.step), first = (int)(blockIdx.z / (u32)w.step) * w.chunk, last = min(first + w.chunk, w.each);
     const PrimeConst m = pc[l];
-    const size_t poly = (size_t)n * N, at = (size_t)l * N + i, from = (size_t)k * 2 * poly + at, of = (size_t)b * 2 * poly + at;
+    const size_t poly = (size_t)n * N;
+    const u32 at = (u32)(l * N) + (blockIdx.x * 256 + threadIdx.x) * 2;
     pdl_wait();
     by_prime(m, [&](auto f) {
-        const auto d0 = f.minus(f.value(g[from]), f.value(mean[of])), d1 = f.minus(f.value(g[from + poly]), f.value(mean[of + poly])), kl = f.value(K.v[l]);
-        const auto x0 = f.negative(f.value(xhat[from])), x1 = f.negative(f.value(xhat[from + poly])), a0 = f.value(dot[of]), a1 = f.value(dot[of + poly]);
-        typename decltype(f)::Sum s[3];
-        for (auto &e : s) e.zero();
-        s[0].mac(d0, kl); s[0].mac(x0, a0);
-        s[1].mac(d1, kl); s[1].mac(x0, a1); s[1].mac(x1, a0);
-        s[2].mac(x1, a1);
-        u64 *o = out + (size_t)k * 3 * poly + at;
-        for (int e = 0; e < 3; ++e) o[e * poly] = s[e].canonical(m);
+        using V = typename decltype(f)::Value;
+        V m0[2], m1[2], a0[2], a1[2];
+        auto pair = [&](const u64 *p, V (&v0)[2], V (&v1)[2]) {
+            Pair y;
+            y.load(p, poly, at);
+            y.values(f, v0, v1);
+        };
+        pair(mean + (size_t)c * 2 * poly, m0, m1);
+        pair(dot + (size_t)c * 2 * poly, a0, a1);
+        const V k = f.value(K.v[l]);
+#pragma unroll 1
+        for (int t = first; t < last; ++t) {
+            const int i = t * w.step + c;
+            V g0[2], g1[2], x0[2], x1[2];
+            pair(g + (size_t)i * 2 * poly, g0, g1);
+            pair(xhat + (size_t)i * 2 * poly, x0, x1);
+            Two d[3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const V n0 = f.negative(x0[e]), n1 = f.negative(x1[e]);
+                typename decltype(f)::Sum s[3];
+                s[0].zero(); s[1].zero(); s[2].zero();
+                s[0].mac(f.minus(g0[e], m0[e]), k); s[0].mac(n0, a0[e]);
+                s[1].mac(f.minus(g1[e], m1[e]), k); s[1].mac(n0, a1[e]); s[1].mac(n1, a0[e]);
+                s[2].mac(n1, a1[e]);
+#pragma unroll
+                for (int j = 0; j < 3; ++j) d[j].v[e] = s[j].canonical(m);
+            }
+            u64 *o = out + (size_t)i * 3 * poly + at;
+#pragma unroll
+            for (int j = 0; j < 3; ++j) store2(o + j * poly, d[j]);
+        }
     });
 }
 
