@@ -148,6 +148,23 @@ class HEMMer {
     // s % tile (member b; s < tile: left half, real part; < 2 tile: right half, real part; < 3 tile: left half, imaginary part; then right half,
     // imaginary part).  One member per vector and column tile: y / 2 is the sum of the real parts of the halves, the same in every row, one level lower.
     CtxtTensor vecMatMul4(const CtxtTensor &x, const hb_qweight *w);
+    // Layer norm over rows that reach across the column tiles of x (members [column tile][token tile]; `columns` of them in all, the last tile may end early, with zeros behind): with mean and variance of
+    // a row, xhat = (x - mean) rstd and y = xhat gamma + beta (NULL: ones, zeros).  rstd is a polynomial of `degree` for 1 / sqrt(variance + eps), right where that lies in [lo, hi] (rows of padding
+    // have a variance of their own and come out as some finite multiple of zero, plus beta).  Takes 4 + polynomialDepth(degree) levels, one more with gamma or a tile that ends early; xhat and rstd are
+    // what the gradients need, one and two levels above y.
+    struct LayerNorm { CtxtTensor y, xhat, rstd; };
+    LayerNorm layerNorm(const CtxtTensor &x, int groups, i64 columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree);
+    // Its gradients: dx, and dgamma and dbeta summed over all rows and token tiles (one member per column tile, the same in every row).
+    struct LayerNormGrads { CtxtTensor dx, dgamma, dbeta; };
+    LayerNormGrads layerNormBackward(const CtxtTensor &dy, const CtxtTensor &xhat, const CtxtTensor &rstd, int groups, i64 columns, const double *gamma);
+    // The square of the norm over all slots of all members of all gradients, in every slot; and the gradients times min(1, max_norm / norm), a polynomial of `degree` in the square, right up to a
+    // norm of `bound`.  Takes 3 + polynomialDepth(degree) levels of the lowest gradient.
+    Ciphertext gradNormSquared(const std::vector<const Ciphertext *> &grads);
+    std::vector<Ciphertext> clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared = nullptr);
+    // their polynomials, as coefficients of T_j(u) with u the place of the argument in [-1, 1]: 1 / sqrt over [lo, hi], min(1, max_norm / sqrt) over [0, bound^2]
+    static std::vector<double> inverseRootPolynomial(double lo, double hi, int degree);
+    static std::vector<double> clipPolynomial(double max_norm, double bound, int degree);
+    static int polynomialDepth(int degree); // levels of their evaluation
     CtxtTensor packedMatMul(const CtxtTensor &a, const CtxtTensor &b, int target_level = 4);
     CtxtTensor packedMatMulPre(const CtxtTensor &a, int target_level = 4);
     Ciphertext packedMatMulPreRot(const CtxtTensor &a, int target_level = 4);

@@ -315,6 +315,48 @@ class Evaluator {
     }
     // encrypted vectors times a matrix in 4 bits, un-rescaled
     Ciphertext matvec4(const Ciphertext &x, const hb_qweight *w, int tile) const { hb_ct *o = nullptr; check(c_, hb_matvec_q4(c_, x.raw(), w, tile, &o)); return Ciphertext(c_, o); }
+    // normalisation (hb_norm_*): members are [column tile][token tile]; what has three polynomials or a factor comes back un-relinearised and un-rescaled
+    Ciphertext normSquares(const Ciphertext &x, const Ciphertext *mean, int groups, int pad) const {
+        hb_ct *o = nullptr; check(c_, hb_norm_squares(c_, x.raw(), mean ? mean->raw() : nullptr, groups, pad, &o)); return Ciphertext(c_, o);
+    }
+    Ciphertext normScale(const Ciphertext &x, const Ciphertext *mean, const Ciphertext &factor, int groups) const {
+        hb_ct *o = nullptr; check(c_, hb_norm_scale(c_, x.raw(), mean ? mean->raw() : nullptr, factor.raw(), groups, &o)); return Ciphertext(c_, o);
+    }
+    // one factor, one addend or both per column tile; those that are absent are an empty list
+    Ciphertext normAffine(const Ciphertext &x, const std::vector<const Plaintext *> &gamma, const std::vector<const Plaintext *> &beta) const {
+        if (!gamma.empty() && !beta.empty() && gamma.size() != beta.size()) throw std::invalid_argument("[normAffine] factors and addends of another number");
+        std::vector<const hb_pt *> g, b;
+        for (auto *p : gamma) g.push_back(p->raw());
+        for (auto *p : beta) b.push_back(p->raw());
+        hb_ct *o = nullptr;
+        check(c_, hb_norm_affine(c_, x.raw(), g.empty() ? nullptr : g.data(), b.empty() ? nullptr : b.data(), (int)std::max(g.size(), b.size()), &o));
+        return Ciphertext(c_, o);
+    }
+    struct GradSums { Ciphertext rows, rowsum, cols, colsum; };
+    GradSums normGradSums(const Ciphertext &dy, const Ciphertext *g, const Ciphertext &xhat, int groups) const {
+        hb_ct *o[4] = {};
+        check(c_, hb_norm_grad_sums(c_, dy.raw(), g ? g->raw() : nullptr, xhat.raw(), groups, &o[0], &o[1], &o[2], &o[3]));
+        return {Ciphertext(c_, o[0]), Ciphertext(c_, o[1]), Ciphertext(c_, o[2]), Ciphertext(c_, o[3])};
+    }
+    Ciphertext normGradInput(const Ciphertext &g, const Ciphertext &mean, const Ciphertext &xhat, const Ciphertext &dot, int groups) const {
+        hb_ct *o = nullptr; check(c_, hb_norm_grad_input(c_, g.raw(), mean.raw(), xhat.raw(), dot.raw(), groups, &o)); return Ciphertext(c_, o);
+    }
+    // the sum of x (x) x over all members of all handles; every one of them times one factor
+    Ciphertext squareSumMany(const std::vector<Ciphertext> &v) const {
+        std::vector<const hb_ct *> raw;
+        for (const auto &x : v) raw.push_back(x.raw());
+        hb_ct *o = nullptr; check(c_, hb_square_sum_many(c_, raw.data(), (int)raw.size(), &o)); return Ciphertext(c_, o);
+    }
+    std::vector<Ciphertext> scaleMany(const std::vector<Ciphertext> &v, const Ciphertext &factor) const {
+        std::vector<const hb_ct *> raw;
+        for (const auto &x : v) raw.push_back(x.raw());
+        std::vector<hb_ct *> o(v.size(), nullptr);
+        check(c_, hb_scale_many(c_, raw.data(), (int)raw.size(), factor.raw(), o.data()));
+        std::vector<Ciphertext> r;
+        for (hb_ct *p : o) r.emplace_back(c_, p);
+        return r;
+    }
+    Ciphertext slice(const Ciphertext &x, int start, int count) const { hb_ct *o = nullptr; check(c_, hb_batch_slice(c_, x.raw(), start, count, &o)); return Ciphertext(c_, o); }
     Ciphertext stack(const std::vector<Ciphertext> &v) const {
         int level = 0, np = 0, sp = 0, b = 1; hb_ct_meta(v[0].raw(), &level, &np, &b, &sp);
         hb_ct *o = nullptr; check(c_, hb_ct_create(c_, level, np, (int)v.size() * b, sp, &o)); // copy k of input j at k*b + j

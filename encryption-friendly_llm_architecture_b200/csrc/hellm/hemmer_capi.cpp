@@ -236,6 +236,65 @@ int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct
         *out = h->h.vecMatMul4(view(bx, d, d, 2 * d), w).get().release();
     });
 }
+int hb_hemmer_layer_norm(hb_hemmer *h, const hb_ct *x, SHAPE_ARGS, int groups, int columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree,
+                         hb_ct **y, hb_ct **xhat, hb_ct **rstd) {
+    return guard([&] {
+        if (!x || !y || !xhat || !rstd) throw std::invalid_argument("[layerNorm] null argument");
+        IN_TENSOR(t, x);
+        HEMMer::LayerNorm r = h->h.layerNorm(t, groups, columns, gamma, beta, eps, lo, hi, degree);
+        *y = r.y.get().release(); *xhat = r.xhat.get().release(); *rstd = r.rstd.get().release();
+    });
+}
+int hb_hemmer_layer_norm_backward(hb_hemmer *h, const hb_ct *dy, const hb_ct *xhat, const hb_ct *rstd, SHAPE_ARGS, int groups, int columns, const double *gamma, hb_ct **dx, hb_ct **dgamma,
+                                  hb_ct **dbeta) {
+    return guard([&] {
+        if (!dy || !xhat || !rstd || !dx || !dgamma || !dbeta) throw std::invalid_argument("[layerNormBackward] null argument");
+        Borrow bd(h->ctx, dy), bx(h->ctx, xhat), br(h->ctx, rstd);
+        const TileTensorShape s(rows, cols, width);
+        CtxtTensor td(s, h->h.eval().view(bd.c, 0, bd.c.getBatch())), tx(s, h->h.eval().view(bx.c, 0, bx.c.getBatch())), tr(s, h->h.eval().view(br.c, 0, br.c.getBatch()));
+        HEMMer::LayerNormGrads r = h->h.layerNormBackward(td, tx, tr, groups, columns, gamma);
+        *dx = r.dx.get().release(); *dgamma = r.dgamma.get().release(); *dbeta = r.dbeta.get().release();
+    });
+}
+namespace {
+struct BorrowList {
+    std::vector<std::unique_ptr<Borrow>> hold;
+    std::vector<const Ciphertext *> p;
+    BorrowList(hb_ctx *ctx, const hb_ct *const *v, int count, const char *what) {
+        if (!v || count < 1) throw std::invalid_argument(std::string("[") + what + "] no gradients");
+        for (int i = 0; i < count; ++i) {
+            if (!v[i]) throw std::invalid_argument(std::string("[") + what + "] null argument");
+            hold.emplace_back(new Borrow(ctx, v[i]));
+            p.push_back(&hold.back()->c);
+        }
+    }
+};
+}
+int hb_hemmer_grad_norm_squared(hb_hemmer *h, const hb_ct *const *grads, int count, hb_ct **out) {
+    return guard([&] {
+        if (!out) throw std::invalid_argument("[gradNormSquared] null argument");
+        BorrowList g(h->ctx, grads, count, "gradNormSquared");
+        *out = h->h.gradNormSquared(g.p).release();
+    });
+}
+int hb_hemmer_clip_grad_norm(hb_hemmer *h, const hb_ct *const *grads, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared) {
+    return guard([&] {
+        if (!outs) throw std::invalid_argument("[clipGradNorm] null argument");
+        BorrowList g(h->ctx, grads, count, "clipGradNorm");
+        Ciphertext square;
+        std::vector<Ciphertext> r = h->h.clipGradNorm(g.p, max_norm, bound, degree, &square);
+        for (size_t k = 0; k < r.size(); ++k) outs[k] = r[k].release();
+        if (norm_squared) *norm_squared = square.release();
+    });
+}
+int hb_hemmer_polynomial(int which, double a, double b, int degree, double *coefficients, int *depth) {
+    return guard([&] {
+        if (which < 0 || which > 1 || !coefficients) throw std::invalid_argument("[polynomial] which of two, and room for its coefficients");
+        const std::vector<double> c = which ? HEMMer::clipPolynomial(a, b, degree) : HEMMer::inverseRootPolynomial(a, b, degree);
+        std::copy(c.begin(), c.end(), coefficients);
+        if (depth) *depth = HEMMer::polynomialDepth(degree);
+    });
+}
 int hb_hemmer_packed_matmul(hb_hemmer *h, const hb_ct *a, int ra, int ca, int wa, const hb_ct *b, int rb, int cb, int wb, int target, hb_ct **out) {
     return guard([&] {
         Borrow ba(h->ctx, a), bb(h->ctx, b);

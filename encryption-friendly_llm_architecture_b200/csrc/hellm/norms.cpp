@@ -1,0 +1,301 @@
+// Layer norm, its gradients, and the clipping of gradients by their global norm, on ciphertexts.  The sums, products and gradients are hb_norm_*, hb_square_sum_many and
+// hb_scale_many; what stands between them (relinearisation, sums over slots by rotations, polynomials of the inverse root) is put together here.
+#include "HEMMer.hpp"
+#include "schedules.hpp"
+
+#include <cmath>
+#include <cstring>
+
+namespace HELLM {
+
+namespace {
+enum NormMask { kFirstColScaled = 0, kConstant = 1, kColumns = 2 };
+constexpr double kPi = 3.14159265358979323846264338327950288;
+
+// a column tile of `columns` values in every row, zeros behind them
+Plaintext columns_plaintext(const HEMMer &h, const TileTensorShape &s, const double *v, i64 columns, int level) {
+    const i64 w = s.getBlockWidth();
+    Message m((size_t)h.slots());
+    for (i64 r = 0; r < s.getNumRows(); ++r)
+        for (i64 c = 0; c < columns; ++c) m.re[(size_t)(r * w + c)] = v ? v[c] : 1.0;
+    return h.eval().encode(m, level);
+}
+// plaintexts that depend on a number: the number's bits are part of their key
+const Plaintext &norm_mask(HEMMer &h, NormMask which, const TileTensorShape &s, double value, int level) {
+    i64 bits;
+    std::memcpy(&bits, &value, 8);
+    const MaskCache::Key k{sched::kNorm + (int)which, s, bits, level};
+    if (const Plaintext *p = h.masks().find(k)) return *p;
+    if (which == kColumns) return h.masks().put(k, columns_plaintext(h, s, nullptr, (i64)value, level));
+    Message m((size_t)h.slots());
+    if (which == kConstant) std::fill(m.re.begin(), m.re.end(), value);
+    else for (i64 r = 0; r < s.getNumRows(); ++r) m.re[(size_t)(r * s.getBlockWidth())] = value;
+    return h.masks().put(k, h.eval().encode(m, level));
+}
+const Plaintext &constant(HEMMer &h, double v, int level) { return norm_mask(h, kConstant, TileTensorShape(), v, level); }
+Ciphertext add_constant(HEMMer &h, const Ciphertext &x, double v) { return h.eval().normAffine(x, {}, {&constant(h, v, x.getLevel())}); }
+Ciphertext switched(const Evaluator &ev, const Ciphertext &x) { return ev.rescale(ev.relinearize(x)); }
+// x at a lower level, or a view of x, which has to outlive it; a temporary is moved
+Ciphertext down(const Evaluator &ev, const Ciphertext &x, int level) { return x.getLevel() == level ? ev.view(x, 0, x.getBatch()) : ev.levelDown(x, level); }
+Ciphertext down(const Evaluator &ev, Ciphertext &&x, int level) { return x.getLevel() == level ? std::move(x) : ev.levelDown(x, level); }
+
+// `scale` times the sum over a row (and `other` times the first column of y), in all its columns; one level
+Ciphertext row_mean(HEMMer &h, Ciphertext x, const TileTensorShape &s, double scale, const Ciphertext *y = nullptr, double other = 0.0) {
+    const Evaluator &ev = h.eval();
+    for (i64 i = 1; i < s.getBlockWidth(); i <<= 1) x = ev.add(x, ev.leftRotate(x, i));
+    const Plaintext &mask = norm_mask(h, kFirstColScaled, s, scale, x.getLevel());
+    x = y ? ev.multSumRescaledOnce({&x, y}, {&mask, &norm_mask(h, kFirstColScaled, s, other, x.getLevel())}) : ev.mult(x, mask);
+    for (i64 i = 1; i < s.getBlockWidth(); i <<= 1) x = ev.add(x, ev.rightRotate(x, i));
+    return x;
+}
+// the sum over all slots that are a multiple of `step` apart, in each of them
+Ciphertext sum_slots(const HEMMer &h, Ciphertext x, i64 step) {
+    for (i64 i = step; i < h.slots(); i <<= 1) x = h.eval().add(x, h.eval().leftRotate(x, i));
+    return x;
+}
+
+struct NormShape { TileTensorShape s; int groups, batch; i64 columns, pad; };
+NormShape norm_shape(const HEMMer &h, const CtxtTensor &x, int groups, i64 columns, const char *what) {
+    const std::string name = std::string("[") + what + "] ";
+    const i64 w = x.getBlockWidth(), rows = x.getHeight();
+    if (w < 1 || (w & (w - 1)) || rows < 1 || rows > h.slots() / w || rows * w != h.slots()) throw std::invalid_argument(name + "rows of a power of two that fill the slots");
+    if (groups < 1 || x.get().getBatch() % groups) throw std::invalid_argument(name + "the batch does not split into that many column tiles");
+    if (columns <= (groups - 1) * w || columns > groups * w) throw std::invalid_argument(name + "columns end in the last tile");
+    return {x.getShape(), groups, x.get().getBatch() / groups, columns, groups * w - columns};
+}
+void need_level(int level, int least, const char *what) {
+    if (level < least) throw std::invalid_argument(std::string("[") + what + "] level too low: " + std::to_string(level) + " of " + std::to_string(least));
+}
+// plaintexts of the column tiles: values (NULL: ones) of the first `columns`, zeros behind them
+std::vector<Plaintext> column_plaintexts(HEMMer &h, const NormShape &n, const double *v, int level) {
+    const i64 w = n.s.getBlockWidth();
+    std::vector<Plaintext> p;
+    for (i64 t = 0; t < n.groups; ++t) {
+        const i64 here = std::min(w, n.columns - t * w);
+        p.push_back(v ? columns_plaintext(h, n.s, v + t * w, here, level) : norm_mask(h, kColumns, n.s, (double)here, level));
+    }
+    return p;
+}
+std::vector<const Plaintext *> pointers(const std::vector<Plaintext> &p) {
+    std::vector<const Plaintext *> r;
+    for (const Plaintext &x : p) r.push_back(&x);
+    return r;
+}
+
+// ---- polynomials in Chebyshev form ----
+// Coefficients of the interpolation of f over [lo, hi] at the n + 1 Chebyshev points: f(x) ~ sum_j c[j] T_j(u), u the place of x in [-1, 1].
+template <class F> std::vector<double> chebyshev(F &&f, double lo, double hi, int n) {
+    std::vector<double> y((size_t)n + 1), c((size_t)n + 1);
+    for (int k = 0; k <= n; ++k) y[(size_t)k] = f(0.5 * (hi + lo) + 0.5 * (hi - lo) * std::cos(kPi * (k + 0.5) / (n + 1)));
+    for (int j = 0; j <= n; ++j) {
+        double s = 0.0;
+        for (int k = 0; k <= n; ++k) s += y[(size_t)k] * std::cos(kPi * j * (k + 0.5) / (n + 1));
+        c[(size_t)j] = s * (j ? 2.0 : 1.0) / (n + 1);
+    }
+    return c;
+}
+int log2_floor(int n) { int l = 0; while (n >> (l + 1)) ++l; return l; }
+// levels of the evaluation below
+int chebyshev_depth(int n) {
+    if (n <= 3) return n;
+    const int m = log2_floor(n), q = n - (1 << m);
+    return std::max(std::max(m, q ? chebyshev_depth(q) : 0) + 1, chebyshev_depth((1 << m) - 1));
+}
+// T_m for m = 1, 2, 3 and the powers of two, from T_2a = 2 T_a^2 - 1 and T_3 = 2 T_1 T_2 - T_1; and sums of them: a polynomial of degree n is q T_m + r for the largest power of two m <= n, with
+// q_j = 2 c_{m+j} (q_0 = c_m) and r_{m-j} = c_{m-j} - c_{m+j}, since T_m T_j = (T_{m+j} + T_{m-j}) / 2.  Constants are added last.
+struct Chebyshev {
+    HEMMer &h;
+    const Evaluator &ev;
+    std::vector<Ciphertext> t; // t[m]
+    Chebyshev(HEMMer &h_, const Ciphertext &u, int n) : h(h_), ev(h_.eval()), t((size_t)std::max(n, 3) + 1) {
+        t[1] = ev.view(u, 0, u.getBatch());
+        for (int m = 2; m <= n; m <<= 1) {
+            const Ciphertext s = ev.square(t[(size_t)m / 2]);
+            t[(size_t)m] = add_constant(h, ev.add(s, s), -1.0);
+        }
+        if (n >= 3) {
+            const Ciphertext s = ev.mult(t[1], t[2]);
+            t[3] = ev.sub(ev.add(s, s), t[1]);
+        }
+    }
+    struct Sum { Ciphertext x; double c = 0.0; }; // x + c; no x: c alone
+    Ciphertext whole(Sum &&s) const { return s.c == 0.0 ? std::move(s.x) : add_constant(h, s.x, s.c); }
+    Sum eval(std::vector<double> c) const {
+        while (c.size() > 1 && c.back() == 0.0) c.pop_back();
+        const int n = (int)c.size() - 1;
+        Sum r;
+        r.c = c[0];
+        if (n == 0) return r;
+        if (n <= 3) {
+            const int level = t[(size_t)n].getLevel();
+            std::vector<Ciphertext> x;
+            std::vector<const Ciphertext *> px;
+            std::vector<const Plaintext *> pc;
+            for (int j = 1; j <= n; ++j) {
+                if (c[(size_t)j] == 0.0) continue;
+                x.push_back(down(ev, t[(size_t)j], level));
+                pc.push_back(&constant(h, c[(size_t)j], level));
+            }
+            for (const Ciphertext &y : x) px.push_back(&y);
+            r.x = ev.multSumRescaledOnce(px, pc);
+            return r;
+        }
+        const int m = 1 << log2_floor(n);
+        std::vector<double> q(c.begin() + m, c.end()), rest(c.begin(), c.begin() + m);
+        for (int j = 1; j <= n - m; ++j) { rest[(size_t)(m - j)] -= q[(size_t)j]; q[(size_t)j] *= 2.0; }
+        Sum high = eval(q), low = eval(rest);
+        const Ciphertext &tm = t[(size_t)m];
+        r.x = high.x.empty() ? ev.mult(tm, constant(h, high.c, tm.getLevel())) : ev.mult(whole(std::move(high)), tm);
+        if (!low.x.empty()) r.x = ev.add(r.x, low.x);
+        r.c = low.c;
+        return r;
+    }
+};
+Ciphertext evaluate(HEMMer &h, const Ciphertext &u, const std::vector<double> &c) {
+    const Chebyshev t(h, u, (int)c.size() - 1);
+    auto s = t.eval(c);
+    if (s.x.empty()) throw std::invalid_argument("[chebyshev] a constant");
+    return t.whole(std::move(s));
+}
+void need_degree(int degree, const char *what) { if (degree < 1 || degree > 63) throw std::invalid_argument(std::string("[") + what + "] polynomials have a degree from 1 to 63"); }
+bool positive(double x) { return x > 0.0 && std::isfinite(x); }
+} // namespace
+
+std::vector<double> HEMMer::inverseRootPolynomial(double lo, double hi, int degree) {
+    need_degree(degree, "layerNorm");
+    if (!positive(lo) || !std::isfinite(hi) || !(hi > lo)) throw std::invalid_argument("[layerNorm] a range of positive variances");
+    return chebyshev([](double x) { return 1.0 / std::sqrt(x); }, lo, hi, degree);
+}
+std::vector<double> HEMMer::clipPolynomial(double max_norm, double bound, int degree) {
+    need_degree(degree, "clipGradNorm");
+    if (!positive(max_norm) || !positive(bound) || !std::isfinite(bound * bound) || !(bound * bound > 0.0)) throw std::invalid_argument("[clipGradNorm] norms are positive");
+    if (!(bound > max_norm)) throw std::invalid_argument("[clipGradNorm] nothing to clip: the bound is not above the norm");
+    return chebyshev([&](double s) { return s > max_norm * max_norm ? max_norm / std::sqrt(s) : 1.0; }, 0.0, bound * bound, degree);
+}
+int HEMMer::polynomialDepth(int degree) { return chebyshev_depth(degree); }
+
+HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree) {
+    const NormShape n = norm_shape(*this, x, groups, columns, "layerNorm");
+    const std::vector<double> c = inverseRootPolynomial(lo, hi, degree);
+    if (!(eps >= 0.0) || !std::isfinite(eps)) throw std::invalid_argument("[layerNorm] eps from 0");
+    for (const double *v : {gamma, beta})
+        for (i64 k = 0; v && k < columns; ++k) if (!std::isfinite(v[k])) throw std::invalid_argument("[layerNorm] a weight is not finite");
+    const bool scaled = gamma || n.pad; // columns past the width come out as zeros
+    need_level(x.getLevel(), 4 + polynomialDepth(degree) + (scaled ? 1 : 0), "layerNorm");
+    const Evaluator &ev = eval_;
+    const Ciphertext mean = row_mean(*this, ev.sumGroups(x.get(), groups), n.s, 1.0 / (double)columns);
+    Ciphertext u;
+    {
+        const double scale = 2.0 / ((hi - lo) * (double)columns);
+        Ciphertext squares = ev.normSquares(down(ev, x.get(), mean.getLevel()), &mean, groups, 0), row;
+        if (n.pad) { // columns past the width hold zeros, whose differences are the mean: their squares are taken off the sum over the row
+            std::vector<Ciphertext> both;
+            both.push_back(std::move(squares)); both.push_back(ev.normSquares(mean, nullptr, 1, 0));
+            const Ciphertext s = switched(ev, ev.concat(both)), of_mean = ev.group(s, 1, 2);
+            row = row_mean(*this, ev.group(s, 0, 2), n.s, scale, &of_mean, -scale * (double)n.pad);
+        } else row = row_mean(*this, switched(ev, squares), n.s, scale);
+        u = add_constant(*this, row, (2.0 * eps - hi - lo) / (hi - lo)); // the variance's place in [-1, 1]
+    }
+    Ciphertext rstd = evaluate(*this, u, c);
+    const int level = rstd.getLevel();
+    const Ciphertext low_mean = down(ev, mean, level);
+    Ciphertext xhat = switched(ev, ev.normScale(down(ev, x.get(), level), &low_mean, rstd, groups));
+    Ciphertext y;
+    if (scaled) {
+        const std::vector<Plaintext> g = column_plaintexts(*this, n, gamma, level - 1), b = beta ? column_plaintexts(*this, n, beta, level - 1) : std::vector<Plaintext>();
+        y = ev.rescale(ev.normAffine(xhat, pointers(g), pointers(b)));
+    } else if (beta) {
+        const std::vector<Plaintext> b = column_plaintexts(*this, n, beta, level - 1);
+        y = ev.normAffine(xhat, {}, pointers(b));
+    } else y = xhat;
+    return {CtxtTensor(n.s, std::move(y)), CtxtTensor(n.s, std::move(xhat)), CtxtTensor(n.s, std::move(rstd))};
+}
+
+HEMMer::LayerNormGrads HEMMer::layerNormBackward(const CtxtTensor &dy, const CtxtTensor &xhat, const CtxtTensor &rstd, int groups, i64 columns, const double *gamma) {
+    const NormShape n = norm_shape(*this, dy, groups, columns, "layerNormBackward");
+    const Evaluator &ev = eval_;
+    if (xhat.get().getBatch() != dy.get().getBatch() || rstd.get().getBatch() != n.batch) throw std::invalid_argument("[layerNormBackward] batches differ");
+    for (i64 k = 0; gamma && k < columns; ++k) if (!std::isfinite(gamma[k])) throw std::invalid_argument("[layerNormBackward] a weight is not finite");
+    const bool scaled = gamma || n.pad;
+    const int level = std::min(dy.getLevel() - (scaled ? 1 : 0), xhat.getLevel());
+    need_level(std::min(level - 3, rstd.getLevel()), n.pad ? 2 : 1, "layerNormBackward");
+    Ciphertext g;
+    if (scaled) {
+        const std::vector<Plaintext> p = column_plaintexts(*this, n, gamma, dy.getLevel());
+        g = down(ev, ev.rescale(ev.normAffine(dy.get(), pointers(p), {})), level);
+    }
+    const Ciphertext low_dy = down(ev, dy.get(), level), low_xhat = down(ev, xhat.get(), level);
+    Evaluator::GradSums s = ev.normGradSums(low_dy, scaled ? &g : nullptr, low_xhat, groups);
+    LayerNormGrads out;
+    const i64 w = n.s.getBlockWidth();
+    out.dgamma = CtxtTensor(n.s, sum_slots(*this, switched(ev, s.cols), w));
+    out.dbeta = CtxtTensor(n.s, sum_slots(*this, s.colsum, w));
+    const Ciphertext dot = row_mean(*this, switched(ev, s.rows), n.s, 1.0 / (double)columns);
+    const Ciphertext mean = down(ev, row_mean(*this, std::move(s.rowsum), n.s, 1.0 / (double)columns), dot.getLevel());
+    const Ciphertext &gl = scaled ? static_cast<const Ciphertext &>(g) : low_dy;
+    const Ciphertext g2 = down(ev, gl, dot.getLevel()), x2 = down(ev, low_xhat, dot.getLevel());
+    const Ciphertext inner = switched(ev, ev.normGradInput(g2, mean, x2, dot, groups));
+    const int last = std::min(inner.getLevel(), rstd.getLevel());
+    const Ciphertext factor = down(ev, rstd.get(), last);
+    Ciphertext dx = switched(ev, ev.normScale(down(ev, inner, last), nullptr, factor, groups));
+    if (n.pad) {
+        const std::vector<Plaintext> ones = column_plaintexts(*this, n, nullptr, dx.getLevel());
+        dx = ev.rescale(ev.normAffine(dx, pointers(ones), {}));
+    }
+    out.dx = CtxtTensor(n.s, std::move(dx));
+    return out;
+}
+
+namespace {
+// all of the lowest level among them
+std::vector<Ciphertext> same_level(const Evaluator &ev, const std::vector<const Ciphertext *> &v) {
+    int level = v[0]->getLevel();
+    for (const Ciphertext *x : v) level = std::min(level, x->getLevel());
+    std::vector<Ciphertext> r;
+    for (const Ciphertext *x : v) r.push_back(down(ev, *x, level));
+    return r;
+}
+}
+
+Ciphertext HEMMer::gradNormSquared(const std::vector<const Ciphertext *> &grads) {
+    if (grads.empty()) throw std::invalid_argument("[gradNormSquared] no gradients");
+    const std::vector<Ciphertext> g = same_level(eval_, grads);
+    need_level(g[0].getLevel(), 1, "gradNormSquared");
+    return sum_slots(*this, switched(eval_, eval_.squareSumMany(g)), 1);
+}
+
+std::vector<Ciphertext> HEMMer::clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared) {
+    const std::vector<double> c = clipPolynomial(max_norm, bound, degree);
+    if (grads.empty()) throw std::invalid_argument("[clipGradNorm] no gradients");
+    int level = grads[0]->getLevel();
+    for (const Ciphertext *x : grads) level = std::min(level, x->getLevel());
+    need_level(level, 3 + polynomialDepth(degree), "clipGradNorm");
+    const Evaluator &ev = eval_;
+    Ciphertext square = gradNormSquared(grads);
+    const Ciphertext u = add_constant(*this, ev.mult(square, constant(*this, 2.0 / (bound * bound), square.getLevel())), -1.0);
+    const Ciphertext factor = evaluate(*this, u, c);
+    std::vector<Ciphertext> low;
+    for (const Ciphertext *x : grads) low.push_back(down(ev, *x, factor.getLevel()));
+    std::vector<Ciphertext> products = ev.scaleMany(low, factor), out;
+    low.clear();
+    // small handles share the launches of their key switches, up to kTogether members
+    constexpr int kTogether = 24;
+    for (size_t k = 0; k < products.size();) {
+        size_t end = k;
+        int members = 0;
+        while (end < products.size() && (end == k || members + products[end].getBatch() <= kTogether)) members += products[end++].getBatch();
+        if (end == k + 1) out.push_back(switched(ev, products[k]));
+        else {
+            std::vector<Ciphertext> part;
+            for (size_t i = k; i < end; ++i) part.push_back(ev.view(products[i], 0, products[i].getBatch()));
+            const Ciphertext all = switched(ev, ev.concat(part));
+            int at = 0;
+            for (size_t i = k; i < end; ++i) { out.push_back(ev.slice(all, at, products[i].getBatch())); at += products[i].getBatch(); }
+        }
+        k = end;
+    }
+    if (norm_squared) *norm_squared = std::move(square);
+    return out;
+}
+
+} // namespace HELLM

@@ -1150,7 +1150,7 @@ hb_ct *do_norm_squares(hb_ctx *c, const hb_ct *x, const hb_ct *mean, int groups,
     norm_operand(c, x, x, "norm_squares");
     const int batch = norm_batch(x, groups, "norm_squares"), n = x->level + 1, N = c->N;
     if (mean) norm_shared(c, mean, x, batch, "norm_squares");
-    if (pad < 0 || pad > c->h->slots || (pad && !mean)) fail(HB_E_ARG, "norm_squares: columns past the width are counted from 0 to the slots, and only beside a mean");
+    if (pad < 0 || pad > c->h->slots || (pad && !mean)) fail(HB_E_ARG, "norm_squares: members of padding are counted from 0 to the slots, and only beside a mean");
     const int log_splits = norm_log_splits(groups, (long)(N / kNormLanes) * batch * n), chunk = norm_chunk(batch, (long)(N / kNormLanes << log_splits) * n, 1);
     const dim3 grid((unsigned)(N / kNormLanes << log_splits), (unsigned)n, (unsigned)((batch + chunk - 1) / chunk));
     hb_ct *r = new_ct(c, x->level, 3, batch, 2);

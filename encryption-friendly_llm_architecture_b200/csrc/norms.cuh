@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256, U == 1 ? 3 : 2) k_square_sums(u64 *out, c
             for (int k = 0; k < 3; ++k)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) r[k].v[e] = s[k][e].canonical(m);
-            if (MEAN && w.pad && part == 0) { // less the squares of the columns past the width
+            if (MEAN && w.pad && part == 0) { // less what members of padding have added
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     s[0][e].zero(); s[1][e].zero(); s[2][e].zero();

@@ -373,6 +373,52 @@ class Hemmer:
         z = self.lib.decrypt_many([(y.ct, k) for k in range(members)])[:, : 2 * d].real
         return (2.0 * (z[:, :d] + z[:, d:])).reshape(members // nb, nb * d)[:, :cols]
 
+    # ---- normalisation ----
+    def _columns(self, v, columns):
+        if v is None:
+            return None, None
+        a = np.ascontiguousarray(v, dtype=np.float64)
+        if a.shape != (columns,):
+            raise ValueError(f"{columns} columns, weights {a.shape}")
+        return a, a.ctypes.data_as(C.POINTER(C.c_double))
+
+    def polynomial(self, which, a, b, degree):
+        """(coefficients of T_j, levels) of "rsqrt" over [a, b] or "clip", min(1, a / sqrt) over [0, b^2], as layer_norm and clip_grad_norm evaluate them."""
+        out, depth = np.zeros(max(0, int(degree)) + 1), C.c_int()
+        rc = self._fn("polynomial")(C.c_int({"rsqrt": 0, "clip": 1}[which]), C.c_double(a), C.c_double(b), _i32(degree), out.ctypes.data_as(C.POINTER(C.c_double)), C.byref(depth))
+        if rc != 0:
+            f = self._fn("last_error")
+            f.restype = C.c_char_p
+            raise HBError(rc, f().decode())
+        return out, depth.value
+
+    def layer_norm(self, x, columns, var_range, groups=1, gamma=None, beta=None, eps=1e-5, degree=15):
+        """(y, xhat, rstd) of rows of `columns` values over `groups` column tiles; var_range: where variance + eps lies."""
+        (_g, pg), (_b, pb) = self._columns(gamma, columns), self._columns(beta, columns)
+        outs = self._call("layer_norm", x.ct.ptr, *self._shp(x), _i32(groups), _i32(columns), pg, pb, C.c_double(eps), C.c_double(var_range[0]), C.c_double(var_range[1]), _i32(degree), n_out=3)
+        return tuple(CtxtTensor(o, *x.shape) for o in outs)
+
+    def layer_norm_backward(self, dy, xhat, rstd, columns, groups=1, gamma=None):
+        """(dx, dgamma, dbeta); the gradients of the weights have one member per column tile, the same in every row."""
+        _g, pg = self._columns(gamma, columns)
+        outs = self._call("layer_norm_backward", dy.ct.ptr, xhat.ct.ptr, rstd.ct.ptr, *self._shp(dy), _i32(groups), _i32(columns), pg, n_out=3)
+        return tuple(CtxtTensor(o, *dy.shape) for o in outs)
+
+    def grad_norm_squared(self, grads):
+        """The square of the global norm of all gradients, in every slot."""
+        arr = (C.c_void_p * len(grads))(*[g.ct.ptr.value for g in grads])
+        return self._call("grad_norm_squared", arr, _i32(len(grads)))
+
+    def clip_grad_norm(self, grads, max_norm, bound, degree=15):
+        """(gradients times min(1, max_norm / norm), square of the norm); right up to norms of `bound`."""
+        arr, outs, square = (C.c_void_p * len(grads))(*[g.ct.ptr.value for g in grads]), (C.c_void_p * len(grads))(), C.c_void_p()
+        rc = self._fn("clip_grad_norm")(self.h, arr, _i32(len(grads)), C.c_double(max_norm), C.c_double(bound), _i32(degree), outs, C.byref(square))
+        if rc != 0:
+            f = self._fn("last_error")
+            f.restype = C.c_char_p
+            raise HBError(rc, f().decode())
+        return [CtxtTensor(Handle(self.lib, C.c_void_p(p), "ct"), *g.shape) for p, g in zip(outs, grads)], Handle(self.lib, square, "ct")
+
     def matmul_pre_rev(self, b, target_level=4):
         return CtxtTensor(self._call("matmul_pre_rev", b.ct.ptr, *self._shp(b), C.c_int(target_level)), *b.shape)
 
