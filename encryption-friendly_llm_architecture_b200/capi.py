@@ -7,6 +7,8 @@ module computes anything: every call lands in native code.
 from __future__ import annotations
 
 import ctypes as C
+import functools
+
 import numpy as np
 
 c_u64p = C.POINTER(C.c_uint64)
@@ -55,6 +57,16 @@ def _i32(v):
     return C.c_int32(v)
 
 
+@functools.lru_cache(maxsize=256)
+def _array(n):
+    return C.c_void_p * n
+
+
+def _pointers(handles):
+    """The addresses of a list of handles, as the C entries take them."""
+    return _array(len(handles))(*[h.ptr.value for h in handles])
+
+
 def _f64(a):
     return None if a is None else a.ctypes.data_as(c_f64p)
 
@@ -67,9 +79,7 @@ class Handle:
 
     def __del__(self):
         if getattr(self, "ptr", None) and self.lib is not None and self.lib.alive:
-            f = getattr(self.lib.dll, f"{self.lib.prefix}{self.kind}_free")
-            f.restype = None
-            f(self.ptr)
+            self.lib._free(self.kind)(self.ptr)
             self.ptr = None
 
 
@@ -102,6 +112,15 @@ class Lib:
 
     def _fn(self, name):
         return getattr(self.dll, self.prefix + name)
+
+    def _free(self, kind):
+        """The function that releases a handle of this kind, looked up once."""
+        known = self.__dict__.setdefault("_frees", {})
+        f = known.get(kind)
+        if f is None:
+            f = known[kind] = self._fn(kind + "_free")
+            f.restype = None
+        return f
 
     def has(self, name):
         return hasattr(self.dll, self.prefix + name)
@@ -440,8 +459,7 @@ class Lib:
         for p in (gamma, beta):
             if p is not None and len(p) != groups.value:
                 raise ValueError(f"{groups.value} column tiles, {len(p)} plaintexts")
-        lists = [None if p is None else (C.c_void_p * len(p))(*[q.ptr.value for q in p]) for p in (gamma, beta)]
-        return self._op("norm_affine", x.ptr, *lists, groups)
+        return self._op("norm_affine", x.ptr, None if gamma is None else _pointers(gamma), None if beta is None else _pointers(beta), groups)
 
     def norm_grad_sums(self, dy, xhat, groups, g=None):
         """(rows, rowsum, cols, colsum): tensor sums of g (None: dy) with xhat over the column tiles, of dy with xhat over the token tiles, and plain sums of g and dy."""
@@ -455,13 +473,13 @@ class Lib:
 
     def square_sum_many(self, xs):
         """The sum of tensor(x, x) over all members of all handles: one member, un-relinearised."""
-        return self._op("square_sum_many", (C.c_void_p * len(xs))(*[x.ptr.value for x in xs]), _i32(len(xs)))
+        return self._op("square_sum_many", _pointers(xs), _i32(len(xs)))
 
     def scale_many(self, xs, factor):
         """tensor(x, factor) for all members of all handles, a handle for each; the factor is one member."""
-        outs = (C.c_void_p * len(xs))()
-        self._chk(self._fn("scale_many")(self.ctx, (C.c_void_p * len(xs))(*[x.ptr.value for x in xs]), _i32(len(xs)), factor.ptr, outs))
-        return [Handle(self, C.c_void_p(p), "ct") for p in outs]
+        outs = _array(len(xs))()
+        self._chk(self._fn("scale_many")(self.ctx, _pointers(xs), _i32(len(xs)), factor.ptr, outs))
+        return [Handle(self, C.c_void_p(p), "ct") for p in outs[:]]
 
     def rotate_sum(self, xs, steps):
         """sum_t rot(xs[t], steps[t]) with one ModDown for the whole sum."""

@@ -1151,19 +1151,14 @@ hb_ct *do_norm_squares(hb_ctx *c, const hb_ct *x, const hb_ct *mean, int groups,
     const int batch = norm_batch(x, groups, "norm_squares"), n = x->level + 1, N = c->N;
     if (mean) norm_shared(c, mean, x, batch, "norm_squares");
     if (pad < 0 || pad > c->h->slots || (pad && !mean)) fail(HB_E_ARG, "norm_squares: members of padding are counted from 0 to the slots, and only beside a mean");
-    const int log_splits = norm_log_splits(groups, (long)(N / kNormLanes) * batch * n), chunk = norm_chunk(batch, (long)(N / kNormLanes << log_splits) * n, 1);
+    const int log_splits = norm_log_splits(groups, (long)(N / kNormLanes) * batch * n), chunk = log_splits ? 1 : norm_chunk(batch, (long)(N / kNormLanes) * n, 1);
     const dim3 grid((unsigned)(N / kNormLanes << log_splits), (unsigned)n, (unsigned)((batch + chunk - 1) / chunk));
     hb_ct *r = new_ct(c, x->level, 3, batch, 2);
     try {
         ALG(c, x->limbs() + (mean ? mean->limbs() : 0) + r->limbs());
         const MemberRun run{x->d, (size_t)2 * n * N};
-        auto go = [&](auto *kernel) { launch(c, kernel, grid, 256, 0, r->d, run, mean ? mean->d : nullptr, SquareShape{groups, batch, chunk, log_splits, (u64)pad}, n, c->pc, N, 0); };
-        const int turn = norm_turn((groups + (1 << log_splits) - 1) >> log_splits);
-        if (!mean) go(k_square_sums<MemberRun, false, 4>);
-        else if (turn == 1) go(k_square_sums<MemberRun, true, 1>);
-        else if (turn == 2) go(k_square_sums<MemberRun, true, 2>);
-        else if (turn == 3) go(k_square_sums<MemberRun, true, 3>);
-        else go(k_square_sums<MemberRun, true, 4>);
+        auto go = [&](auto *kernel) { launch(c, kernel, grid, 256, square_smem(), r->d, run, mean ? mean->d : nullptr, SquareShape{groups, batch, chunk, log_splits, (u64)pad}, n, c->pc, N, 0); };
+        if (mean) go(k_square_sums<MemberRun, true>); else go(k_square_sums<MemberRun, false>);
     } catch (...) { hb_ct_free(r); throw; }
     return r;
 }
@@ -1232,7 +1227,7 @@ GradSums do_norm_grad_sums(hb_ctx *c, const hb_ct *dy, const hb_ct *g, const hb_
         for (int t0 = 0; t0 < groups;) {
             const int some = std::min(grad_tiles(groups), groups - t0);
             auto go = [&](auto tiles, auto same) {
-                launch(c, k_grad_sums<decltype(tiles)::value, decltype(same)::value>, dim3((unsigned)(N / 128), (unsigned)n), 128, 0, s.r[0]->d, s.r[1]->d, s.r[2]->d, s.r[3]->d, dy->d, g->d, xhat->d,
+                launch(c, k_grad_sums<decltype(tiles)::value, decltype(same)::value>, dim3((unsigned)(N / 128), (unsigned)n), 128, grad_smem(decltype(tiles)::value, decltype(same)::value), s.r[0]->d, s.r[1]->d, s.r[2]->d, s.r[3]->d, dy->d, g->d, xhat->d,
                        GradShape{batch, t0}, n, c->pc, N);
             };
             auto by_tiles = [&](auto same) {
@@ -1287,7 +1282,7 @@ hb_ct *do_square_sum_many(hb_ctx *c, const hb_ct *const *xs, int count) {
         auto flush = [&] {
             if (!some) return;
             const int log_splits = norm_log_splits(some, (long)(N / kNormLanes) * n);
-            launch(c, k_square_sums<MemberList, false, 4>, dim3((unsigned)(N / kNormLanes << log_splits), (unsigned)n), 256, 0, r->d, list, nullptr, SquareShape{some, 1, 1, log_splits, 0}, n, c->pc, N, first ? 0 : 1);
+            launch(c, k_square_sums<MemberList, false>, dim3((unsigned)(N / kNormLanes << log_splits), (unsigned)n), 256, square_smem(), r->d, list, nullptr, SquareShape{some, 1, 1, log_splits, 0}, n, c->pc, N, first ? 0 : 1);
             some = first = 0;
         };
         for (int k = 0; k < count; ++k)

@@ -156,8 +156,6 @@ constexpr int norm_log_splits(int members, long each) {
     while (log < 3 && (each << log) < 148 * 4 && members >= 4 << log) ++log;
     return log;
 }
-// Members that a sum of `members` multiplies a turn.  Calls at level 5, us, with two, three and four: 5 of 8 token tiles 84 80 -, 6 of 4 48 43 51, 12 of 4 - 69 68.
-constexpr int norm_turn(int members) { return members <= 4 ? members : members == 5 || members == 6 || members == 9 ? 3 : 4; }
 // Column tiles of a launch of the sums in both directions: even launches of at most eight.
 constexpr int grad_tiles(int tiles) {
     const int launches = (tiles + 7) / 8;

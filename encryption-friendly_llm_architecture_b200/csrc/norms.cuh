@@ -110,69 +110,73 @@ struct OutList {
 };
 
 // out[b] (+)= the sum over t < groups, for `chunk` token tiles one after the other.  Threads of a CTA: `splits` parts (a power of two) of the members by 512 / splits residues; the
-// parts are joined in shared memory, in order.  A register that has been multiplied is filled again at once, with the member four further on or the first one of the next token tile.
+// parts, which have a chunk of one, are joined in shared memory, in order.  Words come through a ring of members, which every thread fills for itself: of a token tile the mean first, then the members.
 // grid = (N splits / 512, n, chunks): quotients by sizes would take a fifth of the instructions
 struct SquareShape { int groups, batch, chunk, log_splits; u64 pad; };
-// U members are multiplied a turn; where a part has fewer left, the first turn takes the mean (or zeros) for the ones that are not there, whose squares are nothing: a product behind a
-// branch would make the sums change registers.
-template <class MEMBERS, bool MEAN, int U>
-__global__ void __launch_bounds__(256, U == 1 ? 3 : 2) k_square_sums(u64 *out, const __grid_constant__ MEMBERS x, const u64 *mean, SquareShape w, int n, const PrimeConst *__restrict__ pc, int N,
-                                                                                 int accumulate) {
-    __shared__ __align__(16) u64 parts[2][3][kNormLanes];
+constexpr int kSquareStages = 4;
+constexpr size_t square_smem() { return (size_t)kSquareStages * 2 * kNormLanes * 8; }
+template <class MEMBERS, bool MEAN>
+__global__ void __launch_bounds__(256, 3) k_square_sums(u64 *out, const __grid_constant__ MEMBERS x, const u64 *mean, SquareShape w, int n, const PrimeConst *__restrict__ pc, int N, int accumulate) {
+    constexpr int S = kSquareStages;
+    extern __shared__ __align__(16) u64 words[]; // [S][2][512]; of parts, which have one token tile a CTA, [3][512] in the end
     const int splits = 1 << w.log_splits, wide = 256 >> w.log_splits, lane = threadIdx.x & (wide - 1), part = threadIdx.x >> (8 - w.log_splits);
     const int l = blockIdx.y, first = blockIdx.z * w.chunk, last = min(first + w.chunk, w.batch);
     const PrimeConst m = pc[l];
     const size_t poly = (size_t)n * N;
     const u32 at = (u32)(l * N) + (blockIdx.x * wide + lane) * 2;
-    const int count = (w.groups - part + splits - 1) >> w.log_splits, turns = (count + U - 1) / U, some = count - (turns - 1) * U; // members of this part, those of the first turn
-    Pair v[U], mr{};
-    auto load = [&](int u, int t, int b) { v[u].load(x.at((t + u * splits) * w.batch + b), poly, at); };
+    const int count = (w.groups - part + splits - 1) >> w.log_splits; // members of this part
+    const u32 ring = smem_u32(words + 2 * threadIdx.x);
+    int f_b = first, f_t = MEAN ? -1 : 0, f_stage = 0, stage = 0; // what is fetched next (-1: the mean), and what is read next
+    auto fetch = [&] {
+        if (f_b < last) {
+            const u64 *p = MEAN && f_t < 0 ? mean + (size_t)f_b * 2 * poly : x.at((part + f_t * splits) * w.batch + f_b);
+            const u32 to = ring + f_stage * (2 * kNormLanes * 8);
+            cp_async16(to, p + at); cp_async16(to + kNormLanes * 8, p + poly + at);
+            if (++f_t == count) { f_t = MEAN ? -1 : 0; ++f_b; }
+            if (++f_stage == S) f_stage = 0;
+        }
+        cp_async_commit();
+    };
     pdl_wait();
-    // the first words do not wait for the constants of the prime
-    if (MEAN) mr.load(mean + (size_t)first * 2 * poly, poly, at);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        if (u < some) load(u, part, first);
-        else v[u] = mr;
-    }
+    for (int j = 0; j < S - 1; ++j) fetch();
     by_prime(m, [&](auto f) {
         using V = typename decltype(f)::Value;
         using Sum = typename decltype(f)::Sum;
+        auto next = [&](V (&v0)[2], V (&v1)[2]) {
+            cp_async_wait<S - 2>();
+            const u64 *y = words + stage * (2 * kNormLanes) + 2 * threadIdx.x;
+            const Two a = load2(y), c = load2(y + kNormLanes);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { v0[e] = f.value(a.v[e]); v1[e] = f.value(c.v[e]); }
+            if (++stage == S) stage = 0;
+            fetch(); // into the stage that this thread read a member ago
+        };
 #pragma unroll 1
         for (int b = first; b < last; ++b) {
             Sum s[3][2];
             V m0[2], m1[2];
-            if (MEAN) {
-                mr.values(f, m0, m1);
-                if (b + 1 < last) mr.load(mean + (size_t)(b + 1) * 2 * poly, poly, at);
-            }
+            if (MEAN) next(m0, m1);
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                s[0][e].zero(); s[1][e].zero(); s[2][e].zero();
-            }
-            int t = part + some * splits, held = 0; // the next turn's first member; products of a sum
+            for (int e = 0; e < 2; ++e) { s[0][e].zero(); s[1][e].zero(); s[2][e].zero(); }
+            auto member = [&] {
+                V v0[2], v1[2];
+                next(v0, v1);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    if (MEAN) { v0[e] = f.minus(v0[e], m0[e]); v1[e] = f.minus(v1[e], m1[e]); }
+                    s[0][e].mac(v0[e], v0[e]); s[1][e].mac(v0[e], v1[e]); s[2][e].mac(v1[e], v1[e]);
+                }
+            };
 #pragma unroll 1
-            for (int turn = 0; turn < turns; ++turn) {
-                if ((held += U) > f.room()) {
+            for (int t = 0; t < count; t += f.room()) {
+                if (t) {
 #pragma unroll
                     for (int k = 0; k < 3; ++k) { s[k][0].relax(m); s[k][1].relax(m); }
-                    held = U;
                 }
-                const bool on = turn + 1 < turns;
-                const int t2 = on ? t : part, b2 = on ? b : b + 1, there = on ? U : b + 1 < last ? some : 0;
-#pragma unroll
-                for (int u = 0; u < U; ++u) {
-                    V v0[2], v1[2];
-                    v[u].values(f, v0, v1);
-                    if (u < there) load(u, t2, b2);
-                    else if (U > 1) v[u] = mr;
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if (MEAN) { v0[e] = f.minus(v0[e], m0[e]); v1[e] = f.minus(v1[e], m1[e]); }
-                        s[0][e].mac(v0[e], v0[e]); s[1][e].mac(v0[e], v1[e]); s[2][e].mac(v1[e], v1[e]);
-                    }
-                }
-                t += U * splits;
+                const int some = min(f.room(), count - t);
+#pragma unroll 1
+                for (int i = 0; i < some; ++i) member(); // one by one: two a turn would save moves and cost the third CTA its registers
             }
             Two r[3];
 #pragma unroll
@@ -188,16 +192,17 @@ __global__ void __launch_bounds__(256, U == 1 ? 3 : 2) k_square_sums(u64 *out, c
                     for (int k = 0; k < 3; ++k) r[k].v[e] = sub_mod(r[k].v[e], mul_mod_any(s[k][e].canonical(m), w.pad, m), m.q);
                 }
             }
-            if (splits > 1) { // the buffers take turns: that of b - 1 is read before the barrier of b, which stands before the writes of b + 1
-                auto &buf = parts[b & 1];
+            if (splits > 1) {
+                u64 *const parts = words;
+                __syncthreads(); // all members have been read
 #pragma unroll
-                for (int k = 0; k < 3; ++k) store2(&buf[k][2 * threadIdx.x], r[k]);
+                for (int k = 0; k < 3; ++k) store2(parts + k * kNormLanes + 2 * threadIdx.x, r[k]);
                 __syncthreads();
                 if (part) continue;
                 for (int j = 1; j < splits; ++j)
 #pragma unroll
                     for (int k = 0; k < 3; ++k) {
-                        const Two y = load2(&buf[k][2 * (threadIdx.x + j * wide)]);
+                        const Two y = load2(parts + k * kNormLanes + 2 * (threadIdx.x + j * wide));
 #pragma unroll
                         for (int e = 0; e < 2; ++e) r[k].v[e] = add_mod(r[k].v[e], y.v[e], m.q);
                     }
@@ -318,30 +323,34 @@ __global__ void __launch_bounds__(256, 4) k_affine(u64 *out, const u64 *x, const
     });
 }
 // Both directions in one pass over dy, g and xhat.  A thread has one residue of TT column tiles: their sums over b stay in its registers, a word each, the sums over t of one b are written (+= for
-// all but the first tiles of a call).  The words of W tiles are in flight; a register that has been multiplied is filled again at once.  SAME: g is dy.
+// all but the first tiles of a call).  The words come through a ring of members in shared memory, which every thread fills for itself, several members ahead.  SAME: g is dy.
 // grid = (N / 128, n)
 struct GradShape { int batch, tile0; };
-constexpr int grad_ctas(int TT, bool SAME) { return TT == 1 ? 7 : TT == 2 ? 5 : TT == 3 ? 4 : TT == 7 || (TT == 5 && !SAME) ? 2 : 3; }
-template <int TT, bool SAME>
-__global__ void __launch_bounds__(128, grad_ctas(TT, SAME)) k_grad_sums(u64 *rows, u64 *rowsum, u64 *cols, u64 *colsum, const u64 *dy, const u64 *g, const u64 *xhat, GradShape w, int n, const PrimeConst *__restrict__ pc, int N) {
-    constexpr int W = TT == 8 ? 2 : TT == 6 ? 3 : TT;
-    static_assert(TT % W == 0, "a tile's words have their place in the registers");
+constexpr int grad_stages(int TT) { return TT == 1 || TT == 6 ? 4 : TT == 8 ? 8 : 6; }
+constexpr size_t grad_smem(int TT, bool same) { return (size_t)grad_stages(TT) * (same ? 4 : 6) * 128 * 8; }
+constexpr int grad_ctas(int TT) { return TT == 1 ? 7 : TT == 2 ? 5 : TT <= 6 ? 4 : 3; }
+template <int TT, bool SAME, int S = grad_stages(TT)>
+__global__ void __launch_bounds__(128, grad_ctas(TT)) k_grad_sums(u64 *rows, u64 *rowsum, u64 *cols, u64 *colsum, const u64 *dy, const u64 *g, const u64 *xhat, GradShape w, int n, const PrimeConst *__restrict__ pc, int N) {
+    constexpr int P = SAME ? 4 : 6;
+    extern __shared__ __align__(16) u64 words[]; // [S][P][128]
     const int l = blockIdx.y;
     const PrimeConst m = pc[l];
     // an address is one that all threads share, and a short offset: pointers of every tile and polynomial would take more registers than the sums
     const size_t poly = (size_t)n * N, per_tile = (size_t)w.batch * 2 * poly;
     const u32 at = (u32)(l * N) + blockIdx.x * 128 + threadIdx.x;
-    size_t from = (size_t)w.tile0 * per_tile;
-    u64 v[W][6];
-    auto fetch = [&](int t, size_t i) {
-        i += t * per_tile;
-        u64 (&y)[6] = v[t % W];
-        y[0] = (xhat + i)[at]; y[1] = (xhat + i + poly)[at]; y[2] = (dy + i)[at]; y[3] = (dy + i + poly)[at];
-        if (!SAME) { y[4] = (g + i)[at]; y[5] = (g + i + poly)[at]; }
+    const u32 ring = smem_u32(words + threadIdx.x);
+    auto fetch = [&](int t, int b, u32 to) {
+        const size_t i = (size_t)(w.tile0 + t) * per_tile + (size_t)b * 2 * poly;
+        cp_async8(to, xhat + i + at); cp_async8(to + 1024, xhat + i + poly + at);
+        cp_async8(to + 2048, dy + i + at); cp_async8(to + 3072, dy + i + poly + at);
+        if (!SAME) { cp_async8(to + 4096, g + i + at); cp_async8(to + 5120, g + i + poly + at); }
     };
     pdl_wait();
 #pragma unroll
-    for (int t = 0; t < W; ++t) fetch(t, from);
+    for (int j = 0; j < S - 1; ++j) {
+        if (j / TT < w.batch) fetch(j % TT, j / TT, ring + j * (P * 1024));
+        cp_async_commit();
+    }
     by_prime(m, [&](auto f) {
         using F = decltype(f);
         using Rows = std::conditional_t<SAME, typename F::Lean, typename F::Sum>;
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(128, grad_ctas(TT, SAME)) k_grad_sums(u64 *row
             for (int k = 0; k < 3; ++k) c[t][k].zero();
             cs[t][0].zero(); cs[t][1].zero();
         }
-        int held = 0;
+        int held = 0, stage = 0;
 #pragma unroll 1
         for (int b = 0; b < w.batch; ++b) {
             if (held == F::kFewest) { // members of a plain sum; a lean one has room for 32
@@ -371,13 +380,15 @@ __global__ void __launch_bounds__(128, grad_ctas(TT, SAME)) k_grad_sums(u64 *row
 #pragma unroll
             for (int k = 0; k < 3; ++k) r[k].zero();
             rs[0].zero(); rs[1].zero();
-            const bool on = b + 1 < w.batch;
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
-                const u64 (&y)[6] = v[t % W];
-                const auto x0 = f.value(y[0]), x1 = f.value(y[1]), d0 = f.value(y[2]), d1 = f.value(y[3]), g0 = SAME ? d0 : f.value(y[4]), g1 = SAME ? d1 : f.value(y[5]);
-                if (t + W < TT) fetch(t + W, from);
-                else if (on) fetch(t + W - TT, from + 2 * poly);
+                cp_async_wait<S - 2>();
+                const u64 *const y = words + stage * (P * 128) + threadIdx.x;
+                const auto x0 = f.value(y[0]), x1 = f.value(y[128]), d0 = f.value(y[256]), d1 = f.value(y[384]), g0 = SAME ? d0 : f.value(y[512 % (P * 128)]), g1 = SAME ? d1 : f.value(y[640 % (P * 128)]);
+                // into the stage that this thread has read a member ago
+                if (b + (t + S - 1) / TT < w.batch) fetch((t + S - 1) % TT, b + (t + S - 1) / TT, ring + (stage ? stage - 1 : S - 1) * (P * 1024));
+                cp_async_commit();
+                if (++stage == S) stage = 0;
                 typename F::Lean p[3];
                 p[0].set(d0, x0, m); p[1].set(d0, x1, d1, x0, m); p[2].set(d1, x1, m);
 #pragma unroll
@@ -395,7 +406,6 @@ __global__ void __launch_bounds__(128, grad_ctas(TT, SAME)) k_grad_sums(u64 *row
                 }
                 rs[0].add(g0); rs[1].add(g1);
             }
-            from += 2 * poly;
             const u64 res[5] = {r[0].canonical(m), r[1].canonical(m), r[2].canonical(m), rs[0].canonical(m), rs[1].canonical(m)};
             u64 *const o = rows + (size_t)b * 3 * poly, *const os = rowsum + (size_t)b * 2 * poly;
 #pragma unroll
