@@ -444,6 +444,15 @@ class Lib:
         return self._op("matmul_acc_grouped", pre.ptr, _i32(inputs), which, (C.c_int32 * len(sizes))(*[_i32(n) for n in sizes]), C.c_int(len(sizes)), arr, C.c_int(bcount), C.c_int(tiles),
                         C.c_int64(row_step))
 
+    def add_const(self, a, v):
+        return self._op("add_const", a.ptr, C.c_double(v))
+
+    def combine(self, xs, coefficients, constant=0.0):
+        """sum_j coefficients[j] xs[j] + constant, un-rescaled."""
+        if len(coefficients) != len(xs):
+            raise ValueError(f"{len(xs)} terms, {len(coefficients)} coefficients")
+        return self._op("combine", _pointers(xs), (C.c_double * len(xs))(*coefficients), C.c_int(len(xs)), C.c_double(constant))
+
     # ---- normalisation: members are [column tile][token tile] ----
     def norm_squares(self, x, groups, mean=None, pad=0):
         """sum_t tensor(x[t][b] - mean[b], itself) - pad * tensor(mean[b], mean[b]), un-relinearised."""

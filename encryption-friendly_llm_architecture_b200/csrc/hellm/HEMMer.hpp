@@ -57,6 +57,7 @@ class MaskCache {
     using Key = std::tuple<int, TileTensorShape, i64, int>; // kind, shape, index, level
     const Plaintext *find(const Key &k) const { auto it = enc_.find(k); return it == enc_.end() ? nullptr : &it->second; }
     const Plaintext &put(const Key &k, Plaintext p) { return enc_.emplace(k, std::move(p)).first->second; }
+    size_t count(int kind) const { size_t n = 0; for (const auto &e : enc_) n += std::get<0>(e.first) == kind; return n; }
     // rotation keys that carry a wrap mask (schedule 2), per (kind, shape, shift index, level)
     const MaskedKey *findKey(const Key &k) const { auto it = keys_.find(k); return it == keys_.end() ? nullptr : &it->second; }
     const MaskedKey &putKey(const Key &k, MaskedKey m) { return keys_.emplace(k, std::move(m)).first->second; }

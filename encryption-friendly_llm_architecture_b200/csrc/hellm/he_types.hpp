@@ -315,6 +315,14 @@ class Evaluator {
     }
     // encrypted vectors times a matrix in 4 bits, un-rescaled
     Ciphertext matvec4(const Ciphertext &x, const hb_qweight *w, int tile) const { hb_ct *o = nullptr; check(c_, hb_matvec_q4(c_, x.raw(), w, tile, &o)); return Ciphertext(c_, o); }
+    // x + v in every slot, and sums of products with constants, un-rescaled (hb_combine)
+    Ciphertext addConstant(const Ciphertext &x, double v) const { hb_ct *o = nullptr; check(c_, hb_add_const(c_, x.raw(), v, &o)); return Ciphertext(c_, o); }
+    Ciphertext combine(const std::vector<const Ciphertext *> &x, const std::vector<double> &c, double constant = 0.0) const {
+        if (c.size() != x.size()) throw std::invalid_argument("[combine] coefficients of another number");
+        std::vector<const hb_ct *> raw;
+        for (auto *y : x) raw.push_back(y->raw());
+        hb_ct *o = nullptr; check(c_, hb_combine(c_, raw.data(), c.data(), (int)raw.size(), constant, &o)); return Ciphertext(c_, o);
+    }
     // normalisation (hb_norm_*): members are [column tile][token tile]; what has three polynomials or a factor comes back un-relinearised and un-rescaled
     Ciphertext normSquares(const Ciphertext &x, const Ciphertext *mean, int groups, int pad) const {
         hb_ct *o = nullptr; check(c_, hb_norm_squares(c_, x.raw(), mean ? mean->raw() : nullptr, groups, pad, &o)); return Ciphertext(c_, o);

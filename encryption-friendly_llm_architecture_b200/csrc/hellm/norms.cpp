@@ -9,7 +9,6 @@
 namespace HELLM {
 
 namespace {
-enum NormMask { kFirstColScaled = 0, kConstant = 1, kColumns = 2 };
 constexpr double kPi = 3.14159265358979323846264338327950288;
 
 // a column tile of `columns` values in every row, zeros behind them
@@ -20,20 +19,23 @@ Plaintext columns_plaintext(const HEMMer &h, const TileTensorShape &s, const dou
         for (i64 c = 0; c < columns; ++c) m.re[(size_t)(r * w + c)] = v ? v[c] : 1.0;
     return h.eval().encode(m, level);
 }
-// plaintexts that depend on a number: the number's bits are part of their key
-const Plaintext &norm_mask(HEMMer &h, NormMask which, const TileTensorShape &s, double value, int level) {
+// Masks that depend on a number: the number's bits are part of their key.  They stay, since recorded graphs hold their addresses, and so there are kNormMasks of a kind at most:
+// a program with more (another range of variances at every step) encodes the others at every call.
+constexpr size_t kNormMasks = 64;
+Plaintext norm_mask(HEMMer &h, int kind, const TileTensorShape &s, double value, int level) {
     i64 bits;
     std::memcpy(&bits, &value, 8);
-    const MaskCache::Key k{sched::kNorm + (int)which, s, bits, level};
+    const MaskCache::Key k{kind, s, bits, level};
     if (const Plaintext *p = h.masks().find(k)) return *p;
-    if (which == kColumns) return h.masks().put(k, columns_plaintext(h, s, nullptr, (i64)value, level));
-    Message m((size_t)h.slots());
-    if (which == kConstant) std::fill(m.re.begin(), m.re.end(), value);
-    else for (i64 r = 0; r < s.getNumRows(); ++r) m.re[(size_t)(r * s.getBlockWidth())] = value;
-    return h.masks().put(k, h.eval().encode(m, level));
+    Plaintext p;
+    if (kind == sched::kNormColumns) p = columns_plaintext(h, s, nullptr, (i64)value, level);
+    else {
+        Message m((size_t)h.slots());
+        for (i64 r = 0; r < s.getNumRows(); ++r) m.re[(size_t)(r * s.getBlockWidth())] = value;
+        p = h.eval().encode(m, level);
+    }
+    return h.masks().count(kind) < kNormMasks ? h.masks().put(k, p) : p;
 }
-const Plaintext &constant(HEMMer &h, double v, int level) { return norm_mask(h, kConstant, TileTensorShape(), v, level); }
-Ciphertext add_constant(HEMMer &h, const Ciphertext &x, double v) { return h.eval().normAffine(x, {}, {&constant(h, v, x.getLevel())}); }
 Ciphertext switched(const Evaluator &ev, const Ciphertext &x) { return ev.rescale(ev.relinearize(x)); }
 // x at a lower level, or a view of x, which has to outlive it; a temporary is moved
 Ciphertext down(const Evaluator &ev, const Ciphertext &x, int level) { return x.getLevel() == level ? ev.view(x, 0, x.getBatch()) : ev.levelDown(x, level); }
@@ -43,8 +45,11 @@ Ciphertext down(const Evaluator &ev, Ciphertext &&x, int level) { return x.getLe
 Ciphertext row_mean(HEMMer &h, Ciphertext x, const TileTensorShape &s, double scale, const Ciphertext *y = nullptr, double other = 0.0) {
     const Evaluator &ev = h.eval();
     for (i64 i = 1; i < s.getBlockWidth(); i <<= 1) x = ev.add(x, ev.leftRotate(x, i));
-    const Plaintext &mask = norm_mask(h, kFirstColScaled, s, scale, x.getLevel());
-    x = y ? ev.multSumRescaledOnce({&x, y}, {&mask, &norm_mask(h, kFirstColScaled, s, other, x.getLevel())}) : ev.mult(x, mask);
+    const Plaintext mask = norm_mask(h, sched::kNormFirstCol, s, scale, x.getLevel());
+    if (y) {
+        const Plaintext second = norm_mask(h, sched::kNormFirstCol, s, other, x.getLevel());
+        x = ev.multSumRescaledOnce({&x, y}, {&mask, &second});
+    } else x = ev.mult(x, mask);
     for (i64 i = 1; i < s.getBlockWidth(); i <<= 1) x = ev.add(x, ev.rightRotate(x, i));
     return x;
 }
@@ -72,7 +77,7 @@ std::vector<Plaintext> column_plaintexts(HEMMer &h, const NormShape &n, const do
     std::vector<Plaintext> p;
     for (i64 t = 0; t < n.groups; ++t) {
         const i64 here = std::min(w, n.columns - t * w);
-        p.push_back(v ? columns_plaintext(h, n.s, v + t * w, here, level) : norm_mask(h, kColumns, n.s, (double)here, level));
+        p.push_back(v ? columns_plaintext(h, n.s, v + t * w, here, level) : norm_mask(h, sched::kNormColumns, n.s, (double)here, level));
     }
     return p;
 }
@@ -104,14 +109,13 @@ int chebyshev_depth(int n) {
 // T_m for m = 1, 2, 3 and the powers of two, from T_2a = 2 T_a^2 - 1 and T_3 = 2 T_1 T_2 - T_1; and sums of them: a polynomial of degree n is q T_m + r for the largest power of two m <= n, with
 // q_j = 2 c_{m+j} (q_0 = c_m) and r_{m-j} = c_{m-j} - c_{m+j}, since T_m T_j = (T_{m+j} + T_{m-j}) / 2.  Constants are added last.
 struct Chebyshev {
-    HEMMer &h;
     const Evaluator &ev;
     std::vector<Ciphertext> t; // t[m]
-    Chebyshev(HEMMer &h_, const Ciphertext &u, int n) : h(h_), ev(h_.eval()), t((size_t)std::max(n, 3) + 1) {
+    Chebyshev(const Evaluator &e, const Ciphertext &u, int n) : ev(e), t((size_t)std::max(n, 3) + 1) {
         t[1] = ev.view(u, 0, u.getBatch());
         for (int m = 2; m <= n; m <<= 1) {
             const Ciphertext s = ev.square(t[(size_t)m / 2]);
-            t[(size_t)m] = add_constant(h, ev.add(s, s), -1.0);
+            t[(size_t)m] = ev.addConstant(ev.add(s, s), -1.0);
         }
         if (n >= 3) {
             const Ciphertext s = ev.mult(t[1], t[2]);
@@ -119,7 +123,7 @@ struct Chebyshev {
         }
     }
     struct Sum { Ciphertext x; double c = 0.0; }; // x + c; no x: c alone
-    Ciphertext whole(Sum &&s) const { return s.c == 0.0 ? std::move(s.x) : add_constant(h, s.x, s.c); }
+    Ciphertext whole(Sum &&s) const { return s.c == 0.0 ? std::move(s.x) : ev.addConstant(s.x, s.c); }
     Sum eval(std::vector<double> c) const {
         while (c.size() > 1 && c.back() == 0.0) c.pop_back();
         const int n = (int)c.size() - 1;
@@ -130,14 +134,15 @@ struct Chebyshev {
             const int level = t[(size_t)n].getLevel();
             std::vector<Ciphertext> x;
             std::vector<const Ciphertext *> px;
-            std::vector<const Plaintext *> pc;
+            std::vector<double> k;
             for (int j = 1; j <= n; ++j) {
                 if (c[(size_t)j] == 0.0) continue;
                 x.push_back(down(ev, t[(size_t)j], level));
-                pc.push_back(&constant(h, c[(size_t)j], level));
+                k.push_back(c[(size_t)j]);
             }
             for (const Ciphertext &y : x) px.push_back(&y);
-            r.x = ev.multSumRescaledOnce(px, pc);
+            r.x = ev.rescale(ev.combine(px, k, r.c));
+            r.c = 0.0;
             return r;
         }
         const int m = 1 << log2_floor(n);
@@ -145,14 +150,14 @@ struct Chebyshev {
         for (int j = 1; j <= n - m; ++j) { rest[(size_t)(m - j)] -= q[(size_t)j]; q[(size_t)j] *= 2.0; }
         Sum high = eval(q), low = eval(rest);
         const Ciphertext &tm = t[(size_t)m];
-        r.x = high.x.empty() ? ev.mult(tm, constant(h, high.c, tm.getLevel())) : ev.mult(whole(std::move(high)), tm);
+        r.x = high.x.empty() ? ev.rescale(ev.combine({&tm}, {high.c})) : ev.mult(whole(std::move(high)), tm);
         if (!low.x.empty()) r.x = ev.add(r.x, low.x);
         r.c = low.c;
         return r;
     }
 };
-Ciphertext evaluate(HEMMer &h, const Ciphertext &u, const std::vector<double> &c) {
-    const Chebyshev t(h, u, (int)c.size() - 1);
+Ciphertext evaluate(const Evaluator &ev, const Ciphertext &u, const std::vector<double> &c) {
+    const Chebyshev t(ev, u, (int)c.size() - 1);
     auto s = t.eval(c);
     if (s.x.empty()) throw std::invalid_argument("[chebyshev] a constant");
     return t.whole(std::move(s));
@@ -194,9 +199,9 @@ HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns
             const Ciphertext s = switched(ev, ev.concat(both)), of_mean = ev.group(s, 1, 2);
             row = row_mean(*this, ev.group(s, 0, 2), n.s, scale, &of_mean, -scale * (double)n.pad);
         } else row = row_mean(*this, switched(ev, squares), n.s, scale);
-        u = add_constant(*this, row, (2.0 * eps - hi - lo) / (hi - lo)); // the variance's place in [-1, 1]
+        u = ev.addConstant(row, (2.0 * eps - hi - lo) / (hi - lo)); // the variance's place in [-1, 1]
     }
-    Ciphertext rstd = evaluate(*this, u, c);
+    Ciphertext rstd = evaluate(eval_, u, c);
     const int level = rstd.getLevel();
     const Ciphertext low_mean = down(ev, mean, level);
     Ciphertext xhat = switched(ev, ev.normScale(down(ev, x.get(), level), &low_mean, rstd, groups));
@@ -272,8 +277,8 @@ std::vector<Ciphertext> HEMMer::clipGradNorm(const std::vector<const Ciphertext 
     need_level(level, 3 + polynomialDepth(degree), "clipGradNorm");
     const Evaluator &ev = eval_;
     Ciphertext square = gradNormSquared(grads);
-    const Ciphertext u = add_constant(*this, ev.mult(square, constant(*this, 2.0 / (bound * bound), square.getLevel())), -1.0);
-    const Ciphertext factor = evaluate(*this, u, c);
+    const Ciphertext u = ev.rescale(ev.combine({&square}, {2.0 / (bound * bound)}, -1.0));
+    const Ciphertext factor = evaluate(eval_, u, c);
     std::vector<Ciphertext> low;
     for (const Ciphertext *x : grads) low.push_back(down(ev, *x, factor.getLevel()));
     std::vector<Ciphertext> products = ev.scaleMany(low, factor), out;

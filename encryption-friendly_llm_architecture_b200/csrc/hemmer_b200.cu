@@ -1320,6 +1320,47 @@ void do_scale_many(hb_ctx *c, const hb_ct *const *xs, int count, const hb_ct *fa
     }
     flush();
 }
+// ---- constants ----
+// v times the scale of a level as a whole number, modulo every prime
+void constant_words(const hb_ctx *c, int level, double v, u64 *k, const char *what) {
+    const double whole = std::rint(v * c->h->scale[(size_t)level]);
+    if (!std::isfinite(v)) fail(HB_E_ARG, std::string(what) + ": a constant is not finite");
+    if (!(std::fabs(whole) < 0x1p62)) fail(HB_E_LIMIT, std::string(what) + ": a constant beyond 62 bits at the scale");
+    for (int i = 0; i <= level; ++i) {
+        const u64 q = c->h->q[(size_t)i], a = (u64)std::fabs(whole) % q;
+        k[i] = whole < 0 && a ? q - a : a;
+    }
+}
+// products: with the coefficients, at the scale of a product; otherwise x + constant
+hb_ct *do_combine(hb_ctx *c, const hb_ct *const *xs, const double *coefficients, int count, double constant, const char *what) {
+    if (!xs) fail(HB_E_ARG, std::string(what) + ": null argument");
+    if (count < 1 || count > kCombineTerms) fail(HB_E_LIMIT, std::string(what) + ": 1 to 16 terms");
+    for (int j = 0; j < count; ++j) {
+        if (!xs[j]) fail(HB_E_ARG, std::string(what) + ": null argument");
+        own(c, xs[j]);
+        check_same(xs[0], xs[j], what);
+    }
+    const hb_ct *a = xs[0];
+    if (a->spow != 1) fail(HB_E_SHAPE, std::string(what) + ": operand not rescaled");
+    const i64 polynomials = (i64)a->batch * a->np;
+    if (polynomials > 65535) fail(HB_E_LIMIT, std::string(what) + ": too many members");
+    CombineList l{};
+    l.count = count; l.np = a->np;
+    constant_words(c, a->level, constant, l.k0, what);
+    const Scalars K = whole_scale(c, a->level);
+    for (int j = 0; j < count; ++j) {
+        l.x[j] = xs[j]->d;
+        if (coefficients) constant_words(c, a->level, coefficients[j], l.k[j], what);
+        else for (int i = 0; i <= a->level; ++i) l.k[j][i] = 1;
+    }
+    for (int i = 0; coefficients && i <= a->level; ++i) l.k0[i] = hbhost::mulmod(l.k0[i], K.v[i], c->h->q[(size_t)i]);
+    hb_ct *r = new_ct(c, a->level, a->np, a->batch, coefficients ? 2 : 1);
+    try {
+        ALG(c, (size_t)(count + 1) * a->limbs());
+        launch(c, k_combine, dim3((unsigned)(c->N / kNormLanes), (unsigned)(a->level + 1), (unsigned)polynomials), 256, 0, r->d, l, a->level + 1, c->pc, c->N);
+    } catch (...) { hb_ct_free(r); throw; }
+    return r;
+}
 hb_ct *do_level_down(hb_ctx *c, const hb_ct *a, int target) {
     own(c, a);
     if (target > a->level || target < 0) fail(HB_E_LEVEL, "level_down: bad target");
@@ -2394,6 +2435,12 @@ int hb_norm_grad_sums(hb_ctx *c, const hb_ct *dy, const hb_ct *g, const hb_ct *x
 }
 int hb_norm_grad_input(hb_ctx *c, const hb_ct *g, const hb_ct *mean, const hb_ct *xhat, const hb_ct *dot, int groups, hb_ct **out) {
     return guard(c, [&] { if (!out) fail(HB_E_ARG, "norm_grad_input: null argument"); *out = do_norm_grad_input(c, g, mean, xhat, dot, groups); });
+}
+int hb_combine(hb_ctx *c, const hb_ct *const *xs, const double *coefficients, int count, double constant, hb_ct **out) {
+    return guard(c, [&] { if (!coefficients || !out) fail(HB_E_ARG, "combine: null argument"); *out = do_combine(c, xs, coefficients, count, constant, "combine"); });
+}
+int hb_add_const(hb_ctx *c, const hb_ct *a, double re, hb_ct **out) {
+    return guard(c, [&] { if (!out) fail(HB_E_ARG, "add_const: null argument"); *out = do_combine(c, &a, nullptr, 1, re, "add_const"); });
 }
 int hb_square_sum_many(hb_ctx *c, const hb_ct *const *xs, int count, hb_ct **out) {
     return guard(c, [&] { if (!out) fail(HB_E_ARG, "square_sum_many: null argument"); *out = do_square_sum_many(c, xs, count); });

@@ -467,4 +467,30 @@ __global__ void __launch_bounds__(256, 3) k_grad_input(u64 *out, const u64 *g, c
     });
 }
 
+// ---- constants ----
+// out = sum_j k[j] x_j + k0 on the first polynomial of every member, without the constant on the others; a plaintext of a constant would be N words of it.
+// grid = (N / 512, n, polynomials of all members)
+constexpr int kCombineTerms = 16;
+struct CombineList { const u64 *x[kCombineTerms]; u64 k[kCombineTerms][kMaxPrimes], k0[kMaxPrimes]; int count, np; };
+__global__ void __launch_bounds__(256, 4) k_combine(u64 *out, const __grid_constant__ CombineList c, int n, const PrimeConst *__restrict__ pc, int N) {
+    const int l = blockIdx.y;
+    const PrimeConst m = pc[l];
+    const size_t from = ((size_t)blockIdx.z * n + l) * N;
+    const u32 at = (blockIdx.x * 256 + threadIdx.x) * 2;
+    const u64 add = blockIdx.z % (u32)c.np ? 0 : c.k0[l];
+    pdl_wait();
+    by_prime(m, [&](auto f) {
+        typename decltype(f)::Sum s[2];
+        s[0].zero(); s[1].zero();
+#pragma unroll 2
+        for (int j = 0; j < c.count; ++j) {
+            const Two x = load2(c.x[j] + from + at);
+            if (j && j % f.kFewest == 0) { s[0].relax(m); s[1].relax(m); }
+            const auto k = f.value(c.k[j][l]);
+            s[0].mac(f.value(x.v[0]), k); s[1].mac(f.value(x.v[1]), k);
+        }
+        store2(out + from + at, Two{{add_mod(s[0].canonical(m), add, m.q), add_mod(s[1].canonical(m), add, m.q)}});
+    });
+}
+
 } // namespace hb

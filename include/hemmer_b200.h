@@ -198,6 +198,10 @@ int hb_relin(hb_ctx *ctx, const hb_ct *a, hb_ct **out);                         
 int hb_mul(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, hb_ct **out);           /* mult(ct,ct) :311-312 */
 int hb_square(hb_ctx *ctx, const hb_ct *a, hb_ct **out);                        /* square :363 */
 int hb_mul_const(hb_ctx *ctx, const hb_ct *a, double re, double im, hb_ct **out); /* mult(ct, Complex / Real) :275-278 */
+/* a + re in every slot (HomEvaluator::add(ct, Real)), and sum_j coefficients[j] xs[j] + constant for 1 to 16 ciphertexts of one shape, un-rescaled: constants as whole
+ * numbers at the scale of the level (62 bits at most, HB_E_LIMIT otherwise), so no plaintext is encoded and the calls can be recorded */
+int hb_add_const(hb_ctx *ctx, const hb_ct *a, double re, hb_ct **out);
+int hb_combine(hb_ctx *ctx, const hb_ct *const *xs, const double *coefficients, int count, double constant, hb_ct **out);
 int hb_rotate(hb_ctx *ctx, const hb_ct *a, int64_t left_steps, hb_ct **out);    /* leftRotate :383 / rightRotate :403 */
 int hb_conjugate(hb_ctx *ctx, const hb_ct *a, hb_ct **out);                     /* conjugate :465 */
 /* Hoisted rotations: hb_decompose does the part of leftRotate that does not depend on the step (inverse NTT,

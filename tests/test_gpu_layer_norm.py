@@ -219,6 +219,57 @@ def test_a_step_of_training(deep):
         assert np.abs(_decrypt(h, o, 1, 1)[0, 0] - v * f).max() < TOL
 
 
+def test_replayed_from_a_graph(deep):
+    """A layer norm without weights, its gradients and their clipping need nothing from the host after their first run."""
+    h, T, B, D, w, rows = deep, 2, 1, 64, 32, 16
+    rng = np.random.default_rng(11)
+    x, dy = [_data(rng, B, rows, D) for _ in range(2)], rng.uniform(-1, 1, (B, rows, D))
+    cx, other, cdy = _encrypt(h, _tiles(x[0], T, w)), _encrypt(h, _tiles(x[1], T, w), seed=7), _encrypt(h, _tiles(dy, T, w), seed=8)
+
+    def step():
+        y, xhat, rstd = h.layer_norm(cx, D, RANGE, groups=T, degree=3)
+        grads = h.layer_norm_backward(cdy, xhat, rstd, D, groups=T)
+        square = h.grad_norm_squared([cdy])
+        return [y.ct, xhat.ct, rstd.ct, square, *[t.ct for t in grads]], (y, xhat, rstd, grads)
+
+    first = [h.lib.ct_export(o) for o in step()[0]]
+    h.lib.graph_begin()
+    outs, held = step()
+    graph = h.lib.graph_end()
+    keep = h.lib.ct_export(cx.ct)
+    h.lib.ct_import(cx.ct, h.lib.ct_export(other.ct))
+    h.lib.graph_launch(graph)
+    c, _ = h.polynomial("rsqrt", *RANGE, 3)
+    assert np.abs(_whole(_decrypt(h, held[0], T, B), D) - _model(x[1], 1.0, 0.0, 1e-5, RANGE, c)[0]).max() < TOL
+    h.lib.ct_import(cx.ct, keep)
+    h.lib.graph_launch(graph)
+    for o, want in zip(outs, first):
+        assert np.array_equal(h.lib.ct_export(o), want)
+
+
+def test_ranges_without_end(deep):
+    """Masks that depend on the range are kept up to a number; beyond it a call makes its own, with the same result."""
+    h, D, w, rows = deep, 32, 32, 16
+    rng = np.random.default_rng(12)
+    x = _data(rng, 1, rows, D)
+    cx = _encrypt(h, _tiles(x, 1, w))
+
+    def used():
+        total, now = C.c_uint64(), C.c_uint64()
+        h.lib._fn("mem_info")(h.lib.ctx, C.byref(total), C.byref(now))
+        return now.value
+
+    sizes = []
+    for k in range(140):
+        rng_k = (0.1, 1.3 + 0.01 * k)
+        y, _, _ = h.layer_norm(cx, D, rng_k, degree=3)
+        if k % 35 == 34:
+            c, _ = h.polynomial("rsqrt", *rng_k, 3)
+            assert np.abs(_whole(_decrypt(h, y, 1, 1), D) - _model(x, 1.0, 0.0, 1e-5, rng_k, c)[0]).max() < TOL
+            sizes.append(used())
+    assert sizes[-1] == sizes[-2], sizes
+
+
 def test_refusals(pkg, deep):
     h, rng = deep, np.random.default_rng(1)
     x = _encrypt(h, rng.uniform(-1, 1, (2, 1, 16, 32)))

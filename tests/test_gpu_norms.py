@@ -178,6 +178,60 @@ def test_primes_of_other_lengths(pkg, n_bits):
         g.close()
 
 
+def _whole(v, scale):
+    return int(np.rint(v * scale))
+
+
+@pytest.mark.parametrize("edge", [False, True])
+@pytest.mark.parametrize("terms,members,polys,level", [(1, 1, 2, 3), (2, 3, 2, 0), (3, 2, 3, 5), (8, 1, 2, 1), (9, 2, 1, 2), (16, 5, 2, 8)])
+def test_combine(ring, terms, members, polys, level, edge):
+    g = ring
+    rng = np.random.default_rng(terms)
+    xs = [_rand(g, level, members, 20 + j, polys=polys, edge=edge) for j in range(terms)]
+    at = _points(g, rng, 12)
+    handles, scale = [_ct(g, x) for x in xs], float(g.scales[level])
+    coefficients = [float(v) for v in rng.uniform(-3, 3, terms)]
+    coefficients[0] = 0.0 if edge else -1.0
+    for constant in (0.0, 0.75, -1234.5):
+        k, k0 = [_whole(v, scale) for v in coefficients], _whole(constant, scale) * _scale(g, level)
+        want = []
+        for b in range(members):
+            total = sum(kk * _objects(x, at)[b] for kk, x in zip(k, xs))
+            total[0] = total[0] + k0
+            want.append(total)
+        _check(g, g.combine(handles, coefficients, constant), want, at, level, polys, 2)
+        want = [_objects(xs[0], at)[b].copy() for b in range(members)]
+        for v in want:
+            v[0] = v[0] + _whole(constant, scale)
+        _check(g, g.add_const(handles[0], constant), want, at, level, polys, 1)
+
+
+def test_constants_are_what_encoded_ones_are(gpu_small):
+    """Slots of x + v, and of sums with coefficients, after decryption."""
+    g = gpu_small
+    rng = np.random.default_rng(3)
+    z = [rng.uniform(-1, 1, g.slots) for _ in range(3)]
+    cts = [g.encrypt(g.encode(v, 4), 50 + k) for k, v in enumerate(z)]
+    assert np.abs(g.decrypt(g.add_const(cts[0], -2.25)) - (z[0] - 2.25)).max() < 2.0 ** -20
+    got = g.rescale(g.combine(cts, [0.5, -3.0, 1e-3], 7.125))
+    assert np.abs(g.decrypt(got) - (0.5 * z[0] - 3.0 * z[1] + 1e-3 * z[2] + 7.125)).max() < 2.0 ** -20 and g.ct_meta(got)[0] == 3
+
+
+def test_constants_that_are_refused(pkg, gpu_small, gpu_mid):
+    g = gpu_small
+    x, low, raw = _ct(g, _rand(g, 3, 2, 1)), _ct(g, _rand(g, 2, 2, 1)), _ct(g, _rand(g, 3, 2, 1), 2)
+    for code, call in ((-1, lambda: g.add_const(x, float("nan"))), (-1, lambda: g.add_const(x, float("inf"))), (-9, lambda: g.add_const(x, 2.0 ** 21)), (-3, lambda: g.add_const(raw, 1.0)),
+                       (-1, lambda: g.combine([x], [float("nan")])), (-9, lambda: g.combine([x], [-2.0 ** 21])), (-9, lambda: g.combine([x], [1.0], 2.0 ** 21)), (-2, lambda: g.combine([x, low], [1.0, 1.0])),
+                       (-9, lambda: g.combine([], [])), (-9, lambda: g.combine([x] * 17, [1.0] * 17)), (-1, lambda: g.combine([_ct(gpu_mid, _rand(gpu_mid, 3, 2, 1))], [1.0]))):
+        with pytest.raises(pkg.HBError) as e:
+            call()
+        assert e.value.code == code, e.value
+    with pytest.raises(ValueError):
+        g.combine([x], [1.0, 2.0])
+    assert g._fn("combine")(g.ctx, (C.c_void_p * 1)(x.ptr.value), None, 1, C.c_double(0.0), C.byref(C.c_void_p())) == -1
+    assert g._fn("add_const")(g.ctx, None, C.c_double(0.0), C.byref(C.c_void_p())) == -1
+
+
 def test_views_and_whole_calls_of_the_library_agree(gpu_small):
     """Runs of members without a copy as operands, and the residues of hb_tensor, hb_sub and hb_add."""
     g = gpu_small
@@ -201,7 +255,8 @@ def test_replayed_from_a_graph(gpu_small):
 
     def all_calls():
         return [g.norm_squares(h["x"], T, mean=h["m"], pad=3), g.norm_scale(h["x"], h["r"], T, mean=h["m"]), g.norm_affine(h["x"], T, gamma=pts, beta=pts),
-                *g.norm_grad_sums(h["x"], h["y"], T), g.norm_grad_input(h["x"], h["m"], h["y"], h["r"], T), g.square_sum_many([h["x"], h["r"]]), *g.scale_many([h["x"], h["m"]], h["f"])]
+                *g.norm_grad_sums(h["x"], h["y"], T), g.norm_grad_input(h["x"], h["m"], h["y"], h["r"], T), g.square_sum_many([h["x"], h["r"]]), *g.scale_many([h["x"], h["m"]], h["f"]),
+                g.combine([h["x"], h["y"]], [0.5, -2.0])]
 
     want = [g.ct_export(o) for o in all_calls()]
     g.graph_begin()

@@ -1,10 +1,14 @@
 """The polynomials of layer_norm and clip_grad_norm, which need no device, and what the Python layer checks of its arguments."""
 import ctypes as C
+import os
+import subprocess
 from types import SimpleNamespace
 
 import numpy as np
 import pytest
 from numpy.polynomial import chebyshev
+
+from conftest import PKG_NAME, ROOT
 
 
 @pytest.fixture(scope="module")
@@ -54,6 +58,13 @@ def test_polynomials_that_are_refused(pkg, polynomial):
         with pytest.raises(pkg.HBError) as e:
             polynomial(which, a, b, degree)
         assert e.value.code == -1
+
+
+def test_rules_of_dispatch(tmp_path):
+    exe = str(tmp_path / "norm_rules")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-Wall", os.path.join(ROOT, "tests", "integration", "norm_rules.cpp"), "-I", os.path.join(ROOT, PKG_NAME, "csrc"), "-o", exe])
+    done = subprocess.run([exe], capture_output=True, text=True, timeout=120)
+    assert done.returncode == 0, done.stdout[:2000]
 
 
 def test_lists_of_another_length(pkg):
