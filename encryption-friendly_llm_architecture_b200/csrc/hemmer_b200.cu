@@ -1151,7 +1151,7 @@ hb_ct *do_norm_squares(hb_ctx *c, const hb_ct *x, const hb_ct *mean, int groups,
     const int batch = norm_batch(x, groups, "norm_squares"), n = x->level + 1, N = c->N;
     if (mean) norm_shared(c, mean, x, batch, "norm_squares");
     if (pad < 0 || pad > c->h->slots || (pad && !mean)) fail(HB_E_ARG, "norm_squares: members of padding are counted from 0 to the slots, and only beside a mean");
-    const int log_splits = norm_log_splits(groups, (long)(N / kNormLanes) * batch * n), chunk = log_splits ? 1 : norm_chunk(batch, (long)(N / kNormLanes) * n, 1);
+    const int log_splits = norm_log_splits(groups, (long)(N / kNormLanes) * batch * n, 3), chunk = log_splits ? 1 : norm_chunk(batch, (long)(N / kNormLanes) * n, 1);
     const dim3 grid((unsigned)(N / kNormLanes << log_splits), (unsigned)n, (unsigned)((batch + chunk - 1) / chunk));
     hb_ct *r = new_ct(c, x->level, 3, batch, 2);
     try {
@@ -1224,6 +1224,16 @@ GradSums do_norm_grad_sums(hb_ctx *c, const hb_ct *dy, const hb_ct *g, const hb_
     try {
         for (int k = 0; k < 4; ++k) s.r[k] = new_ct(c, dy->level, k % 2 ? 2 : 3, k < 2 ? batch : groups, k % 2 ? 1 : 2);
         ALG(c, (g == dy ? 2 : 3) * dy->limbs() + (size_t)5 * (batch + groups) * n);
+        auto one_way = [&](hb_ct *out, hb_ct *sum, const hb_ct *y, int terms, int results, int by_i, int by_j) {
+            const int log_splits = norm_log_splits(terms, (long)(N / kPairSumLanes) * results * n, 2), chunk = log_splits ? 1 : norm_chunk(results, (long)(N / kPairSumLanes) * n, 1);
+            launch(c, k_pair_sums, dim3((unsigned)(N / kPairSumLanes << log_splits), (unsigned)n, (unsigned)((results + chunk - 1) / chunk)), 128, pair_sum_smem(), out->d, sum->d, y->d, xhat->d,
+                   PairSumShape{terms, results, by_i, by_j, chunk, log_splits}, n, c->pc, N);
+        };
+        if (!grad_together(groups, batch, g == dy, (long)(N / 128) * n)) {
+            one_way(s.r[0], s.r[1], g, groups, batch, batch, 1);
+            one_way(s.r[2], s.r[3], dy, batch, groups, 1, batch);
+            return s;
+        }
         for (int t0 = 0; t0 < groups;) {
             const int some = std::min(grad_tiles(groups), groups - t0);
             auto go = [&](auto tiles, auto same) {
@@ -1281,7 +1291,7 @@ hb_ct *do_square_sum_many(hb_ctx *c, const hb_ct *const *xs, int count) {
         int some = 0, first = 1;
         auto flush = [&] {
             if (!some) return;
-            const int log_splits = norm_log_splits(some, (long)(N / kNormLanes) * n);
+            const int log_splits = norm_log_splits(some, (long)(N / kNormLanes) * n, 3);
             launch(c, k_square_sums<MemberList, false>, dim3((unsigned)(N / kNormLanes << log_splits), (unsigned)n), 256, square_smem(), r->d, list, nullptr, SquareShape{some, 1, 1, log_splits, 0}, n, c->pc, N, first ? 0 : 1);
             some = first = 0;
         };

@@ -142,21 +142,32 @@ constexpr int pair_ranges(PairBlock b, int N, int nr, int nc, int heads, int lim
     return run;
 }
 
-// Members that a CTA takes one after the other where they share a factor: as many as leave `enough` CTAs, eight at most, but more where a grid of 65535 a column of
-// members would not reach them.  `each`: CTAs with one chunk for all members; `columns` of them side by side.
+// Members that a CTA takes one after the other where they share a factor or a place in a ring: up to eight, as long as eight CTAs an SM are left, but more where a grid of 65535 would not reach
+// them.  `each`: CTAs with one chunk for all members of a column; `columns` of them.  Calls at level 5, us, one member a CTA / this: products with one factor 3 tiles of 4 token tiles 50 / 39,
+// of 16 193 / 142, 8 of 16 507 / 336; gradients of the input 68 / 52, 273 / 203, 723 / 485; squares 26 / 24, 93 / 86, 165 / 164.
 constexpr int norm_chunk(int members, long each, long columns) {
     int chunk = members < 8 ? members : 8;
     while (chunk > 1 && each * columns * ((members + chunk - 1) / chunk) < 148 * 8) --chunk;
     while (columns * ((members + chunk - 1L) / chunk) > 65535 && chunk < members) ++chunk;
     return chunk;
 }
-// Parts of the members of a sum, as a power of two up to eight: more while there are CTAs missing and every part has some members left.  `each`: CTAs without parts.
-constexpr int norm_log_splits(int members, long each) {
+// Parts of the members of a sum, as a power of two up to `most`: while SMs have no CTA and every part keeps two members, and up to four CTAs an SM while every part keeps eight.  `each`:
+// CTAs without parts.  Calls, us, without parts / with: 2^16 coefficients, 250 members of one limb 81 / 54, 64 of one 22 / 16, 16 of two 13.4 / 9.2, 40 of three 30 / 24; 2^12, 250 of three 71 / 13.5, 40 tiles of
+// 4 at level 5 22 / 15.  With two members a part throughout, 8 members of two limbs took 9.0 instead of 6.8.
+constexpr int norm_log_splits(int members, long each, int most) {
     int log = 0;
-    while (log < 3 && (each << log) < 148 * 4 && members >= 4 << log) ++log;
+    while (log < most && ((each << log) < 148 ? members >= 4 << log : (each << log) < 148 * 4 && members >= 16 << log)) ++log;
     return log;
 }
-// Column tiles of a launch of the sums in both directions: even launches of at most eight.
+// Whether the sums of a layer norm's gradients go through one kernel for both directions (k_grad_sums, `each` CTAs a launch), which reads dy, g and xhat once, or through one for each (k_pair_sums),
+// which reads xhat twice, but fills the GPU with fewer limbs and has no launches that add up rows.  Calls, us, one kernel / two, and with g = dy: 3 tiles of 4 at level 5 56 / 69, 44 / 69; 8 of 16 478 / 567,
+// 362 / 574; 5 of 8 170 / 202, 118 / 202; 5 of 8 at level 1 78 / 64, 52 / 63; 7 of 8 255 / 277, 177 / 278; 12 of 4 278 / 228, 208 / 228; 24 of 2 at level 2 175 / 130, 147 / 130; 16 of 8 at level 3 408 / 358,
+// 331 / 363; 2^12 coefficients, 12 of 8 at level 6 110 / 33, 65 / 28, 3 of 16 at level 8 29 / 22, 22 / 19, 3 of 2 at level 5 7.9 / 10.1, 7.7 / 10.1.
+constexpr bool grad_together(int tiles, int batch, bool same, long each) {
+    if (tiles <= 8 && tiles * (long)batch <= 8) return true; // the second launch would take longer than the work
+    return same || tiles <= 4 ? each >= 148 * 3 : tiles <= 8 && each >= 148 * 8;
+}
+// Column tiles of a launch of k_grad_sums: even launches of at most eight, as many as its registers hold.  Four at most, 8 tiles of 16 token tiles at level 5: 678 us instead of 499.
 constexpr int grad_tiles(int tiles) {
     const int launches = (tiles + 7) / 8;
     return (tiles + launches - 1) / launches;

@@ -423,6 +423,95 @@ __global__ void __launch_bounds__(128, grad_ctas(TT)) k_grad_sums(u64 *rows, u64
         }
     });
 }
+// One direction: out[j] = sum_i y(i, j) (x) xhat(i, j) and sum[j] = sum_i y(i, j), member (i, j) being i by_i + j by_j, for a chunk of results one after the other.  Parts and the ring as in
+// k_square_sums.  grid = (N splits / 256, n, chunks)
+struct PairSumShape { int terms, results, by_i, by_j, chunk, log_splits; };
+constexpr int kPairSumStages = 4, kPairSumLanes = 256;
+constexpr size_t pair_sum_smem() { return (size_t)kPairSumStages * 4 * kPairSumLanes * 8; }
+__global__ void __launch_bounds__(128, 5) k_pair_sums(u64 *out, u64 *sum, const u64 *y, const u64 *xhat, PairSumShape w, int n, const PrimeConst *__restrict__ pc, int N) {
+    constexpr int S = kPairSumStages, L = kPairSumLanes;
+    extern __shared__ __align__(16) u64 words[]; // [S][4][256]; of parts, which have one result a CTA, [5][256] in the end
+    const int splits = 1 << w.log_splits, wide = 128 >> w.log_splits, lane = threadIdx.x & (wide - 1), part = threadIdx.x >> (7 - w.log_splits);
+    const int l = blockIdx.y, first = blockIdx.z * w.chunk, last = min(first + w.chunk, w.results);
+    const PrimeConst m = pc[l];
+    const size_t poly = (size_t)n * N;
+    const u32 at = (u32)(l * N) + (blockIdx.x * wide + lane) * 2;
+    const int count = (w.terms - part + splits - 1) >> w.log_splits;
+    const u32 ring = smem_u32(words + 2 * threadIdx.x);
+    int f_j = first, f_i = 0, f_stage = 0, stage = 0;
+    auto fetch = [&] {
+        if (f_j < last) {
+            const size_t from = ((size_t)(part + f_i * splits) * w.by_i + (size_t)f_j * w.by_j) * 2 * poly;
+            const u32 to = ring + f_stage * (4 * L * 8);
+            cp_async16(to, y + from + at); cp_async16(to + L * 8, y + from + poly + at);
+            cp_async16(to + 2 * L * 8, xhat + from + at); cp_async16(to + 3 * L * 8, xhat + from + poly + at);
+            if (++f_i == count) { f_i = 0; ++f_j; }
+            if (++f_stage == S) f_stage = 0;
+        }
+        cp_async_commit();
+    };
+    pdl_wait();
+#pragma unroll
+    for (int k = 0; k < S - 1; ++k) fetch();
+    by_prime(m, [&](auto f) {
+        using F = decltype(f);
+        const int room = min(f.room() / 2, F::kFewest); // two products a member in the middle sums, and what a plain sum holds
+#pragma unroll 1
+        for (int j = first; j < last; ++j) {
+            typename F::Sum s[3][2];
+            typename F::Plain p[2][2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { s[0][e].zero(); s[1][e].zero(); s[2][e].zero(); p[0][e].zero(); p[1][e].zero(); }
+#pragma unroll 1
+            for (int t = 0; t < count; t += room) {
+                if (t) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) { s[0][e].relax(m); s[1][e].relax(m); s[2][e].relax(m); p[0][e].relax(m); p[1][e].relax(m); }
+                }
+                const int some = min(room, count - t);
+#pragma unroll 1
+                for (int i = 0; i < some; ++i) {
+                    cp_async_wait<S - 2>();
+                    const u64 *v = words + stage * (4 * L) + 2 * threadIdx.x;
+                    const Two a = load2(v), b = load2(v + L), c = load2(v + 2 * L), d = load2(v + 3 * L);
+                    if (++stage == S) stage = 0;
+                    fetch(); // into the stage that this thread read a member ago
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const auto y0 = f.value(a.v[e]), y1 = f.value(b.v[e]), x0 = f.value(c.v[e]), x1 = f.value(d.v[e]);
+                        s[0][e].mac(y0, x0); s[1][e].mac(y0, x1); s[1][e].mac(y1, x0); s[2][e].mac(y1, x1);
+                        p[0][e].add(y0); p[1][e].add(y1);
+                    }
+                }
+            }
+            Two r[5];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int k = 0; k < 3; ++k) r[k].v[e] = s[k][e].canonical(m);
+                r[3].v[e] = p[0][e].canonical(m); r[4].v[e] = p[1][e].canonical(m);
+            }
+            if (splits > 1) {
+                u64 *const parts = words;
+                __syncthreads(); // all members have been read
+#pragma unroll
+                for (int k = 0; k < 5; ++k) store2(parts + k * L + 2 * threadIdx.x, r[k]);
+                __syncthreads();
+                if (part) continue;
+                for (int q = 1; q < splits; ++q)
+#pragma unroll
+                    for (int k = 0; k < 5; ++k) {
+                        const Two z = load2(parts + k * L + 2 * (threadIdx.x + q * wide));
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) r[k].v[e] = add_mod(r[k].v[e], z.v[e], m.q);
+                    }
+            }
+            u64 *const o = out + (size_t)j * 3 * poly + at, *const os = sum + (size_t)j * 2 * poly + at;
+            store2(o, r[0]); store2(o + poly, r[1]); store2(o + 2 * poly, r[2]);
+            store2(os, r[3]); store2(os + poly, r[4]);
+        }
+    });
+}
 // members c, c + step, ... of token tile c < step share mean and dot, which are read once for a chunk of them.  grid = (N / 512, n, step * chunks)
 __global__ void __launch_bounds__(256, 3) k_grad_input(u64 *out, const u64 *g, const u64 *mean, const u64 *xhat, const u64 *dot, Walk w, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc,
                                                        int N) {

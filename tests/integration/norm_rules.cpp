@@ -18,13 +18,21 @@ int main() {
                 need(chunk * chunks >= members && chunk * (chunks - 1) < members, "chunks hold every member once", members, each, columns);
                 need(columns * chunks <= 65535 || chunk == members, "a grid that reaches them", members, each, columns);
                 if (chunk > 1 && columns * ((members + chunk - 2L) / (chunk - 1)) <= 65535) need(each * columns * chunks >= 148 * 8, "longer chunks only where CTAs are left", members, each, columns);
-                const int log = norm_log_splits(members, each * columns);
-                need(log >= 0 && log <= 3 && (log == 0 || members >= 4 << (log - 1)), "parts of two members at least", members, each, columns);
-                need(log == 0 || (each * columns << (log - 1)) < 148 * 4, "parts only where CTAs are missing", members, each, columns);
+                for (int most : {2, 3}) {
+                    const int log = norm_log_splits(members, each * columns, most);
+                    need(log >= 0 && log <= most && (log == 0 || members >= 4 << (log - 1)), "parts of two members at least", members, each, columns);
+                    need(log == 0 || (each * columns << (log - 1)) < 148 * 4, "parts only where CTAs are missing", members, each, columns);
+                }
             }
     for (int tiles = 1; tiles <= 300; ++tiles) {
         const int some = grad_tiles(tiles), launches = (tiles + some - 1) / some;
         need(some >= 1 && some <= 8 && launches == (tiles + 7) / 8, "as few launches as there can be", tiles, some, launches);
     }
+    for (int tiles = 1; tiles <= 40; ++tiles)
+        for (int batch : {1, 2, 8, 33, 1 << 30}) // a product beyond 32 bits
+            for (bool same : {false, true}) {
+                need(grad_together(tiles, batch, same, 8) == (tiles <= 8 && tiles * (long)batch <= 8), "few CTAs: one kernel only for little work", tiles, batch, same);
+                need(!grad_together(tiles, batch, same, 1 << 20) == (tiles > 8 && !same), "many CTAs: one kernel as long as it takes one launch, or reads nothing twice", tiles, batch, same);
+            }
     return bad != 0;
 }

@@ -36,6 +36,7 @@ def _scale(g, level):
 
 SHAPES = [  # column tiles, token tiles, level
     (1, 1, 3), (2, 1, 0), (3, 2, 5), (4, 3, 2), (5, 1, 1), (6, 4, 3), (7, 5, 2), (8, 1, 8), (9, 2, 1), (12, 3, 3), (13, 2, 2), (1, 17, 1), (33, 1, 2), (2, 40, 1), (130, 1, 0),
+    (4, 1, 3), (6, 1, 2), (7, 1, 4), (4, 2, 1), (2, 4, 3), (1, 8, 2),
 ]
 
 
@@ -154,26 +155,43 @@ def test_scale_many(ring, sizes, edge):
     _check(g, cf, _objects(f, at), at, level, 2, 1)
 
 
-@pytest.mark.parametrize("n_bits", [(58, 58), (50, 50), (44, 60), (43, 60)])
-def test_primes_of_other_lengths(pkg, n_bits):
-    """Scaling primes that leave room for eight products of a sum, and those that go by pieces."""
-    g = pkg.open_gpu(pkg.make_params(log_n=10, max_level=4, dnum=3 if n_bits[0] < 50 else 5, num_special=3, q0_bits=60, q_bits=n_bits[0], p_bits=60, hamming_weight=32))
-    try:
-        level, T, B = 3, 19, 2
-        at = np.arange(g.N)
-        x, mean, r = _rand(g, level, T * B, 1, edge=True), _rand(g, level, B, 2), _rand(g, level, B, 3, edge=True)
-        mean[0] = 0
-        xo, mo, ro = (_objects(v, at) for v in (x, mean, r))
-        cx, cm, cr = (_ct(g, v) for v in (x, mean, r))
-        _check(g, g.norm_squares(cx, T, mean=cm, pad=7), [sum(_pair(xo[t * B + b] - mo[b], xo[t * B + b] - mo[b]) for t in range(T)) - 7 * _pair(mo[b], mo[b]) for b in range(B)], at, level, 3, 2)
-        _check(g, g.norm_scale(cx, cr, T, mean=cm), [_pair(xo[k] - mo[k % B], ro[k % B]) for k in range(T * B)], at, level, 3, 2)
-        rows, rowsum, cols, colsum = g.norm_grad_sums(cx, cx, T)
-        _check(g, rows, [sum(_pair(xo[t * B + b], xo[t * B + b]) for t in range(T)) for b in range(B)], at, level, 3, 2)
-        _check(g, colsum, [sum(xo[t * B + b] for b in range(B)) for t in range(T)], at, level, 2, 1)
+def _all_sums(g, level, T, B, at, check_input=True):
+    x, z, mean, r = _rand(g, level, T * B, 1, edge=True), _rand(g, level, T * B, 4, edge=True), _rand(g, level, B, 2), _rand(g, level, B, 3, edge=True)
+    mean[0] = 0
+    xo, zo, mo, ro = (_objects(v, at) for v in (x, z, mean, r))
+    cx, cz, cm, cr = (_ct(g, v) for v in (x, z, mean, r))
+    _check(g, g.norm_squares(cx, T, mean=cm, pad=7), [sum(_pair(xo[t * B + b] - mo[b], xo[t * B + b] - mo[b]) for t in range(T)) - 7 * _pair(mo[b], mo[b]) for b in range(B)], at, level, 3, 2)
+    _check(g, g.norm_scale(cx, cr, T, mean=cm), [_pair(xo[k] - mo[k % B], ro[k % B]) for k in range(T * B)], at, level, 3, 2)
+    for handle, q in ((None, xo), (cz, zo)):
+        rows, rowsum, cols, colsum = g.norm_grad_sums(cx, cx, T, g=handle)
+        _check(g, rows, [sum(_pair(q[t * B + b], xo[t * B + b]) for t in range(T)) for b in range(B)], at, level, 3, 2)
+        _check(g, rowsum, [sum(q[t * B + b] for t in range(T)) for b in range(B)], at, level, 2, 1)
         _check(g, cols, [sum(_pair(xo[t * B + b], xo[t * B + b]) for b in range(B)) for t in range(T)], at, level, 3, 2)
-        K, nothing = _scale(g, level), 0 * xo[0][:1]
-        _check(g, g.norm_grad_input(cx, cm, cx, cr, T), [np.concatenate([K * (xo[k] - mo[k % B]), nothing]) - _pair(xo[k], ro[k % B]) for k in range(T * B)], at, level, 3, 2)
-        _check(g, g.square_sum_many([cx, cm]), [sum(_pair(v, v) for v in [*xo, *mo])], at, level, 3, 2)
+        _check(g, colsum, [sum(xo[t * B + b] for b in range(B)) for t in range(T)], at, level, 2, 1)
+    K, nothing = _scale(g, level), 0 * xo[0][:1]
+    _check(g, g.norm_grad_input(cx, cm, cx, cr, T), [np.concatenate([K * (xo[k] - mo[k % B]), nothing]) - _pair(xo[k], ro[k % B]) for k in range(T * B)], at, level, 3, 2)
+    _check(g, g.square_sum_many([cx, cm]), [sum(_pair(v, v) for v in [*xo, *mo])], at, level, 3, 2)
+
+
+@pytest.mark.parametrize("n_bits", [58, 50, 45, 44, 43])
+@pytest.mark.parametrize("T,B", [(19, 2), (8, 1), (5, 1), (2, 9)])
+def test_primes_of_other_lengths(pkg, n_bits, T, B):
+    """Scaling primes that leave room for eight products of a sum, and those that go by pieces."""
+    g = pkg.open_gpu(pkg.make_params(log_n=10, max_level=4, dnum=3 if n_bits < 50 else 5, num_special=3, q0_bits=60, q_bits=n_bits, p_bits=60, hamming_weight=32))
+    try:
+        _all_sums(g, 3, T, B, np.arange(g.N))
+    finally:
+        g.close()
+
+
+@pytest.mark.parametrize("n_bits", [50, 44])
+def test_primes_of_other_lengths_in_the_full_ring(pkg, n_bits):
+    """Sums of both directions in one kernel, past every reduction."""
+    g = pkg.open_gpu(pkg.make_params(log_n=16, max_level=3, dnum=3 if n_bits < 50 else 4, num_special=3, q0_bits=60, q_bits=n_bits, p_bits=60, hamming_weight=32))
+    try:
+        at = np.array([0, 1, 127, 128, 511, 512, 40000, 65535])
+        _all_sums(g, 1, 3, 19, at)
+        _all_sums(g, 2, 8, 2, at)
     finally:
         g.close()
 

@@ -7,7 +7,7 @@ from test_gpu_norms import _check, _ct, _objects, _pair, _pt, _rand, _scale
 pytestmark = pytest.mark.gpu
 
 # column tiles, token tiles, level: chunks of two with one left, of eight with one left, of eight without a rest, of one; sums in parts and whole
-SHAPES = [(2, 9, 2), (9, 4, 2), (3, 16, 1), (1, 33, 1), (12, 1, 0), (3, 4, 5), (40, 1, 0)]
+SHAPES = [(2, 9, 2), (9, 4, 2), (3, 16, 1), (1, 33, 1), (12, 1, 0), (3, 4, 5), (40, 1, 0), (6, 2, 3), (7, 2, 3), (5, 2, 2), (8, 2, 2), (4, 9, 2)]
 
 
 @pytest.mark.parametrize("T,B,level", SHAPES)
