@@ -7,6 +7,10 @@
 //   grad sums    rows[b] = sum_t g[t][b] (x) xhat[t][b], cols[t] = sum_b dy[t][b] (x) xhat[t][b], and the plain sums of g and dy over the same indices
 //   grad input   out[t][b] = K (g[t][b] - m[b]) - xhat[t][b] (x) a[b]
 // Sums are exact until one reduction at their end (FpAcc, PieceAcc).
+//
+// All of it is bound by HBM: 3 to 8 products of residues for 32 to 88 bytes, 20 to 60 FP64 instructions where the bytes take 45 to 120 issue slots of a scheduler.  What it takes to be so bound, in the
+// order of what it gave: words of the members ahead in flight while those before are multiplied (registers where every member has a result of its own, rings of asynchronous copies where they are
+// summed, since a sum's registers leave no room), several members a CTA, no quotients by sizes, and addresses of a base that all threads share and a 32-bit offset.
 #pragma once
 #include "kernels.cuh"
 #include <type_traits>
@@ -111,6 +115,9 @@ struct OutList {
 
 // out[b] (+)= the sum over t < groups, for `chunk` token tiles one after the other.  Threads of a CTA: `splits` parts (a power of two) of the members by 512 / splits residues; the
 // parts, which have a chunk of one, are joined in shared memory, in order.  Words come through a ring of members, which every thread fills for itself: of a token tile the mean first, then the members.
+// Level 5, us (floor: the bytes at the copy bandwidth): 3 tiles of 4 token tiles 24 (21), of 16 85 (85), 8 of 16 162 (162), 102 members of a list 97 (100).  Words straight to registers, four
+// members ahead, two CTAs an SM: 31, 107, 188 and 103; rings of five and six stages and two CTAs, which let the sums of two members go without moves: 25.0 and 25.1, 88 and 86, 165 and 162, 99 and 97; four
+// CTAs of 64 registers, which spill: 35, 111, 223 and 196.
 // grid = (N splits / 512, n, chunks): quotients by sizes would take a fifth of the instructions
 struct SquareShape { int groups, batch, chunk, log_splits; u64 pad; };
 constexpr int kSquareStages = 4;
@@ -225,6 +232,7 @@ __global__ void __launch_bounds__(256, 3) k_square_sums(u64 *out, const __grid_c
 // Members c, c + step, ... of a column c < step, `each` of them; a CTA takes a chunk of them one after the other.
 struct Walk { int each, step, chunk; };
 // out[i] = (x[i] - mean[c]) (x) r[c] for the members i = c, c + step, ... of column c < step: mean and factor are read once for a chunk of members.  EACH: a factor per member.
+// Level 5, us (floor): 3 tiles of 4 token tiles 39 (37), of 16 142 (146), 8 of 16 335 (339); 102 members of a list 252 (246).
 // grid = (N / 512, n, step * chunks)
 template <class MEMBERS, class OUT, bool MEAN, bool EACH>
 __global__ void __launch_bounds__(256, 4) k_scale_members(const __grid_constant__ OUT out, const __grid_constant__ MEMBERS x, const u64 *mean, const u64 *r, Walk w, int n, const PrimeConst *__restrict__ pc, int N) {
@@ -274,6 +282,7 @@ __global__ void __launch_bounds__(256, 4) k_scale_members(const __grid_constant_
 constexpr int kNormTiles = 128; // of a launch
 struct AffineList { const u64 *gamma[kNormTiles], *beta[kNormTiles]; int tile0, tiles, batch, chunk; };
 // members of the tiles tile0 ..: out = x gamma + K beta on the first polynomial, x gamma on the second; without gammas x + beta.  A CTA takes a chunk of one tile's members.
+// Level 5, us (floor): 3 tiles of 4 token tiles 28.6 (26), of 16 100 (95), 8 of 16 264 (254).
 // grid = (N / 512, n, tiles * chunks)
 template <bool GAMMA>
 __global__ void __launch_bounds__(256, 4) k_affine(u64 *out, const u64 *x, const __grid_constant__ AffineList a, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc, int N) {
@@ -324,6 +333,9 @@ __global__ void __launch_bounds__(256, 4) k_affine(u64 *out, const u64 *x, const
 }
 // Both directions in one pass over dy, g and xhat.  A thread has one residue of TT column tiles: their sums over b stay in its registers, a word each, the sums over t of one b are written (+= for
 // all but the first tiles of a call).  The words come through a ring of members in shared memory, which every thread fills for itself, several members ahead.  SAME: g is dy.
+// Level 5, us (floor): 3 tiles of 4 token tiles 55 (51), of 16 195 (184), 8 of 16 478 to 498 (427), with g = dy 43 (40), 145 (138), 362 (304).  Sums over b as two words (h, l) a sum, registers for the words
+// ahead: 61, 210 and 943 (spills); as one word, reduced at every product: 57, 201 and 561; with the ring 55, 195 and 480.  Tiles in teams of 128 threads that join their rows in shared memory
+// behind a barrier a token tile: 579 for 8 of 16.  Stages and CTAs an SM by tiles: eight stages of 8 tiles 476, six 490, four 482; 6 tiles four stages and four CTAs 119, six and three 130.
 // grid = (N / 128, n)
 struct GradShape { int batch, tile0; };
 constexpr int grad_stages(int TT) { return TT == 1 || TT == 6 ? 4 : TT == 8 ? 8 : 6; }
@@ -424,7 +436,8 @@ __global__ void __launch_bounds__(128, grad_ctas(TT)) k_grad_sums(u64 *rows, u64
     });
 }
 // One direction: out[j] = sum_i y(i, j) (x) xhat(i, j) and sum[j] = sum_i y(i, j), member (i, j) being i by_i + j by_j, for a chunk of results one after the other.  Parts and the ring as in
-// k_square_sums.  grid = (N splits / 256, n, chunks)
+// k_square_sums.  Both directions, level 5, us (floor of one pass over dy, g and xhat): 12 tiles of 4 token tiles 228 (177), 24 of 2 at level 2 130 (101); six CTAs an SM 221 and 133, and 56 instead of 53
+// for 40 tiles of 4 in a ring with 2^12 coefficients.  grid = (N splits / 256, n, chunks)
 struct PairSumShape { int terms, results, by_i, by_j, chunk, log_splits; };
 constexpr int kPairSumStages = 4, kPairSumLanes = 256;
 constexpr size_t pair_sum_smem() { return (size_t)kPairSumStages * 4 * kPairSumLanes * 8; }
@@ -512,7 +525,8 @@ __global__ void __launch_bounds__(128, 5) k_pair_sums(u64 *out, u64 *sum, const 
         }
     });
 }
-// members c, c + step, ... of token tile c < step share mean and dot, which are read once for a chunk of them.  grid = (N / 512, n, step * chunks)
+// members c, c + step, ... of token tile c < step share mean and dot, which are read once for a chunk of them.  Level 5, us (floor): 3 tiles of 4 token tiles 51 (48), of 16 200 (192), 8 of 16
+// 460 to 485 (462).  grid = (N / 512, n, step * chunks)
 __global__ void __launch_bounds__(256, 3) k_grad_input(u64 *out, const u64 *g, const u64 *mean, const u64 *xhat, const u64 *dot, Walk w, const __grid_constant__ Scalars K, int n, const PrimeConst *__restrict__ pc,
                                                        int N) {
     const int l = blockIdx.y, c = (int)(blockIdx.z % (u32)w.step), first = (int)(blockIdx.z / (u32)w.step) * w.chunk, last = min(first + w.chunk, w.each);
@@ -557,7 +571,8 @@ __global__ void __launch_bounds__(256, 3) k_grad_input(u64 *out, const u64 *g, c
 }
 
 // ---- constants ----
-// out = sum_j k[j] x_j + k0 on the first polynomial of every member, without the constant on the others; a plaintext of a constant would be N words of it.
+// out = sum_j k[j] x_j + k0 on the first polynomial of every member, without the constant on the others; a plaintext of a constant would be N words of it.  32 members of two terms at level 5: 134 us, 4.3 TB/s;
+// the sums of a polynomial have one member a token tile.
 // grid = (N / 512, n, polynomials of all members)
 constexpr int kCombineTerms = 16;
 struct CombineList { const u64 *x[kCombineTerms]; u64 k[kCombineTerms][kMaxPrimes], k0[kMaxPrimes]; int count, np; };
