@@ -497,6 +497,10 @@ class Lib:
         st = (C.c_int64 * n)(*[int(v) for v in steps])
         return self._op("rotate_sum", arr, st, C.c_int(n))
 
+    def rotate_sum_hoisted(self, a, digits, steps):
+        """sum_t rot(a, steps[t]) from the digits of `a`, with one ModDown for the whole sum."""
+        return self._op("rotate_sum_hoisted", a.ptr, digits.ptr, (C.c_int64 * len(steps))(*[int(v) for v in steps]), C.c_int(len(steps)))
+
     def assemble_rot(self, a, s1, p1, s2, p2):
         """rescale(p1 (.) rot(a, s1) + p2 (.) rot(a, s2)) with one division by P * q_level for the sum."""
         return self._op("assemble_rot", a.ptr, C.c_int64(s1), p1.ptr, C.c_int64(s2), p2.ptr)

@@ -289,6 +289,11 @@ class Evaluator {
         check(c_, hb_gen_rot_keys(c_, steps.data(), (int)steps.size()));
         hb_ct *o = nullptr; check(c_, hb_rotate_sum_grouped(c_, x.raw(), steps.data(), (int)steps.size(), &o)); return Ciphertext(c_, o);
     }
+    // sum_t leftRotate(a, steps[t]) with one decomposition and one ModDown
+    Ciphertext rotateSumHoisted(const Ciphertext &a, const Hoisted &h, const std::vector<i64> &steps) const {
+        check(c_, hb_gen_rot_keys(c_, steps.data(), (int)steps.size()));
+        hb_ct *o = nullptr; check(c_, hb_rotate_sum_hoisted(c_, a.raw(), h.raw(), steps.data(), (int)steps.size(), &o)); return Ciphertext(c_, o);
+    }
     // acc += tensor(a, b)
     void tensorAccumulate(Ciphertext &acc, const Ciphertext &a, const Ciphertext &b) const {
         hb_ct *p = acc.release();

@@ -41,22 +41,31 @@ Ciphertext switched(const Evaluator &ev, const Ciphertext &x) { return ev.rescal
 Ciphertext down(const Evaluator &ev, const Ciphertext &x, int level) { return x.getLevel() == level ? ev.view(x, 0, x.getBatch()) : ev.levelDown(x, level); }
 Ciphertext down(const Evaluator &ev, Ciphertext &&x, int level) { return x.getLevel() == level ? std::move(x) : ev.levelDown(x, level); }
 
+// the sum of x rotated by 0, step, ... (count - 1) step, count a power of two: four terms at a time with one decomposition and one ModDown
+Ciphertext sum_rotations(const Evaluator &ev, Ciphertext x, i64 step, i64 count) {
+    while (count > 1) {
+        const i64 some = count >= 4 ? 4 : 2;
+        std::vector<i64> steps;
+        for (i64 k = 0; k < some; ++k) steps.push_back(k * step);
+        x = ev.rotateSumHoisted(x, ev.decompose(x), steps);
+        step *= some; count /= some;
+    }
+    return x;
+}
 // `scale` times the sum over a row (and `other` times the first column of y), in all its columns; one level
 Ciphertext row_mean(HEMMer &h, Ciphertext x, const TileTensorShape &s, double scale, const Ciphertext *y = nullptr, double other = 0.0) {
     const Evaluator &ev = h.eval();
-    for (i64 i = 1; i < s.getBlockWidth(); i <<= 1) x = ev.add(x, ev.leftRotate(x, i));
+    x = sum_rotations(ev, std::move(x), 1, s.getBlockWidth());
     const Plaintext mask = norm_mask(h, sched::kNormFirstCol, s, scale, x.getLevel());
     if (y) {
         const Plaintext second = norm_mask(h, sched::kNormFirstCol, s, other, x.getLevel());
         x = ev.multSumRescaledOnce({&x, y}, {&mask, &second});
     } else x = ev.mult(x, mask);
-    for (i64 i = 1; i < s.getBlockWidth(); i <<= 1) x = ev.add(x, ev.rightRotate(x, i));
-    return x;
+    return sum_rotations(ev, std::move(x), -1, s.getBlockWidth());
 }
 // the sum over all slots that are a multiple of `step` apart, in each of them
 Ciphertext sum_slots(const HEMMer &h, Ciphertext x, i64 step) {
-    for (i64 i = step; i < h.slots(); i <<= 1) x = h.eval().add(x, h.eval().leftRotate(x, i));
-    return x;
+    return sum_rotations(h.eval(), std::move(x), step, h.slots() / step);
 }
 
 struct NormShape { TileTensorShape s; int groups, batch; i64 columns, pad; };

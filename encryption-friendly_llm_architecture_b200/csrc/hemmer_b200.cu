@@ -2555,6 +2555,17 @@ int hb_rotate_sum_grouped(hb_ctx *c, const hb_ct *x, const int64_t *steps, int g
         *out = rotate_sum_core(c, base.data(), steps, groups, level, batch, x->spow, dt.p, dt_stride);
     });
 }
+// the same when every term is a rotation of one ciphertext, whose digits are there
+int hb_rotate_sum_hoisted(hb_ctx *c, const hb_ct *a, const hb_digits *dg, const int64_t *steps, int count, hb_ct **out) {
+    return guard(c, [&] {
+        if (!a || !dg || !steps || !out) fail(HB_E_ARG, "rotate_sum_hoisted: null argument");
+        if (count < 1 || count > 32) fail(HB_E_LIMIT, "rotate_sum: 1 to 32 terms");
+        own(c, a); own(c, dg);
+        if (a->np != 2 || dg->level != a->level || dg->batch != a->batch) fail(HB_E_SHAPE, "rotate_sum_hoisted: digits do not belong to this ciphertext");
+        const std::vector<const u64 *> base((size_t)count, a->d);
+        *out = rotate_sum_core(c, base.data(), steps, count, a->level, a->batch, a->spow, dg->d, 0);
+    });
+}
 int hb_rotate(hb_ctx *c, const hb_ct *a, int64_t steps, hb_ct **out) { return guard(c, [&] { *out = do_galois(c, a, c->h->galois_rot(steps)); }); }
 int hb_conjugate(hb_ctx *c, const hb_ct *a, hb_ct **out) { return guard(c, [&] { *out = do_galois(c, a, c->h->galois_conj()); }); }
 int hb_ntt(hb_ctx *c, hb_ct *a, int inverse) { return guard(c, [&] { own(c, a); ntt_inplace(c, a->d, (int)a->limbs(), c->qmap(a->level), inverse != 0); }); }

@@ -8,7 +8,7 @@
 //   grad input   out[t][b] = K (g[t][b] - m[b]) - xhat[t][b] (x) a[b]
 // Sums are exact until one reduction at their end (FpAcc, PieceAcc).
 //
-// All of it is bound by HBM: 3 to 8 products of residues for 32 to 88 bytes, 20 to 60 FP64 instructions where the bytes take 45 to 120 issue slots of a scheduler.  What it takes to be so bound, in the
+// All of it is bound by HBM: a member's 18 to 58 FP64 instructions keep the pipes of an SM for 9 to 29 cycles a warp, its bytes take 22 to 77.  What it takes to be so bound, in the
 // order of what it gave: words of the members ahead in flight while those before are multiplied (registers where every member has a result of its own, rings of asynchronous copies where they are
 // summed, since a sum's registers leave no room), several members a CTA, no quotients by sizes, and addresses of a base that all threads share and a 32-bit offset.
 #pragma once

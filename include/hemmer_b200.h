@@ -225,6 +225,8 @@ int hb_rotate_sum(hb_ctx *ctx, const hb_ct *const *xs, const int64_t *left_steps
 /* The same when the terms are the member groups of ONE ciphertext (group t = members t * batch / groups onwards): the
  * digits of all groups are lifted by one batched call.  out has batch / groups members. */
 int hb_rotate_sum_grouped(hb_ctx *ctx, const hb_ct *x, const int64_t *left_steps, int groups, hb_ct **out);
+/* The same when every term is a rotation of one ciphertext `a`, with its digits from hb_decompose: residues of hb_rotate_sum of that many times `a`. */
+int hb_rotate_sum_hoisted(hb_ctx *ctx, const hb_ct *a, const hb_digits *digits, const int64_t *left_steps, int count, hb_ct **out);
 /* The masked pair of rotations that makes one wrapped copy in the shift loops (MatrixUtils.cpp:1416-1427:
  * two leftRotate, two multWithoutRescale, add, rescale) as one operation:
  *     out = p1 (.) rot(a, s1) + p2 (.) rot(a, s2),   at level(a) - 1.

@@ -250,6 +250,67 @@ def test_constants_that_are_refused(pkg, gpu_small, gpu_mid):
     assert g._fn("add_const")(g.ctx, None, C.c_double(0.0), C.byref(C.c_void_p())) == -1
 
 
+@pytest.mark.parametrize("members", [1, 3, 5])
+@pytest.mark.parametrize("steps", [[0], [5], [0, 1, 2, 3], [-1, -2, -3, 0], [7, 7, 0], list(range(1, 17)) + [0]])
+def test_sums_of_rotations_of_one_ciphertext(pkg, gpu_small, members, steps):
+    g = gpu_small
+    x = _ct(g, _rand(g, 4, members, 1))
+    g.gen_rot_keys(steps)
+    digits = g.decompose(x)
+    if sum(s == 0 for s in steps) <= 16 and len(steps) <= 32:
+        assert np.array_equal(g.ct_export(g.rotate_sum_hoisted(x, digits, steps)), g.ct_export(g.rotate_sum([x] * len(steps), steps)))
+    with pytest.raises(pkg.HBError):   # digits of another ciphertext
+        g.rotate_sum_hoisted(_ct(g, _rand(g, 3, members, 1)), digits, steps)
+    with pytest.raises(pkg.HBError):
+        g.rotate_sum_hoisted(x, digits, [])
+    with pytest.raises(pkg.HBError):
+        g.rotate_sum_hoisted(x, digits, [1] * 17)
+
+
+def _device(handle, shape):
+    import torch
+    ptr = handle.lib._fn("ct_device_ptr")
+    ptr.restype = C.c_void_p
+
+    class View:
+        __cuda_array_interface__ = {"shape": shape, "typestr": "<i8", "data": (ptr(handle.ptr), False), "version": 3, "strides": None}
+
+    return torch.as_tensor(View(), device="cuda")
+
+
+def test_more_members_than_a_grid_has_rows(pkg, gpu_small):
+    """70000 token tiles of one column tile: past 65535 the sums take more of them a CTA, and calls that go member by member are refused."""
+    import torch
+    g, B, q = gpu_small, 70000, int(gpu_small.primes[0])
+    x, m = g.ct_create(0, 2, B), g.ct_create(0, 2, B)
+    for k, h in enumerate((x, m)):
+        _device(h, (B, 2, 1, g.N)).random_(0, q, generator=torch.Generator(device="cuda").manual_seed(k))
+    torch.cuda.synchronize()
+    at, some = np.array([0, 1, 511, 512, g.N - 1]), [0, 1, 65534, 65535, 65536, B - 1]
+    xo, mo = ({b: g.ct_export(g.batch_slice(h, b, 1))[0][..., at].astype(object) for b in some} for h in (x, m))
+
+    def same(handle, want, polys):
+        assert g.ct_meta(handle)[1:3] == (polys, B)
+        for b in some:
+            assert np.array_equal(g.ct_export(g.batch_slice(handle, b, 1))[0][..., at].astype(object), want(b) % q)
+
+    same(g.norm_squares(x, 1, mean=m), lambda b: _pair(xo[b] - mo[b], xo[b] - mo[b]), 3)
+    p = _rand(g, 0, 1, 5, polys=1)[0, 0]
+    pt, po = _pt(g, p), p[..., at].astype(object)
+    same(g.norm_affine(x, 1, gamma=[pt]), lambda b: np.stack([xo[b][0] * po, xo[b][1] * po]), 2)
+    rows, rowsum, cols, colsum = g.norm_grad_sums(x, m, 1)
+    same(rows, lambda b: _pair(xo[b], mo[b]), 3)
+    same(rowsum, lambda b: xo[b], 2)
+    want = (_device(x, (B, 2, 1, g.N))[:, 0, 0, at].cpu().numpy().astype(object).sum(0)) % q
+    assert np.array_equal(g.ct_export(colsum)[0, 0, 0, at].astype(object), want)
+    for call in (lambda: g.norm_scale(x, m, 1), lambda: g.norm_grad_input(x, m, x, m, 1), lambda: g.add_const(x, 1.0)):
+        with pytest.raises(pkg.HBError) as e:
+            call()
+        assert e.value.code == -9
+    del x, m, rows, rowsum, cols, colsum
+    g._chk(g._fn("release_cached")(g.ctx))
+
+
 def test_views_and_whole_calls_of_the_library_agree(gpu_small):
     """Runs of members without a copy as operands, and the residues of hb_tensor, hb_sub and hb_add."""
     g = gpu_small
