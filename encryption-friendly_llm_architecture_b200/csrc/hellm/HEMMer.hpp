@@ -150,11 +150,11 @@ class HEMMer {
     // imaginary part).  One member per vector and column tile: y / 2 is the sum of the real parts of the halves, the same in every row, one level lower.
     CtxtTensor vecMatMul4(const CtxtTensor &x, const hb_qweight *w);
     // Layer norm over rows that reach across the column tiles of x (members [column tile][token tile]; `columns` of them in all, the last tile may end early, with zeros behind): with mean and variance of
-    // a row, xhat = (x - mean) rstd and y = xhat gamma + beta (NULL: ones, zeros).  rstd is a polynomial of `degree` for 1 / sqrt(variance + eps), right where that lies in [lo, hi] (rows of padding
-    // have a variance of their own and come out as some finite multiple of zero, plus beta).  Takes 4 + polynomialDepth(degree) levels, one more with gamma or a tile that ends early; xhat and rstd are
+    // a row, xhat = (x - mean) rstd and y = xhat gamma + beta (NULL: ones, zeros).  rstd is a polynomial of `degree` for 1 / sqrt(variance + eps), right where that lies in [lo, hi].  Rows of padding,
+    // all zeros, lie outside: `tokens` says how many rows of every token tile are none (NULL: all), the others come out as beta.  Takes 4 + polynomialDepth(degree) levels, one more with gamma or a tile that ends early; xhat and rstd are
     // what the gradients need, one and two levels above y.
     struct LayerNorm { CtxtTensor y, xhat, rstd; };
-    LayerNorm layerNorm(const CtxtTensor &x, int groups, i64 columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree);
+    LayerNorm layerNorm(const CtxtTensor &x, int groups, i64 columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree, const int32_t *tokens = nullptr);
     // Its gradients: dx, and dgamma and dbeta summed over all rows and token tiles (one member per column tile, the same in every row).
     struct LayerNormGrads { CtxtTensor dx, dgamma, dbeta; };
     LayerNormGrads layerNormBackward(const CtxtTensor &dy, const CtxtTensor &xhat, const CtxtTensor &rstd, int groups, i64 columns, const double *gamma);

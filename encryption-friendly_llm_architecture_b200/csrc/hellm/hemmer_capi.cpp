@@ -237,11 +237,11 @@ int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct
     });
 }
 int hb_hemmer_layer_norm(hb_hemmer *h, const hb_ct *x, SHAPE_ARGS, int groups, int columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree,
-                         hb_ct **y, hb_ct **xhat, hb_ct **rstd) {
+                         const int32_t *tokens, hb_ct **y, hb_ct **xhat, hb_ct **rstd) {
     return guard([&] {
         if (!x || !y || !xhat || !rstd) throw std::invalid_argument("[layerNorm] null argument");
         IN_TENSOR(t, x);
-        HEMMer::LayerNorm r = h->h.layerNorm(t, groups, columns, gamma, beta, eps, lo, hi, degree);
+        HEMMer::LayerNorm r = h->h.layerNorm(t, groups, columns, gamma, beta, eps, lo, hi, degree, tokens);
         *y = r.y.get().release(); *xhat = r.xhat.get().release(); *rstd = r.rstd.get().release();
     });
 }

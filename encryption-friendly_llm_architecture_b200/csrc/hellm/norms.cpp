@@ -188,8 +188,13 @@ std::vector<double> HEMMer::clipPolynomial(double max_norm, double bound, int de
 }
 int HEMMer::polynomialDepth(int degree) { return chebyshev_depth(degree); }
 
-HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree) {
+HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree, const int32_t *tokens) {
     const NormShape n = norm_shape(*this, x, groups, columns, "layerNorm");
+    bool padded = false;
+    for (int b = 0; tokens && b < n.batch; ++b) {
+        if (tokens[b] < 0 || tokens[b] > n.s.getNumRows()) throw std::invalid_argument("[layerNorm] a token tile has 0 to all of its rows");
+        padded = padded || tokens[b] < n.s.getNumRows();
+    }
     const std::vector<double> c = inverseRootPolynomial(lo, hi, degree);
     if (!(eps >= 0.0) || !std::isfinite(eps)) throw std::invalid_argument("[layerNorm] eps from 0");
     for (const double *v : {gamma, beta})
@@ -208,7 +213,17 @@ HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns
             const Ciphertext s = switched(ev, ev.concat(both)), of_mean = ev.group(s, 1, 2);
             row = row_mean(*this, ev.group(s, 0, 2), n.s, scale, &of_mean, -scale * (double)n.pad);
         } else row = row_mean(*this, switched(ev, squares), n.s, scale);
-        u = ev.addConstant(row, (2.0 * eps - hi - lo) / (hi - lo)); // the variance's place in [-1, 1]
+        const double zero = (2.0 * eps - hi - lo) / (hi - lo); // where a variance of nothing has its place
+        u = ev.addConstant(row, zero); // the variance's place in [-1, 1]
+        if (padded) { // rows of padding, all zeros, are moved to the middle of the range: where the polynomial is large, their noise would come out as values, or spoil all slots
+            std::vector<Plaintext> p;
+            for (int b = 0; b < n.batch; ++b) {
+                Message m((size_t)slots_);
+                std::fill(m.re.begin() + tokens[b] * n.s.getBlockWidth(), m.re.end(), -zero);
+                p.push_back(eval_.encode(m, u.getLevel()));
+            }
+            u = ev.normAffine(u, {}, pointers(p));
+        }
     }
     Ciphertext rstd = evaluate(eval_, u, c);
     const int level = rstd.getLevel();

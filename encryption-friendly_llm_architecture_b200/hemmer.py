@@ -392,10 +392,16 @@ class Hemmer:
             raise HBError(rc, f().decode())
         return out, depth.value
 
-    def layer_norm(self, x, columns, var_range, groups=1, gamma=None, beta=None, eps=1e-5, degree=15):
-        """(y, xhat, rstd) of rows of `columns` values over `groups` column tiles; var_range: where variance + eps lies."""
+    def layer_norm(self, x, columns, var_range, groups=1, gamma=None, beta=None, eps=1e-5, degree=15, tokens=None):
+        """(y, xhat, rstd) of rows of `columns` values over `groups` column tiles; var_range: where variance + eps lies; tokens: the rows of every token tile that are not
+        padding (None: all)."""
+        if tokens is not None:
+            members, tokens = self.lib.ct_meta(x.ct)[2], [_i32(t) for t in tokens]
+            if groups < 1 or len(tokens) * groups != members:
+                raise ValueError(f"{members} members of {groups} column tiles, tokens of {len(tokens)} token tiles")
+            tokens = (C.c_int32 * len(tokens))(*tokens)
         (_g, pg), (_b, pb) = self._columns(gamma, columns), self._columns(beta, columns)
-        outs = self._call("layer_norm", x.ct.ptr, *self._shp(x), _i32(groups), _i32(columns), pg, pb, C.c_double(eps), C.c_double(var_range[0]), C.c_double(var_range[1]), _i32(degree), n_out=3)
+        outs = self._call("layer_norm", x.ct.ptr, *self._shp(x), _i32(groups), _i32(columns), pg, pb, C.c_double(eps), C.c_double(var_range[0]), C.c_double(var_range[1]), _i32(degree), tokens, n_out=3)
         return tuple(CtxtTensor(o, *x.shape) for o in outs)
 
     def layer_norm_backward(self, dy, xhat, rstd, columns, groups=1, gamma=None):

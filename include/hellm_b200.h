@@ -154,16 +154,17 @@ int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct
 /* Layer norm and its gradients over rows that reach across `groups` column tiles (members [column tile][token tile], tiles whose rows fill the slots); `columns`
  * in all, the last tile may end early.  gamma, beta: `columns` doubles on the host, or NULL.  y = xhat gamma + beta with xhat = (x - mean) rstd; rstd is the polynomial of `degree`
  * (1 to 63) that stands for 1 / sqrt(variance + eps) on [lo, hi].  x needs 4 levels, those of the polynomial (hb_hemmer_polynomial), and one for gamma or a tile that
- * ends early.  Outside [lo, hi], as in rows of padding, the polynomial's value is what it is: finite, but no root.  Columns past the width have to be zero in x and dy and come out as zeros in y, dx, dgamma and dbeta;
+ * ends early.  Outside [lo, hi] the polynomial soon grows beyond all bounds, and a slot beyond the modulus spoils all of them, so rows of padding
+ * (all zeros) have to be named: `tokens` has the number of rows in front of them for every token tile (NULL: all rows), and they come out as beta.  Columns past the width have to be zero in x and dy and come out as zeros in y, dx, dgamma and dbeta;
  * in xhat they are not.  dy may be of another level than xhat; dgamma and dbeta have one member per column tile, summed over all rows and token tiles, in every row.  Plaintexts are encoded from
- * the host at every call that has gamma or beta, which cannot be recorded then.  No counterparts in the reference's HEMMer: its LayerNorm class does the like with other polynomials. */
+ * the host at every call that has gamma, beta or padding, which cannot be recorded then.  No counterparts in the reference's HEMMer: its LayerNorm class does the like with other polynomials. */
 int hb_hemmer_layer_norm(hb_hemmer *h, const hb_ct *x, int rows, int cols, int width, int groups, int columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree,
-                         hb_ct **y, hb_ct **xhat, hb_ct **rstd);
+                         const int32_t *tokens, hb_ct **y, hb_ct **xhat, hb_ct **rstd);
 int hb_hemmer_layer_norm_backward(hb_hemmer *h, const hb_ct *dy, const hb_ct *xhat, const hb_ct *rstd, int rows, int cols, int width, int groups, int columns, const double *gamma, hb_ct **dx,
                                   hb_ct **dgamma, hb_ct **dbeta);
 /* The square of the global norm of the gradients, over all slots of all members of all handles (imaginary parts have to be zero), in every slot, one level below the lowest of them; and all of
  * them times min(1, max_norm / norm): a polynomial of `degree` in the square of the norm, right up to norms of `bound` > max_norm, which a degree of 15 meets to 0.05 for bound = 4 max_norm.  3 levels and those of the
- * polynomial; outs receives a handle per gradient, norm_squared (may be NULL) the square. */
+ * polynomial; outs receives a handle per gradient, norm_squared (may be NULL) the square.  Beyond `bound` the polynomial is no root and soon grows beyond all bounds: decrypted, norm_squared tells. */
 int hb_hemmer_grad_norm_squared(hb_hemmer *h, const hb_ct *const *grads, int count, hb_ct **out);
 int hb_hemmer_clip_grad_norm(hb_hemmer *h, const hb_ct *const *grads, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared);
 /* Those polynomials: which = 0 for 1 / sqrt over [a, b], 1 for min(1, a / sqrt) over [0, b^2], as degree + 1 coefficients of T_j(u), u the place of the argument in [-1, 1].  depth (may be NULL):

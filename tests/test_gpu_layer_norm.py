@@ -118,8 +118,35 @@ def test_forward_and_backward(deep, T, B, D, degree, weights):
         assert abs(_whole(got, D)[b, row, col] - want) < TOL + 4 * rel * slack + 1e-6
 
 
-def test_rows_of_padding(deep):
-    """Rows without tokens: variance 0 lies outside the range of the polynomial, whose value there is finite; the product with the row's zeros is zero, and what comes out is beta."""
+@pytest.mark.parametrize("lo,hi,degree", [(0.1, 1.3, 7), (0.2, 1.2, 15), (0.2, 0.9, 31), (0.25, 0.75, 31)])
+@pytest.mark.parametrize("tokens", [(5, 0), (16, 0), (0, 0), (1, 15)])
+def test_rows_that_are_named_as_padding(deep, lo, hi, degree, tokens):
+    """Ranges so narrow that the polynomial's terms at a variance of 0 reach 26 to 10^17: the padded rows come out as beta all the same, and the tokens beside them as ever."""
+    h, T, B, D, w, rows = deep, 2, 2, 50, 32, 16
+    rng = np.random.default_rng(degree)
+    x, dy, gamma, beta = rng.uniform(-1, 1, (B, rows, D)), rng.uniform(-1, 1, (B, rows, D)), rng.uniform(0.5, 1.5, D), rng.uniform(-1, 1, D)
+    x *= np.sqrt(rng.uniform(lo + 0.05, hi - 0.05, (B, rows, 1))) / x.std(-1, keepdims=True)
+    x += rng.uniform(-0.5, 0.5, (B, rows, 1))
+    for b, n in enumerate(tokens):
+        x[b, n:], dy[b, n:] = 0.0, 0.0
+    c, _ = h.polynomial("rsqrt", lo, hi, degree)
+    y0, xhat0, r0 = _model(x, gamma, beta, 1e-3, (lo, hi), c)
+    for b, n in enumerate(tokens):
+        y0[b, n:], xhat0[b, n:], r0[b, n:] = beta, 0.0, chebyshev.chebval(0.0, c)
+    y, xhat, rstd = h.layer_norm(_encrypt(h, _tiles(x, T, w)), D, (lo, hi), groups=T, gamma=gamma, beta=beta, eps=1e-3, degree=degree, tokens=tokens)
+    assert np.abs(_whole(_decrypt(h, y, T, B), D) - y0).max() < TOL
+    assert np.abs(_whole(_decrypt(h, xhat, T, B), D) - xhat0).max() < TOL
+    assert np.abs(_decrypt(h, rstd, 1, B)[0] - r0).max() < TOL
+    if degree == 7:
+        g = dy * gamma
+        dx0 = r0 * (g - g.mean(-1, keepdims=True) - xhat0 * (g * xhat0).mean(-1, keepdims=True))
+        dx, dgamma, dbeta = h.layer_norm_backward(_encrypt(h, _tiles(dy, T, w), seed=3), xhat, rstd, D, groups=T, gamma=gamma)
+        assert np.abs(_whole(_decrypt(h, dx, T, B), D) - dx0).max() < TOL
+        assert np.abs(_whole(_decrypt(h, dgamma, T, 1), D) - (dy * xhat0).sum((0, 1))).max() < B * rows * TOL / 8
+
+
+def test_rows_of_padding_that_are_not_named(deep):
+    """In a wide range the polynomial's value at variance 0 is small; the product with the row's zeros is zero, and what comes out is beta."""
     h, T, B, D, w, rows = deep, 2, 2, 50, 32, 16
     rng = np.random.default_rng(5)
     x, dy, gamma, beta = _data(rng, B, rows, D), rng.uniform(-1, 1, (B, rows, D)), rng.uniform(0.5, 1.5, D), rng.uniform(-1, 1, D)
@@ -134,6 +161,31 @@ def test_rows_of_padding(deep):
     assert np.abs(_whole(_decrypt(h, dx, T, B), D)[1]).max() < TOL
     assert np.abs(_whole(_decrypt(h, dgamma, T, 1), D) - (dy * xhat0).sum((0, 1))).max() < B * rows * TOL / 8
     assert np.abs(_whole(_decrypt(h, dbeta, T, 1), D) - dy.sum((0, 1))).max() < B * rows * TOL / 8
+
+
+@pytest.mark.parametrize("D,weights", [(64, False), (64, True), (50, False)])
+def test_the_last_levels(deep, D, weights):
+    """From the lowest level that is let through down to level 0, and one level less is refused."""
+    h, T, B, w, rows = deep, 2, 1, 32, 16
+    rng = np.random.default_rng(8)
+    x, dy = _data(rng, B, rows, D), rng.uniform(-1, 1, (B, rows, D))
+    gamma = rng.uniform(0.5, 1.5, D) if weights else None
+    g1 = gamma if weights else np.ones(D)
+    c, depth = h.polynomial("rsqrt", *RANGE, 3)
+    least = 4 + depth + (weights or D < 64)
+    y0, xhat0, r0 = _model(x, g1, 0.0, 1e-3, RANGE, c)
+    y, xhat, rstd = h.layer_norm(_encrypt(h, _tiles(x, T, w), least), D, RANGE, groups=T, gamma=gamma, eps=1e-3, degree=3)
+    assert h.lib.ct_meta(y.ct)[0] == 0 and np.abs(_whole(_decrypt(h, y, T, B), D) - y0).max() < TOL
+    with pytest.raises(Exception):
+        h.layer_norm(_encrypt(h, _tiles(x, T, w), least - 1), D, RANGE, groups=T, gamma=gamma, eps=1e-3, degree=3)
+    low = 4 + (weights or D < 64) + (D < 64)
+    e_x, e_r = _encrypt(h, _tiles(xhat0, T, w), low, seed=5), _encrypt(h, np.broadcast_to(r0, (B, rows, w))[None].copy(), low, seed=6)
+    dx, _, _ = h.layer_norm_backward(_encrypt(h, _tiles(dy, T, w), low, seed=4), e_x, e_r, D, groups=T, gamma=gamma)
+    g = dy * g1
+    dx0 = r0 * (g - g.mean(-1, keepdims=True) - xhat0 * (g * xhat0).mean(-1, keepdims=True))
+    assert h.lib.ct_meta(dx.ct)[0] == 0 and np.abs(_whole(_decrypt(h, dx, T, B), D) - dx0).max() < TOL
+    with pytest.raises(Exception):
+        h.layer_norm_backward(_encrypt(h, _tiles(dy, T, w), low - 1, seed=4), e_x, e_r, D, groups=T, gamma=gamma)
 
 
 @pytest.mark.parametrize("dy_level,r_down", [(16, 0), (9, 0), (7, 0), (16, 4), (7, 5)])
@@ -291,6 +343,11 @@ def test_refusals(pkg, deep):
     for degree in (0, -3, 64):
         refused(h.layer_norm, x, 64, RANGE, groups=2, degree=degree)
         refused(h.clip_grad_norm, [x], 1.0, 2.0, degree)
+    refused(h.layer_norm, x, 64, RANGE, groups=2, tokens=[17])
+    refused(h.layer_norm, x, 64, RANGE, groups=2, tokens=[-1])
+    for tokens in ([], [1, 2]):
+        with pytest.raises(ValueError):
+            h.layer_norm(x, 64, RANGE, groups=2, tokens=tokens)
     refused(h.layer_norm, x, 64, RANGE, groups=2, eps=-1.0)
     refused(h.layer_norm, x, 64, RANGE, groups=2, eps=float("nan"))
     refused(h.layer_norm, x, 64, RANGE, groups=2, gamma=np.full(64, np.inf))
@@ -310,7 +367,7 @@ def test_refusals(pkg, deep):
     null = (C.c_void_p * 2)()
     assert h._fn("grad_norm_squared")(h.h, null, 2, C.byref(C.c_void_p())) == -1
     assert h._fn("clip_grad_norm")(h.h, null, 2, C.c_double(1.0), C.c_double(2.0), 7, null, None) == -1
-    assert h._fn("layer_norm")(h.h, x.ct.ptr, 16, 32, 32, 2, 64, None, None, C.c_double(0.0), C.c_double(0.1), C.c_double(1.0), 7, None, None, None) == -1
+    assert h._fn("layer_norm")(h.h, x.ct.ptr, 16, 32, 32, 2, 64, None, None, C.c_double(0.0), C.c_double(0.1), C.c_double(1.0), 7, None, None, None, None) == -1
 
 
 def test_the_full_ring(pkg, gpu_full):

@@ -79,7 +79,11 @@ def test_lists_of_another_length(pkg):
         lib.norm_affine(x, 2 ** 31, gamma=[x])
     h = object.__new__(pkg.Hemmer)
     h._call = lambda *a, **k: pytest.fail("reached the library")
+    h.lib = SimpleNamespace(ct_meta=lambda ct: (3, 2, 6, 1))
     t = pkg.CtxtTensor(x, 16, 16, 32)
+    for tokens in ([], [1, 2], [1, 2, 3, 4], [2 ** 31] * 3):
+        with pytest.raises(ValueError):
+            h.layer_norm(t, 40, (1.0, 2.0), groups=2, tokens=tokens)
     for gamma in (np.ones(39), np.ones(41), np.ones((40, 1)), 1.0):
         with pytest.raises(ValueError):
             h.layer_norm(t, 40, (1.0, 2.0), groups=2, gamma=gamma)
