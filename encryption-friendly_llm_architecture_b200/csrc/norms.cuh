@@ -353,9 +353,10 @@ __global__ void __launch_bounds__(128, grad_ctas(TT)) k_grad_sums(u64 *rows, u64
     const u32 ring = smem_u32(words + threadIdx.x);
     auto fetch = [&](int t, int b, u32 to) {
         const size_t i = (size_t)(w.tile0 + t) * per_tile + (size_t)b * 2 * poly;
-        cp_async8(to, xhat + i + at); cp_async8(to + 1024, xhat + i + poly + at);
-        cp_async8(to + 2048, dy + i + at); cp_async8(to + 3072, dy + i + poly + at);
-        if (!SAME) { cp_async8(to + 4096, g + i + at); cp_async8(to + 5120, g + i + poly + at); }
+        constexpr u32 line = 128 * 8;
+        cp_async8(to, xhat + i + at); cp_async8(to + line, xhat + i + poly + at);
+        cp_async8(to + 2 * line, dy + i + at); cp_async8(to + 3 * line, dy + i + poly + at);
+        if (!SAME) { cp_async8(to + 4 * line, g + i + at); cp_async8(to + 5 * line, g + i + poly + at); }
     };
     pdl_wait();
 #pragma unroll
