@@ -353,6 +353,36 @@ def test_replayed_from_a_graph(gpu_small):
         assert np.array_equal(g.ct_export(o), w)
 
 
+def test_two_contexts_at_once(pkg, gpu_small):
+    """Calls of two contexts from two threads, each on its own stream, while the other's are under way."""
+    import threading
+    other = pkg.open_gpu(pkg.make_params(log_n=12, max_level=8, dnum=3, num_special=3, hamming_weight=64))
+    try:
+        jobs, wrong = [], []
+        for g, T, B in ((gpu_small, 5, 3), (other, 12, 4)):
+            x, y, m, r = (_ct(g, _rand(g, 3, n, s)) for s, n in enumerate((T * B, T * B, B, B)))
+
+            def calls(g=g, T=T, x=x, y=y, m=m, r=r):
+                outs = [g.norm_squares(x, T, mean=m), g.norm_scale(x, r, T, mean=m), *g.norm_grad_sums(x, y, T), g.norm_grad_input(x, m, y, r, T), g.square_sum_many([x, y]), *g.scale_many([x, m], g.batch_slice(r, 0, 1))]
+                return [g.ct_export(o) for o in outs]
+
+            jobs.append((calls, calls()))
+
+        def work(calls, want):
+            for _ in range(20):
+                if not all(np.array_equal(a, b) for a, b in zip(calls(), want)):
+                    wrong.append(calls)
+
+        threads = [threading.Thread(target=work, args=job) for job in jobs]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong
+    finally:
+        other.close()
+
+
 def test_refusals(pkg, gpu_small, gpu_mid):
     g, level, T, B = gpu_small, 3, 2, 2
     x, m, f = _ct(g, _rand(g, level, T * B, 1)), _ct(g, _rand(g, level, B, 2)), _ct(g, _rand(g, level, 1, 3))
