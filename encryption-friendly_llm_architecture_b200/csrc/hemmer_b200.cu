@@ -1313,8 +1313,9 @@ void do_scale_many(hb_ctx *c, const hb_ct *const *xs, int count, const hb_ct *fa
     OutList to;
     int some = 0;
     auto flush = [&] {
+        if (!some) return; // the launch before was full
         const Walk w = walk(c, some, 1, n);
-        if (some) launch(c, k_scale_members<MemberList, OutList, false, false>, walk_grid(c, w, n, "scale_many"), 256, 0, to, list, nullptr, factor->d, w, n, c->pc, N);
+        launch(c, k_scale_members<MemberList, OutList, false, false>, walk_grid(c, w, n, "scale_many"), 256, 0, to, list, nullptr, factor->d, w, n, c->pc, N);
         some = 0;
     };
     ALG(c, factor->limbs());

@@ -146,7 +146,7 @@ constexpr int pair_ranges(PairBlock b, int N, int nr, int nc, int heads, int lim
 // them.  `each`: CTAs with one chunk for all members of a column; `columns` of them.  Calls at level 5, us, one member a CTA / this: products with one factor 3 tiles of 4 token tiles 50 / 39,
 // of 16 193 / 142, 8 of 16 507 / 336; gradients of the input 68 / 52, 273 / 203, 723 / 485; squares 26 / 24, 93 / 86, 165 / 164.
 constexpr int norm_chunk(int members, long each, long columns) {
-    int chunk = members < 8 ? members : 8;
+    int chunk = members < 1 ? 1 : members < 8 ? members : 8;
     while (chunk > 1 && each * columns * ((members + chunk - 1) / chunk) < 148 * 8) --chunk;
     while (columns * ((members + chunk - 1L) / chunk) > 65535 && chunk < members) ++chunk;
     return chunk;
