@@ -114,6 +114,14 @@ class Evaluator {
   public:
     explicit Evaluator(hb_ctx *c) : c_(c) {}
     hb_ctx *ctx() const { return c_; }
+    // scale of a level: what 1 is in whole numbers
+    double scale(int level) const {
+        int top = 0;
+        check(c_, hb_ctx_dims(c_, nullptr, &top, nullptr));
+        std::vector<double> v((size_t)top + 1);
+        check(c_, hb_ctx_info(c_, nullptr, v.data()));
+        return v.at((size_t)level);
+    }
 
     Plaintext encode(const Message &m, int level) const {
         hb_pt *p = nullptr; check(c_, hb_encode(c_, m.re.data(), m.im.data(), m.size(), level, &p)); return Plaintext(p);

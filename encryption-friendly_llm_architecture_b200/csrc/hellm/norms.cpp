@@ -294,14 +294,24 @@ Ciphertext HEMMer::gradNormSquared(const std::vector<const Ciphertext *> &grads)
 }
 
 std::vector<Ciphertext> HEMMer::clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared) {
-    const std::vector<double> c = clipPolynomial(max_norm, bound, degree);
+    std::vector<double> c = clipPolynomial(max_norm, bound, degree);
     if (grads.empty()) throw std::invalid_argument("[clipGradNorm] no gradients");
     int level = grads[0]->getLevel();
     for (const Ciphertext *x : grads) level = std::min(level, x->getLevel());
     need_level(level, 3 + polynomialDepth(degree), "clipGradNorm");
     const Evaluator &ev = eval_;
+    // 2 / bound^2 is a whole number of units of the scale.  Below 2^20 of them the rounding would be seen: the bound is widened to where they are whole, and the polynomial is that of the wider one.
+    // With eight, the fewest, that is by up to 1/16 (at a scale of 2^42: bounds of 10^6), where the kink of a degree of 15 at bound = 4 max_norm comes out to 0.036 instead of 0.033.
+    const double unit = ev.scale(level - 1);
+    double factor_u = 2.0 / (bound * bound);
+    if (factor_u * unit < 0x1p20) {
+        const double whole = std::floor(factor_u * unit);
+        if (whole < 8.0) throw std::invalid_argument("[clipGradNorm] the bound is too large for the scale: 2 / bound^2 has less than eight units of it");
+        factor_u = whole / unit;
+        c = clipPolynomial(max_norm, std::sqrt(2.0 / factor_u), degree);
+    }
     Ciphertext square = gradNormSquared(grads);
-    const Ciphertext u = ev.rescale(ev.combine({&square}, {2.0 / (bound * bound)}, -1.0));
+    const Ciphertext u = ev.rescale(ev.combine({&square}, {factor_u}, -1.0));
     const Ciphertext factor = evaluate(eval_, u, c);
     std::vector<Ciphertext> low;
     for (const Ciphertext *x : grads) low.push_back(down(ev, *x, factor.getLevel()));

@@ -164,7 +164,9 @@ int hb_hemmer_layer_norm_backward(hb_hemmer *h, const hb_ct *dy, const hb_ct *xh
                                   hb_ct **dgamma, hb_ct **dbeta);
 /* The square of the global norm of the gradients, over all slots of all members of all handles (imaginary parts have to be zero), in every slot, one level below the lowest of them; and all of
  * them times min(1, max_norm / norm): a polynomial of `degree` in the square of the norm, right up to norms of `bound` > max_norm, which a degree of 15 meets to 0.05 for bound = 4 max_norm.  3 levels and those of the
- * polynomial; outs receives a handle per gradient, norm_squared (may be NULL) the square.  Beyond `bound` the polynomial is no root and soon grows beyond all bounds: decrypted, norm_squared tells. */
+ * polynomial; outs receives a handle per gradient, norm_squared (may be NULL) the square.  Beyond `bound` the polynomial is no root and soon grows beyond all bounds: decrypted, norm_squared tells.
+ * 2 / bound^2 is a whole number at the scale (2^42): from a bound of 2048 on the bound is widened to where it is one, by up to 1/16 at 10^6; larger ones are refused, as are
+ * those below 2^-9, whose number has more than 62 bits. */
 int hb_hemmer_grad_norm_squared(hb_hemmer *h, const hb_ct *const *grads, int count, hb_ct **out);
 int hb_hemmer_clip_grad_norm(hb_hemmer *h, const hb_ct *const *grads, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared);
 /* Those polynomials: which = 0 for 1 / sqrt over [a, b], 1 for min(1, a / sqrt) over [0, b^2], as degree + 1 coefficients of T_j(u), u the place of the argument in [-1, 1].  depth (may be NULL):
