@@ -202,11 +202,17 @@ HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns
     const bool scaled = gamma || n.pad; // columns past the width come out as zeros
     need_level(x.getLevel(), 4 + polynomialDepth(degree) + (scaled ? 1 : 0), "layerNorm");
     const Evaluator &ev = eval_;
-    const Ciphertext mean = row_mean(*this, ev.sumGroups(x.get(), groups), n.s, 1.0 / (double)columns);
+    // Masks hold 1 / columns and 2 / ((hi - lo) columns), and where a wide range leaves the second few units of the scale, its rounding is seen in the variance: 13 units in a sum of 32 columns, 100 in one of 256.
+    // So mean and squares are those of x / 2^k, which the way down of x to the mean's level takes with it: the second factor grows by 4^k, until it has 2^24 units or as many as the first is left with.
+    const double unit = ev.scale(x.getLevel() - 2);
+    double shrink = 1.0, mean_scale = 1.0 / (double)columns, scale = 2.0 / ((hi - lo) * (double)columns);
+    while (scale * unit < 0x1p24 && scale < mean_scale) { shrink *= 0.5; mean_scale *= 0.5; scale *= 4.0; }
+    if (!(scale * unit >= 0x1p16)) throw std::invalid_argument("[layerNorm] the range is too wide for the scale");
+    const Ciphertext mean = row_mean(*this, ev.sumGroups(x.get(), groups), n.s, mean_scale);
+    auto resized = [&](const Ciphertext &y, double by) { return ev.rescale(ev.combine({&y}, {by})); }; // one level lower
     Ciphertext u;
     {
-        const double scale = 2.0 / ((hi - lo) * (double)columns);
-        Ciphertext squares = ev.normSquares(down(ev, x.get(), mean.getLevel()), &mean, groups, 0), row;
+        Ciphertext squares = ev.normSquares(shrink == 1.0 ? down(ev, x.get(), mean.getLevel()) : resized(x.get(), shrink), &mean, groups, 0), row;
         if (n.pad) { // columns past the width hold zeros, whose differences are the mean: their squares are taken off the sum over the row
             std::vector<Ciphertext> both;
             both.push_back(std::move(squares)); both.push_back(ev.normSquares(mean, nullptr, 1, 0));
@@ -227,7 +233,7 @@ HEMMer::LayerNorm HEMMer::layerNorm(const CtxtTensor &x, int groups, i64 columns
     }
     Ciphertext rstd = evaluate(eval_, u, c);
     const int level = rstd.getLevel();
-    const Ciphertext low_mean = down(ev, mean, level);
+    const Ciphertext low_mean = shrink == 1.0 ? down(ev, mean, level) : down(ev, resized(mean, 1.0 / shrink), level);
     Ciphertext xhat = switched(ev, ev.normScale(down(ev, x.get(), level), &low_mean, rstd, groups));
     Ciphertext y;
     if (scaled) {
