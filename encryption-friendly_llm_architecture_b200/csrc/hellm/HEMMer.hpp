@@ -160,8 +160,10 @@ class HEMMer {
     LayerNormGrads layerNormBackward(const CtxtTensor &dy, const CtxtTensor &xhat, const CtxtTensor &rstd, int groups, i64 columns, const double *gamma);
     // The square of the norm over all slots of all members of all gradients, in every slot; and the gradients times min(1, max_norm / norm), a polynomial of `degree` in the square, right up to a
     // norm of `bound`.  Takes 3 + polynomialDepth(degree) levels of the lowest gradient.
-    Ciphertext gradNormSquared(const std::vector<const Ciphertext *> &grads);
-    std::vector<Ciphertext> clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared = nullptr);
+    // `periods`: for every gradient the slots (a power of two) after which its values repeat, so that each counts once; empty, or all slots: they do not.  dgamma and dbeta of layerNormBackward
+    // repeat after the block width.
+    Ciphertext gradNormSquared(const std::vector<const Ciphertext *> &grads, const std::vector<i64> &periods = {});
+    std::vector<Ciphertext> clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared = nullptr, const std::vector<i64> &periods = {});
     // their polynomials, as coefficients of T_j(u) with u the place of the argument in [-1, 1]: 1 / sqrt over [lo, hi], min(1, max_norm / sqrt) over [0, bound^2]
     static std::vector<double> inverseRootPolynomial(double lo, double hi, int degree);
     static std::vector<double> clipPolynomial(double max_norm, double bound, int degree);

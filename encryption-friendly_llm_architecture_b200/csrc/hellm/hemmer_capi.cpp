@@ -270,19 +270,23 @@ struct BorrowList {
     }
 };
 }
-int hb_hemmer_grad_norm_squared(hb_hemmer *h, const hb_ct *const *grads, int count, hb_ct **out) {
+int hb_hemmer_grad_norm_squared(hb_hemmer *h, const hb_ct *const *grads, int count, hb_ct **out) { return hb_hemmer_grad_norm_squared_periodic(h, grads, nullptr, count, out); }
+int hb_hemmer_grad_norm_squared_periodic(hb_hemmer *h, const hb_ct *const *grads, const int32_t *periods, int count, hb_ct **out) {
     return guard([&] {
         if (!out) throw std::invalid_argument("[gradNormSquared] null argument");
         BorrowList g(h->ctx, grads, count, "gradNormSquared");
-        *out = h->h.gradNormSquared(g.p).release();
+        *out = h->h.gradNormSquared(g.p, periods ? std::vector<i64>(periods, periods + count) : std::vector<i64>()).release();
     });
 }
 int hb_hemmer_clip_grad_norm(hb_hemmer *h, const hb_ct *const *grads, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared) {
+    return hb_hemmer_clip_grad_norm_periodic(h, grads, nullptr, count, max_norm, bound, degree, outs, norm_squared);
+}
+int hb_hemmer_clip_grad_norm_periodic(hb_hemmer *h, const hb_ct *const *grads, const int32_t *periods, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared) {
     return guard([&] {
         if (!outs) throw std::invalid_argument("[clipGradNorm] null argument");
         BorrowList g(h->ctx, grads, count, "clipGradNorm");
         Ciphertext square;
-        std::vector<Ciphertext> r = h->h.clipGradNorm(g.p, max_norm, bound, degree, &square);
+        std::vector<Ciphertext> r = h->h.clipGradNorm(g.p, max_norm, bound, degree, &square, periods ? std::vector<i64>(periods, periods + count) : std::vector<i64>());
         for (size_t k = 0; k < r.size(); ++k) outs[k] = r[k].release();
         if (norm_squared) *norm_squared = square.release();
     });

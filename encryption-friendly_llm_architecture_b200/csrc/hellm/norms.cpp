@@ -5,6 +5,7 @@
 
 #include <cmath>
 #include <cstring>
+#include <functional>
 
 namespace HELLM {
 
@@ -282,28 +283,48 @@ HEMMer::LayerNormGrads HEMMer::layerNormBackward(const CtxtTensor &dy, const Ctx
 }
 
 namespace {
-// all of the lowest level among them
-std::vector<Ciphertext> same_level(const Evaluator &ev, const std::vector<const Ciphertext *> &v) {
+int lowest_level(const std::vector<const Ciphertext *> &v) {
     int level = v[0]->getLevel();
     for (const Ciphertext *x : v) level = std::min(level, x->getLevel());
-    std::vector<Ciphertext> r;
-    for (const Ciphertext *x : v) r.push_back(down(ev, *x, level));
-    return r;
+    return level;
+}
+void need_periods(const std::vector<i64> &periods, size_t count, i64 slots, const char *what) {
+    if (periods.empty()) return;
+    if (periods.size() != count) throw std::invalid_argument(std::string("[") + what + "] a period for every gradient");
+    for (const i64 p : periods)
+        if (p < 1 || p > slots || (p & (p - 1))) throw std::invalid_argument(std::string("[") + what + "] periods are powers of two up to the slots");
 }
 }
 
-Ciphertext HEMMer::gradNormSquared(const std::vector<const Ciphertext *> &grads) {
+// A sum of squares with period p is the same after a sum over p slots as any other after one over all of them.  So the sums over the slots go from the longest period to the next, where the squares
+// of that period come in, and so on: as many rotations as without periods.
+Ciphertext HEMMer::gradNormSquared(const std::vector<const Ciphertext *> &grads, const std::vector<i64> &periods) {
     if (grads.empty()) throw std::invalid_argument("[gradNormSquared] no gradients");
-    const std::vector<Ciphertext> g = same_level(eval_, grads);
-    need_level(g[0].getLevel(), 1, "gradNormSquared");
-    return sum_slots(*this, switched(eval_, eval_.squareSumMany(g)), 1);
+    need_periods(periods, grads.size(), slots_, "gradNormSquared");
+    const Evaluator &ev = eval_;
+    const int level = lowest_level(grads);
+    need_level(level, 1, "gradNormSquared");
+    std::map<i64, std::vector<Ciphertext>, std::greater<i64>> by_period;
+    for (size_t k = 0; k < grads.size(); ++k) by_period[periods.empty() ? slots_ : periods[k]].push_back(down(ev, *grads[k], level));
+    std::vector<Ciphertext> sums;
+    for (const auto &g : by_period) sums.push_back(ev.squareSumMany(g.second));
+    const int kinds = (int)sums.size();
+    Ciphertext squares = kinds == 1 ? switched(ev, sums[0]) : switched(ev, ev.concat(sums));
+    Ciphertext sum;
+    int k = 0;
+    for (auto g = by_period.begin(); g != by_period.end(); ++k) {
+        const i64 period = g->first, next = ++g == by_period.end() ? 1 : g->first;
+        Ciphertext own = kinds == 1 ? std::move(squares) : ev.group(squares, k, kinds); // a view of several comes back from the sum as a ciphertext of its own, since another period follows
+        sum = sum_rotations(ev, k ? ev.add(sum, own) : std::move(own), next, period / next);
+    }
+    return sum;
 }
 
-std::vector<Ciphertext> HEMMer::clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared) {
+std::vector<Ciphertext> HEMMer::clipGradNorm(const std::vector<const Ciphertext *> &grads, double max_norm, double bound, int degree, Ciphertext *norm_squared, const std::vector<i64> &periods) {
     std::vector<double> c = clipPolynomial(max_norm, bound, degree);
     if (grads.empty()) throw std::invalid_argument("[clipGradNorm] no gradients");
-    int level = grads[0]->getLevel();
-    for (const Ciphertext *x : grads) level = std::min(level, x->getLevel());
+    need_periods(periods, grads.size(), slots_, "clipGradNorm");
+    const int level = lowest_level(grads);
     need_level(level, 3 + polynomialDepth(degree), "clipGradNorm");
     const Evaluator &ev = eval_;
     // 2 / bound^2 is a whole number of units of the scale.  Below 2^20 of them the rounding would be seen: the bound is widened to where they are whole, and the polynomial is that of the wider one.
@@ -316,7 +337,7 @@ std::vector<Ciphertext> HEMMer::clipGradNorm(const std::vector<const Ciphertext 
         factor_u = whole / unit;
         c = clipPolynomial(max_norm, std::sqrt(2.0 / factor_u), degree);
     }
-    Ciphertext square = gradNormSquared(grads);
+    Ciphertext square = gradNormSquared(grads, periods);
     const Ciphertext u = ev.rescale(ev.combine({&square}, {factor_u}, -1.0));
     const Ciphertext factor = evaluate(eval_, u, c);
     std::vector<Ciphertext> low;

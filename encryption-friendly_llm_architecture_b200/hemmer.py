@@ -410,15 +410,24 @@ class Hemmer:
         outs = self._call("layer_norm_backward", dy.ct.ptr, xhat.ct.ptr, rstd.ct.ptr, *self._shp(dy), _i32(groups), _i32(columns), pg, n_out=3)
         return tuple(CtxtTensor(o, *dy.shape) for o in outs)
 
-    def grad_norm_squared(self, grads):
-        """The square of the global norm of all gradients, in every slot."""
-        arr = (C.c_void_p * len(grads))(*[g.ct.ptr.value for g in grads])
-        return self._call("grad_norm_squared", arr, _i32(len(grads)))
+    def _periods(self, periods, count):
+        if periods is None:
+            return None
+        if len(periods) != count:
+            raise ValueError(f"{count} gradients, {len(periods)} periods")
+        return (C.c_int32 * count)(*[_i32(self.lib.slots if p is None else p) for p in periods])
 
-    def clip_grad_norm(self, grads, max_norm, bound, degree=15):
-        """(gradients times min(1, max_norm / norm), square of the norm); right up to norms of `bound`."""
+    def grad_norm_squared(self, grads, periods=None):
+        """The square of the global norm of all gradients, in every slot.  periods: for every gradient the slots after which its values repeat (None: they do not), so that each counts once:
+        the width of dgamma and dbeta, which stand in every row."""
+        arr = (C.c_void_p * len(grads))(*[g.ct.ptr.value for g in grads])
+        return self._call("grad_norm_squared_periodic", arr, self._periods(periods, len(grads)), _i32(len(grads)))
+
+    def clip_grad_norm(self, grads, max_norm, bound, degree=15, periods=None):
+        """(gradients times min(1, max_norm / norm), square of the norm); right up to norms of `bound`.  periods: as for grad_norm_squared."""
+        periods = self._periods(periods, len(grads))
         arr, outs, square = (C.c_void_p * len(grads))(*[g.ct.ptr.value for g in grads]), (C.c_void_p * len(grads))(), C.c_void_p()
-        rc = self._fn("clip_grad_norm")(self.h, arr, _i32(len(grads)), C.c_double(max_norm), C.c_double(bound), _i32(degree), outs, C.byref(square))
+        rc = self._fn("clip_grad_norm_periodic")(self.h, arr, periods, _i32(len(grads)), C.c_double(max_norm), C.c_double(bound), _i32(degree), outs, C.byref(square))
         if rc != 0:
             f = self._fn("last_error")
             f.restype = C.c_char_p

@@ -169,6 +169,10 @@ int hb_hemmer_layer_norm_backward(hb_hemmer *h, const hb_ct *dy, const hb_ct *xh
  * those below 2^-9, whose number has more than 62 bits. */
 int hb_hemmer_grad_norm_squared(hb_hemmer *h, const hb_ct *const *grads, int count, hb_ct **out);
 int hb_hemmer_clip_grad_norm(hb_hemmer *h, const hb_ct *const *grads, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared);
+/* Those count every slot: a gradient that holds its values several times, as dgamma and dbeta of hb_hemmer_layer_norm_backward do in every row, counts as many times.  With `periods`, a power of two
+ * for every gradient (the block width for dgamma and dbeta, the number of slots for those that do not repeat), values count once; what is said to repeat has to.  NULL: none does. */
+int hb_hemmer_grad_norm_squared_periodic(hb_hemmer *h, const hb_ct *const *grads, const int32_t *periods, int count, hb_ct **out);
+int hb_hemmer_clip_grad_norm_periodic(hb_hemmer *h, const hb_ct *const *grads, const int32_t *periods, int count, double max_norm, double bound, int degree, hb_ct **outs, hb_ct **norm_squared);
 /* Those polynomials: which = 0 for 1 / sqrt over [a, b], 1 for min(1, a / sqrt) over [0, b^2], as degree + 1 coefficients of T_j(u), u the place of the argument in [-1, 1].  depth (may be NULL):
  * levels of its evaluation.  Needs no device. */
 int hb_hemmer_polynomial(int which, double a, double b, int degree, double *coefficients, int *depth);
