@@ -161,6 +161,12 @@ class Lib:
         self._chk(self._fn("encode")(self.ctx, _f64(re), _f64(im), C.c_size_t(re.size), C.c_int(level), C.byref(out)))
         return Handle(self, out, "pt")
 
+    def encode_mask(self, value, step, width, level):
+        """`value` in the first `width` of every `step` slots, made on the device."""
+        out = C.c_void_p()
+        self._chk(self._fn("encode_mask")(self.ctx, C.c_double(value), _i32(step), _i32(width), _i32(level), C.byref(out)))
+        return Handle(self, out, "pt")
+
     def encode_ext(self, z, level):
         """encode() with K further limbs modulo the special primes: the plaintext operand of assemble_rot."""
         z = np.asarray(z)

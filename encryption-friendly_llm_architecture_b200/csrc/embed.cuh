@@ -59,6 +59,12 @@ template <int TOP> __device__ __forceinline__ void fwd_round(double2 (&v)[16], c
 // x86 semantics of a conversion to 64 bits: everything that does not fit becomes the most negative value
 __device__ __forceinline__ i64 to_i64(double rounded) { return fabs(rounded) < 0x1p63 ? (i64)rounded : (i64)0x8000000000000000ull; }
 
+// slots re [n] of a mask: `value` where the slot's number modulo `step` (a power of two) is below `width`, 0 elsewhere.  grid = (n / 256)
+__global__ void __launch_bounds__(256) k_mask_slots(double *re, double value, int step, int width, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    pdl_wait();
+    if (i < n) re[i] = (i & (step - 1)) < width ? value : 0.0;
+}
 constexpr int kEmbThreads = 128;
 // messages re / im [count][n] (im may be null, slots from n on are zero) -> half-transformed slots v [count][2^15].  grid = (16, count)
 __global__ void __launch_bounds__(kEmbThreads) k_embed_inv_cols(double2 *v, const double *re, const double *im, int n, EmbedTables tb) {

@@ -126,6 +126,8 @@ class Evaluator {
     Plaintext encode(const Message &m, int level) const {
         hb_pt *p = nullptr; check(c_, hb_encode(c_, m.re.data(), m.im.data(), m.size(), level, &p)); return Plaintext(p);
     }
+    // `value` in the first `width` of every `step` slots, without a copy from the host
+    Plaintext encodeMask(double value, int step, int width, int level) const { hb_pt *p = nullptr; check(c_, hb_encode_mask(c_, value, step, width, level, &p)); return Plaintext(p); }
     Plaintext encodeExtended(const Message &m, int level) const {
         hb_pt *p = nullptr; check(c_, hb_encode_ext(c_, m.re.data(), m.im.data(), m.size(), level, &p)); return Plaintext(p);
     }

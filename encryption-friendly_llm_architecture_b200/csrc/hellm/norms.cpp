@@ -21,21 +21,20 @@ Plaintext columns_plaintext(const HEMMer &h, const TileTensorShape &s, const dou
     return h.eval().encode(m, level);
 }
 // Masks that depend on a number: the number's bits are part of their key.  They stay, since recorded graphs hold their addresses, and so there are kNormMasks of a kind at most:
-// a program with more (another range of variances at every step) encodes the others at every call.
+// a program with more (another range of variances at every step) makes the others at every call, on the device, so that it can be recorded too.
 constexpr size_t kNormMasks = 64;
 Plaintext norm_mask(HEMMer &h, int kind, const TileTensorShape &s, double value, int level) {
     i64 bits;
     std::memcpy(&bits, &value, 8);
     const MaskCache::Key k{kind, s, bits, level};
     if (const Plaintext *p = h.masks().find(k)) return *p;
-    Plaintext p;
-    if (kind == sched::kNormColumns) p = columns_plaintext(h, s, nullptr, (i64)value, level);
-    else {
-        Message m((size_t)h.slots());
-        for (i64 r = 0; r < s.getNumRows(); ++r) m.re[(size_t)(r * s.getBlockWidth())] = value;
-        p = h.eval().encode(m, level);
-    }
-    return h.masks().count(kind) < kNormMasks ? h.masks().put(k, p) : p;
+    const bool columns = kind == sched::kNormColumns; // ones in as many columns; otherwise the value in the first column.  Rows fill the slots (norm_shape)
+    const int step = (int)s.getBlockWidth();
+    if (h.masks().count(kind) >= kNormMasks) return h.eval().encodeMask(columns ? 1.0 : value, step, columns ? (int)value : 1, level);
+    if (columns) return h.masks().put(k, columns_plaintext(h, s, nullptr, (i64)value, level));
+    Message m((size_t)h.slots());
+    for (i64 r = 0; r < s.getNumRows(); ++r) m.re[(size_t)(r * step)] = value;
+    return h.masks().put(k, h.eval().encode(m, level)); // not while a graph records, when the mask would hold nothing until its replay
 }
 Ciphertext switched(const Evaluator &ev, const Ciphertext &x) { return ev.rescale(ev.relinearize(x)); }
 // x at a lower level, or a view of x, which has to outlive it; a temporary is moved

@@ -1517,7 +1517,7 @@ void host_copy(const hb_ctx *c, double *dst, const double *src, size_t words) {
 void embed_inverse(hb_ctx *c, i64 *coef, const double *re, const double *im, int n, int count, double sc) {
     if (c->logn == 16) {
         Tmp v(c, (size_t)count);
-        LAUNCH(c), k_embed_inv_cols<<<dim3(16, (unsigned)count), kEmbThreads, 0, c->st>>>((double2 *)v.p, re, im, n, c->emb_tb); // comes after a copy, not after a kernel
+        LAUNCH(c), k_embed_inv_cols<<<dim3(16, (unsigned)count), kEmbThreads, 0, c->st>>>((double2 *)v.p, re, im, n, c->emb_tb); // mostly after a copy, not after a kernel
         CK(cudaPeekAtLastError());
         launch(c, k_embed_inv_rows, dim3(16, (unsigned)count), kEmbThreads, 0, coef, (const double2 *)v.p, sc, c->emb_tb);
     } else {
@@ -1948,6 +1948,24 @@ int hb_encode(hb_ctx *c, const double *re, const double *im, size_t n, int level
         if (level < 0 || level > c->L) fail(HB_E_LEVEL, "encode: bad level");
         hb_pt *p = new_pt(c, level, 1);
         encode_into(c, p, re, im, n, c->qmap(level));
+        *out = p;
+    });
+}
+int hb_encode_mask(hb_ctx *c, double value, int step, int width, int level, hb_pt **out) {
+    return guard(c, [&] {
+        const int slots = c->h->slots;
+        if (!out || !std::isfinite(value)) fail(HB_E_ARG, "encode_mask: a finite value, and room for the result");
+        if (step < 1 || step > slots || (step & (step - 1)) || width < 0 || width > step) fail(HB_E_ARG, "encode_mask: a step that is a power of two up to the slots, and a width up to the step");
+        if (level < 0 || level > c->L) fail(HB_E_LEVEL, "encode_mask: bad level");
+        hb_pt *p = new_pt(c, level, 1);
+        try {
+            TmpBytes re(c, (size_t)slots * sizeof(double)), coef(c, (size_t)c->N * sizeof(i64));
+            launch(c, k_mask_slots, dim3((unsigned)(slots + 255) / 256), 256, 0, (double *)re.p, value, step, width, slots);
+            embed_inverse(c, (i64 *)coef.p, (const double *)re.p, nullptr, slots, 1, c->h->scale[level]);
+            const LimbMap map = c->qmap(level);
+            message_residues(c, p->d, (const i64 *)coef.p, 1, map);
+            ntt_inplace(c, p->d, map.n, map, false);
+        } catch (...) { hb_pt_free(p); throw; }
         *out = p;
     });
 }

@@ -96,6 +96,9 @@ uint64_t hb_galois_for_rotation(const hb_ctx *ctx, int64_t left_steps);
 /* EnDecoder::encode / decode -- EnDecoder.hpp:51,66.  im may be NULL (real message). */
 int hb_encode(hb_ctx *ctx, const double *re, const double *im, size_t n_slots, int level, hb_pt **out);
 int hb_decode(hb_ctx *ctx, const hb_pt *pt, double *re, double *im);
+/* hb_encode of a mask, made on the device: `value` in the slots whose number modulo `step` (a power of two) is below `width`, 0 in the others.
+ * Bit for bit hb_encode of those slot values.  Nothing is copied from the host, so the call can be recorded.  No counterpart in the reference. */
+int hb_encode_mask(hb_ctx *ctx, double value, int step, int width, int level, hb_pt **out);
 /* hb_encode with K further limbs modulo the special primes after the level + 1 usual ones: the plaintext operand of
  * hb_assemble_rot.  Usable wherever a plaintext of that level is.  No counterpart in the reference. */
 int hb_encode_ext(hb_ctx *ctx, const double *re, const double *im, size_t n_slots, int level, hb_pt **out);

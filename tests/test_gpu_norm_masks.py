@@ -66,3 +66,33 @@ def test_the_same_as_in_a_cache_with_room(pkg, full_cache):
     for a, b in zip(h.layer_norm(cx, D, span, groups=2, degree=3), fresh.layer_norm(cx, D, span, groups=2, degree=3)):
         assert np.array_equal(h.lib.ct_export(a.ct), h.lib.ct_export(b.ct))
     fresh.close()
+
+
+@pytest.mark.parametrize("ring", ["gpu_small", "gpu_mid", "gpu_full"])
+def test_masks_made_on_the_device(ring, request):
+    """Bit for bit hb_encode of the same slots, again and again, recorded or not."""
+    g = request.getfixturevalue(ring)
+    for value, step, width, level in [(1.0, 32, 32, 3), (1.0 / 768, 256, 1, 8), (-0.3, 64, 23, 0), (2.5e-7, 2, 1, 5), (1e6, g.slots, 7, 2), (3.0, 1, 1, 1), (1.0, 16, 0, 4), (1e-30, 16, 3, 1)]:
+        z = np.where(np.arange(g.slots) % step < width, value, 0.0)
+        want = g.pt_export(g.encode(z, level))
+        for _ in range(3):
+            assert np.array_equal(g.pt_export(g.encode_mask(value, step, width, level)), want)
+        g.graph_begin()
+        pt = g.encode_mask(value, step, width, level)
+        graph = g.graph_end()
+        for _ in range(2):
+            g.graph_launch(graph)
+            assert np.array_equal(g.pt_export(pt), want)
+
+
+def test_masks_that_are_refused(pkg, gpu_small):
+    g = gpu_small
+    for value, step, width, level in [(float("nan"), 16, 1, 1), (float("inf"), 16, 1, 1), (1.0, 0, 0, 1), (1.0, 24, 1, 1), (1.0, -16, 1, 1), (1.0, 2 * g.slots, 1, 1), (1.0, 16, 17, 1), (1.0, 16, -1, 1)]:
+        with pytest.raises(pkg.HBError) as e:
+            g.encode_mask(value, step, width, level)
+        assert e.value.code == -1
+    for level in (-1, g.L + 1):
+        with pytest.raises(pkg.HBError):
+            g.encode_mask(1.0, 16, 1, level)
+    with pytest.raises(ValueError):
+        g.encode_mask(1.0, 2 ** 32, 1, 1)
