@@ -126,6 +126,7 @@ struct hb_ctx {
     unsigned gx() const { return (unsigned)((N + 256 * kElems - 1) / (256 * kElems)); } // blocks per limb of the element-wise kernels
     dim3 egrid(int count) const { return dim3(gx(), (unsigned)count); }
     u64 *alloc_limbs(size_t limbs) { return (u64 *)pool.get(limbs * (size_t)N * 8); }
+    u64 *lasting_limbs(size_t limbs) { return (u64 *)pool.lasting(limbs * (size_t)N * 8); }
     u64 *spare_limbs(size_t limbs) { return (u64 *)pool.spare(limbs * (size_t)N * 8); }
 };
 
@@ -157,7 +158,7 @@ hb_ct *new_ct(hb_ctx *c, int level, int np, int batch, int spow) {
 }
 hb_pt *new_pt(hb_ctx *c, int level, int spow) {
     hb_pt *x = new hb_pt{c, level, spow, nullptr};
-    try { x->d = c->alloc_limbs((size_t)level + 1); } catch (...) { delete x; throw; }
+    try { x->d = c->lasting_limbs((size_t)level + 1); } catch (...) { delete x; throw; }
     return x;
 }
 struct Tmp { // pool buffer released at scope exit
@@ -640,7 +641,7 @@ Evk make_key(hb_ctx *c, u64 kid, u32 g) {
     no_capture(c, "key generation");
     const HostCtx &h = *c->h;
     const int N = c->N, np = c->nprimes, nd = h.digit_of(h.L) + 1;
-    Evk k; k.nd = nd; k.d = c->alloc_limbs((size_t)nd * 2 * np);
+    Evk k; k.nd = nd; k.d = c->lasting_limbs((size_t)nd * 2 * np);
     try {
         const LimbMap am = c->allmap();
         Tmp e(c, (size_t)nd * np);
@@ -1977,7 +1978,7 @@ int hb_encode_ext(hb_ctx *c, const double *re, const double *im, size_t n, int l
         const int ne = level + 1 + c->K;
         hb_pt *p = new hb_pt{c, level, 1, nullptr};
         p->ext = 1;
-        try { p->d = c->alloc_limbs((size_t)ne); } catch (...) { delete p; throw; }
+        try { p->d = c->lasting_limbs((size_t)ne); } catch (...) { delete p; throw; }
         LimbMap em{}; em.n = ne;
         for (int j = 0; j < ne; ++j) em.prime[j] = (unsigned char)(j <= level ? j : c->L + 1 + (j - level - 1));
         encode_into(c, p, re, im, n, em);
@@ -1992,7 +1993,7 @@ int hb_qweight_create(hb_ctx *c, const uint8_t *codes, const float *scales, int 
         const size_t bytes = ((size_t)rows + 1) / 2 * cols, at = (bytes + 3) & ~(size_t)3, words = (((size_t)rows - 1) / group + 1) * cols;
         for (size_t k = 0; k < words; ++k) if (!std::isfinite(scales[k])) fail(HB_E_ARG, "qweight: a scale is not finite");
         std::unique_ptr<hb_qweight> w(new hb_qweight{c, {}, nullptr});
-        w->d = (unsigned char *)c->pool.get(at + words * 4);
+        w->d = (unsigned char *)c->pool.lasting(at + words * 4);
         w->w = Weights4{w->d, (const float *)(w->d + at), rows, cols, group};
         try {
             CK(cudaMemcpyAsync(w->d, codes, bytes, cudaMemcpyHostToDevice, c->st));
@@ -2416,8 +2417,8 @@ int hb_masked_key_create(hb_ctx *c, int64_t steps, const hb_pt *m1, const hb_pt 
         const PlanDims d = plan_dims(c, level);
         hb_mkey *k = new hb_mkey{c, level, (u32)g, nullptr, nullptr};
         try {
-            k->key = c->alloc_limbs((size_t)d.nd * 2 * d.ne);
-            k->pm = c->alloc_limbs((size_t)d.n);
+            k->key = c->lasting_limbs((size_t)d.nd * 2 * d.ne);
+            k->pm = c->lasting_limbs((size_t)d.n);
             LAUNCH(c), k_mask_key<<<dim3(c->gx(), d.ne, d.nd * 2), 256, 0, c->st>>>(k->key, key.d, c->nprimes, m1->d, m2 ? m2->d : nullptr, pl, c->pc, N);
             LAUNCH(c), k_mask_p<<<dim3(c->gx(), d.n), 256, 0, c->st>>>(k->pm, m1->d, m2 ? m2->d : nullptr, dv, c->pc, N);
             CK(cudaGetLastError());
@@ -2933,7 +2934,7 @@ int hb_pt_load(hb_ctx *c, const char *path, hb_pt **out) {
         if ((int)h.level > c->L || limbs * c->N != host.size()) fail(HB_E_ARG, std::string(path) + ": size does not match its header");
         hb_pt *r = new hb_pt{c, (int)h.level, (int)h.scale_pow, nullptr};
         r->ext = h.ext ? 1 : 0;
-        try { r->d = c->alloc_limbs(limbs); upload(c, r->d, host); } catch (...) { if (r->d) c->pool.put(r->d); delete r; throw; }
+        try { r->d = c->lasting_limbs(limbs); upload(c, r->d, host); } catch (...) { if (r->d) c->pool.put(r->d); delete r; throw; }
         *out = r;
     });
 }
@@ -2966,7 +2967,7 @@ int hb_keys_load(hb_ctx *c, const char *dir, const uint64_t *galois, int count) 
             const int nd = c->h->digit_of(c->h->L) + 1;
             const size_t limbs = (size_t)nd * 2 * c->nprimes;
             if ((int)h.digits != nd || h.galois != g || w.size() != limbs * c->N) fail(HB_E_ARG, path + ": does not fit this context");
-            Evk k; k.nd = nd; k.d = c->alloc_limbs(limbs);
+            Evk k; k.nd = nd; k.d = c->lasting_limbs(limbs);
             try { upload(c, k.d, w); } catch (...) { c->pool.put(k.d); throw; }
             return k;
         };

@@ -5,6 +5,7 @@
 
 #include <cuda_runtime_api.h>
 
+#include <cstddef>
 #include <string>
 #include <unordered_map>
 #include <unordered_set>
@@ -33,6 +34,21 @@ struct Pool {
         bytes = (bytes + 255) & ~(size_t)255;
         void *p = idle(bytes);
         if (!p) { p = raw(bytes); total += bytes; }
+        return hand_out(p, bytes);
+    }
+    // A buffer for what stays while graphs come and go (plaintexts, keys): not one that a recorded graph writes to at every replay.  Made while a graph records it is that graph's, as any other.
+    void *lasting(size_t bytes) {
+        if (recording) return get(bytes);
+        bytes = (bytes + 255) & ~(size_t)255;
+        auto &v = free_[bytes];
+        for (size_t k = v.size(); k-- > 0;) {
+            void *p = v[k];
+            if (held_.count(p)) continue;
+            v.erase(v.begin() + (std::ptrdiff_t)k);
+            return hand_out(p, bytes);
+        }
+        void *p = raw(bytes);
+        total += bytes;
         return hand_out(p, bytes);
     }
     // A buffer that the caller can do without: an idle one or what the driver has left; null otherwise, and no idle buffer goes back to the driver for it.
