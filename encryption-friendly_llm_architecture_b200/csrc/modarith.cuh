@@ -177,8 +177,9 @@ __device__ __forceinline__ u64 canon_fp64(double v, double q_inv, double qd) {
 
 // ---- exact sums of a few such products -------------------------------------------------------------------------
 // h collects the products rounded to multiples of 2^40 (it starts at 1.5 * 2^92, whose ulp that is), l the remainders: four FP64
-// instructions per product instead of seven, one quotient for the sum.  a, w >= 0, or a within 0.6 q of zero (ks_rows); the products must add up to less than 2^91 in magnitude:
-// 2^7 of them for primes below 2^42, eight below 2^44.
+// instructions per product instead of seven, one quotient for the sum.  a and w are whole numbers of either sign (residues, their negatives, differences of two) below q in magnitude; the products must
+// add up to less than 2^91 in magnitude: 2^7 of them for primes below 2^42, eight below 2^44.  Then h stays between 2^92 and 2^93, so its ulp is 2^40 throughout and the difference of two of its values
+// is exact, and what each product leaves is at most 2^39: 2^7 of those add up exactly in l.
 constexpr double kGrid40 = 1.5 * 0x1p92;
 struct FpAcc {
     double h, l;

@@ -117,7 +117,7 @@ struct OutList {
 // parts, which have a chunk of one, are joined in shared memory, in order.  Words come through a ring of members, which every thread fills for itself: of a token tile the mean first, then the members.
 // Level 5, us (floor: the bytes at the copy bandwidth): 3 tiles of 4 token tiles 24 (21), of 16 85 (85), 8 of 16 162 (162), 102 members of a list 97 (100).  Words straight to registers, four
 // members ahead, two CTAs an SM: 31, 107, 188 and 103; rings of five and six stages and two CTAs, which let the sums of two members go without moves: 25.0 and 25.1, 88 and 86, 165 and 162, 99 and 97; four
-// CTAs of 64 registers, which spill: 35, 111, 223 and 196.
+// CTAs of 64 registers, which spill: 35, 111, 223 and 196.  The third CTA costs the sums with a mean 12 bytes of spills.
 // grid = (N splits / 512, n, chunks): quotients by sizes would take a fifth of the instructions
 struct SquareShape { int groups, batch, chunk, log_splits; u64 pad; };
 constexpr int kSquareStages = 4;
@@ -335,7 +335,10 @@ __global__ void __launch_bounds__(256, 4) k_affine(u64 *out, const u64 *x, const
 // all but the first tiles of a call).  The words come through a ring of members in shared memory, which every thread fills for itself, several members ahead.  SAME: g is dy.
 // Level 5, us (floor): 3 tiles of 4 token tiles 55 (51), of 16 195 (184), 8 of 16 478 to 498 (427), with g = dy 43 (40), 145 (138), 362 (304).  Sums over b as two words (h, l) a sum, registers for the words
 // ahead: 61, 210 and 943 (spills); as one word, reduced at every product: 57, 201 and 561; with the ring 55, 195 and 480.  Tiles in teams of 128 threads that join their rows in shared memory
-// behind a barrier a token tile: 579 for 8 of 16.  Stages and CTAs an SM by tiles: eight stages of 8 tiles 476, six 490, four 482; 6 tiles four stages and four CTAs 119, six and three 130.
+// behind a barrier a token tile: 579 for 8 of 16.  Stages and CTAs an SM by tiles: eight stages of 8 tiles 476, six 490, four 482; 6 tiles of 4 token tiles four stages and four CTAs 119, six and three 130.
+// All tiles of 16 token tiles with four to eight stages and three to five CTAs: what is below is the best of them or within 2 %, but for 5 tiles (322; eight stages and three CTAs 313) and 6 (392; six and three 378, and
+// with g = dy 277 and 264).  One tile wants four stages (91, six 108, and with g = dy eight 88 instead of 76); at five CTAs 4 tiles and more lose (6 tiles 426 to 480, 8 633 to 711), at four 8 tiles do (509).
+// Without g = dy the 60-bit limb's sums spill 32, 108 and 156 bytes with 4, 5 and 6 tiles at four CTAs, which three CTAs do not make faster at 4 (249 against 253).
 // grid = (N / 128, n)
 struct GradShape { int batch, tile0; };
 constexpr int grad_stages(int TT) { return TT == 1 || TT == 6 ? 4 : TT == 8 ? 8 : 6; }

@@ -154,10 +154,14 @@ int hb_hemmer_matvec_q4(hb_hemmer *h, const hb_ct *x, const hb_qweight *w, hb_ct
 /* Layer norm and its gradients over rows that reach across `groups` column tiles (members [column tile][token tile], tiles whose rows fill the slots); `columns`
  * in all, the last tile may end early.  gamma, beta: `columns` doubles on the host, or NULL.  y = xhat gamma + beta with xhat = (x - mean) rstd; rstd is the polynomial of `degree`
  * (1 to 63) that stands for 1 / sqrt(variance + eps) on [lo, hi].  x needs 4 levels, those of the polynomial (hb_hemmer_polynomial), and one for gamma or a tile that
- * ends early.  hi - lo may be as wide as values are large: x is shrunk by a power of two on its way (at most to where the masks of the row sums keep 16 bits, else refused).  Outside [lo, hi] the polynomial soon grows beyond all bounds, and a slot beyond the modulus spoils all of them, so rows of padding
- * (all zeros) have to be named: `tokens` has the number of rows in front of them for every token tile (NULL: all rows), and they come out as beta.  Columns past the width have to be zero in x and dy and come out as zeros in y, dx, dgamma and dbeta;
- * in xhat they are not.  dy may be of another level than xhat; dgamma and dbeta have one member per column tile, summed over all rows and token tiles, in every row.  Plaintexts are encoded from
- * the host at every call that has gamma, beta or padding, which cannot be recorded then.  No counterparts in the reference's HEMMer: its LayerNorm class does the like with other polynomials. */
+ * ends early.  hi - lo may be as wide as values are large: x is shrunk by a power of two on its way (at most to where the masks of the row sums keep 16 bits, else refused).
+ * Outside [lo, hi] the polynomial soon grows beyond all bounds, and a slot beyond the modulus spoils all of them, so rows of padding (all zeros) have to be named: `tokens` has the
+ * number of rows in front of them for every token tile (NULL: all rows), and they come out as beta.  Columns past the width have to be zero in x and dy and come out as zeros in y, dx,
+ * dgamma and dbeta; in xhat they are not.  Rows of padding have to be zero in dy, or dbeta counts them.
+ * The gradients need xhat at level 4 (5 where a tile ends early) and rstd at 1 (2); dy may be of another level than xhat, but is multiplied by gamma first, which takes one of its own.  So
+ * in a ring of 12 levels forward passes of degrees up to 14 keep what they need (up to 6 where a tile ends early); with higher ones xhat ends too low, and the framework has no
+ * bootstrapping to refresh it.  dgamma and dbeta have one member per column tile, summed over all rows and token tiles, in every row.  Plaintexts are encoded from the host at every call that has
+ * gamma, beta or padding, which cannot be recorded then.  No counterparts in the reference's HEMMer: its LayerNorm class does the like with other polynomials. */
 int hb_hemmer_layer_norm(hb_hemmer *h, const hb_ct *x, int rows, int cols, int width, int groups, int columns, const double *gamma, const double *beta, double eps, double lo, double hi, int degree,
                          const int32_t *tokens, hb_ct **y, hb_ct **xhat, hb_ct **rstd);
 int hb_hemmer_layer_norm_backward(hb_hemmer *h, const hb_ct *dy, const hb_ct *xhat, const hb_ct *rstd, int rows, int cols, int width, int groups, int columns, const double *gamma, hb_ct **dx,

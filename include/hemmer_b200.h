@@ -296,7 +296,8 @@ int hb_tensor_acc_cross(hb_ctx *ctx, const hb_ct *a, const hb_ct *b, int groups,
  * of batch(x) / groups token tiles each; all operands of a call are rescaled pairs of one level.  (x): tensor product; m, r, mean and dot
  * have one member per token tile.  What has three polynomials, or a factor, comes back un-relinearised and un-rescaled (scale power 2).
  *   hb_norm_squares     out[b] = sum_t (x[t][b] - m[b]) (x) (x[t][b] - m[b]) - pad m[b] (x) m[b].  mean NULL: the sum of x (x) x.  pad (0 to the slots, only beside
- *                       a mean): members of the sum that are there to fill it up, all zeros, so that each adds m (x) m, which is taken off
+ *                       a mean): members of the sum that are there to fill it up, all zeros, so that each adds m (x) m, which is taken off.  Not for columns past a
+ *                       width, whose differences are the mean in their own slots alone: those are taken off the sum over the row (hb_hemmer_layer_norm)
  *   hb_norm_scale       out[t][b] = (x[t][b] - m[b]) (x) r[b], or (x) r[t][b] when the factor has as many members as x.  mean NULL: x (x) r
  *   hb_norm_affine      out[t][b] = x[t][b] (.) gamma[t] + K beta[t], K the level's scale as a whole number, so that both terms have the scale of
  *                       a product; beta NULL: none.  gamma NULL: out = x + beta[t], not multiplied and so with x's own scale.  `groups` plaintexts each, of x's level
