@@ -36,3 +36,34 @@ def test_bounds_that_are_refused(pkg, deep, bound):  # noqa: F811
     assert e.value.code == -1 and "bound" in str(e.value)
     outs, _ = h.clip_grad_norm([x], 10.0, 40.0, 3)   # and the handle goes on working
     assert h.lib.ct_meta(outs[0].ct)[1] == 2
+
+
+@pytest.mark.parametrize("bound,sizes", [(4.0, [1] * 30), (1e5, [3, 1, 40, 2]), (1e6, [1])])
+def test_recorded(deep, bound, sizes):  # noqa: F811
+    """Clipping many handles as a graph, replayed on other gradients and again on the first."""
+    h = deep
+
+    def gradients(seed):
+        rng = np.random.default_rng(seed)
+        xs = [rng.normal(0, 1, (1, m, 16, 32)) for m in sizes]
+        size = np.sqrt(sum((x ** 2).sum() for x in xs))
+        return [_encrypt(h, x * (0.2 + 0.3 * seed) * bound / size, seed=10 * seed + k) for k, x in enumerate(xs)]
+
+    first, other = gradients(1), gradients(2)
+    periods = [512] * len(sizes)
+
+    def run(grads):
+        outs, square = h.clip_grad_norm(grads, bound / 4, bound, 7, periods=periods)
+        return [*[o.ct for o in outs], square]
+
+    want = [[h.lib.ct_export(o) for o in run(grads)] for grads in (first, other)]
+    held = [h.lib.ct_export(x.ct) for x in first]
+    h.lib.graph_begin()
+    outs = run(first)
+    graph = h.lib.graph_end()
+    for words, res in ((None, want[0]), ([h.lib.ct_export(x.ct) for x in other], want[1]), (held, want[0])):
+        for x, v in zip(first, words or ()):
+            h.lib.ct_import(x.ct, v)
+        h.lib.graph_launch(graph)
+        for o, v in zip(outs, res):
+            assert np.array_equal(h.lib.ct_export(o), v)

@@ -56,3 +56,21 @@ def test_the_full_ring(pkg, gpu_full):
     assert h.lib.ct_meta(y.ct)[0] == h.lib.L - 4 - depth
     assert np.abs(_whole(_decrypt(h, y, T, B), D) - y0).max() < TOL and np.abs(_decrypt(h, rstd, 1, B)[0] / r0 - 1).max() < TOL
     h.close()
+
+
+def test_recorded(deep):  # noqa: F811
+    """A layer norm in a wide range, whose x is shrunk, as a graph on other values."""
+    h, T, B, D, w, rows, size = deep, 2, 1, 60, 32, 16, 1e3
+    xs = [_data(np.random.default_rng(k), B, rows, D) * size for k in range(2)]
+    span = (0.1 * size ** 2, 1.3 * size ** 2)
+    c, _ = h.polynomial("rsqrt", *span, 3)
+    cx, other = (_encrypt(h, _tiles(x, T, w), seed=k) for k, x in enumerate(xs))
+    h.layer_norm(cx, D, span, groups=T, degree=3)
+    h.lib.graph_begin()
+    y, xhat, rstd = h.layer_norm(cx, D, span, groups=T, degree=3)
+    graph = h.lib.graph_end()
+    h.lib.graph_launch(graph)
+    assert np.abs(_whole(_decrypt(h, y, T, B), D) - _model(xs[0], 1.0, 0.0, 1e-5, span, c)[0]).max() < TOL
+    h.lib.ct_import(cx.ct, h.lib.ct_export(other.ct))
+    h.lib.graph_launch(graph)
+    assert np.abs(_whole(_decrypt(h, y, T, B), D) - _model(xs[1], 1.0, 0.0, 1e-5, span, c)[0]).max() < TOL
